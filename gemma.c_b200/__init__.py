@@ -111,6 +111,30 @@ class LayerStepArgs(ctypes.Structure):
     ]
 
 
+class ChunkArgs(ctypes.Structure):
+    """B200KvChunkArgs: runs of new tokens (append, attention over the cache, write)."""
+
+    _fields_ = [
+        ("q", c_void_p), ("k_rows", c_void_p), ("v_rows", c_void_p),
+        ("out", c_void_p), ("lse", c_void_p),
+        ("cache_k", c_void_p), ("cache_v", c_void_p),
+        ("cache_config", KvConfig),
+        ("page_table", c_void_p),
+        ("seq_batch", c_void_p), ("first_position", c_void_p),
+        ("row_count", c_void_p), ("row_start", c_void_p),
+        ("raw_q", c_void_p), ("raw_k", c_void_p), ("raw_v", c_void_p),
+        ("q_norm_weight", c_void_p), ("k_norm_weight", c_void_p),
+        ("cos", c_void_p), ("sin", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("status", c_void_p),
+        ("run_count", c_int32), ("max_row_count", c_int32), ("rows", c_int32),
+        ("cache_layer", c_int32), ("q_heads", c_int32),
+        ("window_size", c_int32), ("sink_tokens", c_int32),
+        ("rotary_dim", c_int32), ("norm_mode", c_int32),
+        ("softmax_scale", c_float),
+    ]
+
+
 class IngressArgs(ctypes.Structure):
     """B200KvIngressArgs: input RMSNorm + [Q|K|V] projection
     (src/gemma4_flash_attention_decode.cu:447-496)."""
@@ -202,6 +226,19 @@ _SIGNATURES = {
     "b200kv_layer_step_launches": (c_int32, [POINTER(LayerStepArgs)]),
     "b200kv_decode_attention_tiled_bf16": (c_int, [_P, _P, _P, _P, _P, KvConfig, _P, _P, c_int32, c_float, c_int32,
                                                   c_int32, c_int32, _P, _P, _P, _P, _P, _P]),
+    "b200kv_chunk_append_bf16": (c_int, [POINTER(ChunkArgs), _P]),
+    "b200kv_chunk_attention_bf16": (c_int, [POINTER(ChunkArgs), _P]),
+    "b200kv_chunk_workspace_bytes": (c_size_t, [c_int32] * 6),
+    "b200kv_chunk_write_bf16": (c_int, [POINTER(ChunkArgs), _P]),
+    "b200kv_chunk_layer_step_bf16": (c_int, [POINTER(ChunkArgs), _P]),
+    "b200kv_pages_ensure": (c_int32, [_P, _P, POINTER(KvConfig), c_int32, c_int32, c_int32, _P, _P, _P, c_int32,
+                                      POINTER(c_int32)]),
+    "b200kv_pages_fork": (c_int32, [_P, _P, POINTER(KvConfig), c_int32, c_int32, c_int32]),
+    "b200kv_pages_release": (c_int32, [_P, _P, POINTER(KvConfig), c_int32, c_int32, c_int32]),
+    "b200kv_pages_compact": (c_int32, [_P, _P, POINTER(KvConfig), _P, _P, _P, c_int32, POINTER(c_int32),
+                                       POINTER(c_int32)]),
+    "b200kv_copy_pages_bf16": (c_int, [_P, _P, KvConfig, _P, _P, _P, c_int32, _P]),
+    "b200kv_copy_pages_fp8": (c_int, [_P, _P, _P, _P, KvConfig, _P, _P, _P, c_int32, _P]),
     "b200kv_decode_ingress_bf16": (c_int, [POINTER(IngressArgs), _P]),
     "b200kv_decode_egress_bf16": (c_int, [POINTER(EgressArgs), _P]),
     "b200kv_decode_attention_layer_bf16": (c_int, [POINTER(AttentionLayerArgs), _P]),
@@ -566,6 +603,101 @@ def decode_step_plan(layers, layer_count: int, forwarded: bool = False):
            True)
     out = (list(held)[:layer_count], [bool(x) for x in list(early)[:layer_count]])
     return out + (list(fwd)[:layer_count],) if forwarded else out
+
+
+# ------------------------------------------------------------------ chunks of new tokens over the cache
+def chunk_append(args: ChunkArgs, stream=None, check: bool = True) -> int:
+    """Norm + rotation of the runs' rows; K and V into the pages, or to args.k_rows / v_rows when those are set."""
+    code = load_library().b200kv_chunk_append_bf16(ctypes.byref(args), _stream(stream))
+    return _check(code, "b200kv_chunk_append_bf16", check)
+
+
+def chunk_attention(args: ChunkArgs, stream=None, check: bool = True) -> int:
+    """Attention of the runs' rows over their sequences' cached keys (and their own rows)."""
+    code = load_library().b200kv_chunk_attention_bf16(ctypes.byref(args), _stream(stream))
+    return _check(code, "b200kv_chunk_attention_bf16", check)
+
+
+def chunk_write(args: ChunkArgs, stream=None, check: bool = True) -> int:
+    code = load_library().b200kv_chunk_write_bf16(ctypes.byref(args), _stream(stream))
+    return _check(code, "b200kv_chunk_write_bf16", check)
+
+
+def chunk_layer_step(args: ChunkArgs, stream=None, check: bool = True) -> int:
+    """chunk_append, chunk_attention and, with k_rows / v_rows, chunk_write."""
+    code = load_library().b200kv_chunk_layer_step_bf16(ctypes.byref(args), _stream(stream))
+    return _check(code, "b200kv_chunk_layer_step_bf16", check)
+
+
+def chunk_workspace_bytes(q_heads: int, kv_heads: int, head_dim: int, run_count: int, max_row_count: int,
+                          sm_count: Optional[int] = None) -> int:
+    """Bytes of ChunkArgs.workspace; sm_count defaults to the current device's."""
+    if sm_count is None:
+        import torch
+
+        sm_count = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
+    return int(load_library().b200kv_chunk_workspace_bytes(q_heads, kv_heads, head_dim, run_count, max_row_count,
+                                                           sm_count))
+
+
+# ------------------------------------------------------------------ pages: sharing, copying, giving back
+class PageCopies:
+    """The page copies the host functions below record for copy_pages: host arrays of `capacity` entries."""
+
+    def __init__(self, capacity: int):
+        self.capacity = capacity
+        self.src, self.dst, self.rows = (np.zeros(max(capacity, 1), dtype=np.int32) for _ in range(3))
+        self._count = c_int32(0)
+
+    @property
+    def count(self) -> int:
+        return self._count.value
+
+    def clear(self):
+        self._count.value = 0
+
+
+def pages_ensure(page_table: np.ndarray, ref_count: np.ndarray, cfg: KvConfig, batch: int, first: int, count: int,
+                 copies: PageCopies) -> int:
+    return int(load_library().b200kv_pages_ensure(
+        _ptr(page_table), _ptr(ref_count), ctypes.byref(cfg), batch, first, count, _ptr(copies.src),
+        _ptr(copies.dst), _ptr(copies.rows), copies.capacity, ctypes.byref(copies._count)))
+
+
+def pages_fork(page_table: np.ndarray, ref_count: np.ndarray, cfg: KvConfig, src: int, dst: int, length: int) -> int:
+    return int(load_library().b200kv_pages_fork(_ptr(page_table), _ptr(ref_count), ctypes.byref(cfg), src, dst,
+                                                length))
+
+
+def pages_release(page_table: np.ndarray, ref_count: np.ndarray, cfg: KvConfig, batch: int, first_slot: int,
+                  slot_count: int) -> int:
+    return int(load_library().b200kv_pages_release(_ptr(page_table), _ptr(ref_count), ctypes.byref(cfg), batch,
+                                                   first_slot, slot_count))
+
+
+def pages_compact(page_table: np.ndarray, ref_count: np.ndarray, cfg: KvConfig, copies: PageCopies):
+    """(0 or -1, pages in use)."""
+    used = c_int32(0)
+    code = load_library().b200kv_pages_compact(
+        _ptr(page_table), _ptr(ref_count), ctypes.byref(cfg), _ptr(copies.src), _ptr(copies.dst), _ptr(copies.rows),
+        copies.capacity, ctypes.byref(copies._count), ctypes.byref(used))
+    return int(code), used.value
+
+
+def copy_pages(cache_k, cache_v, cfg: KvConfig, src_page, dst_page, row_count, count: int, stream=None,
+               check: bool = True) -> int:
+    """Pages src_page[i] -> dst_page[i] in every layer, K and V (row_count: only their first rows; None: all)."""
+    code = load_library().b200kv_copy_pages_bf16(_ptr(cache_k), _ptr(cache_v), cfg, _ptr(src_page), _ptr(dst_page),
+                                                 _ptr(row_count), count, _stream(stream))
+    return _check(code, "b200kv_copy_pages_bf16", check)
+
+
+def copy_pages_fp8(cache_k, cache_v, scale_k, scale_v, cfg: KvConfig, src_page, dst_page, row_count, count: int,
+                   stream=None, check: bool = True) -> int:
+    code = load_library().b200kv_copy_pages_fp8(_ptr(cache_k), _ptr(cache_v), _ptr(scale_k), _ptr(scale_v), cfg,
+                                                _ptr(src_page), _ptr(dst_page), _ptr(row_count), count,
+                                                _stream(stream))
+    return _check(code, "b200kv_copy_pages_fp8", check)
 
 
 def decode_ingress(args: IngressArgs, stream=None, check: bool = True) -> int:

@@ -12,6 +12,7 @@
 // One warp owns one head; lane l holds elements l + 32*i (the reference's
 // ownership), the sum of squares is an fma chain per lane followed by the xor
 // butterfly 16,8,4,2,1 -- that order defines the bit pattern of the scale.
+#include "chunk_common.cuh"
 #include "kernels.cuh"
 #include "prep_common.cuh"
 
@@ -169,12 +170,12 @@ __device__ __forceinline__ float rms_scale_of(float ss) {
 }
 
 // What a warp needs to know about pair `pr` of a token: kind 0 query heads, 1 K
-// heads, 2 V heads; whether the pair has a second row; where its rows lie.
+// heads, 2 V heads; its first head; whether it has a second row; where it is.
 struct PrepPair {
   int kind;
+  int h0;
   bool second;
   const __nv_bfloat16 *src;
-  __nv_bfloat16 *dst;
 };
 
 template <int D>
@@ -182,15 +183,62 @@ __device__ __forceinline__ PrepPair prep_pair_of(const PrefillPrepArgs &a, int64
                                                  int pq, int pk) {
   PrepPair p;
   p.kind = pr < pq ? 0 : (pr < pq + pk ? 1 : 2);
-  const int h0 = 2 * (p.kind == 0 ? pr : (p.kind == 1 ? pr - pq : pr - pq - pk));
-  p.second = h0 + 1 < (p.kind == 0 ? a.q_heads : a.kv_heads);
+  p.h0 = 2 * (p.kind == 0 ? pr : (p.kind == 1 ? pr - pq : pr - pq - pk));
+  p.second = p.h0 + 1 < (p.kind == 0 ? a.q_heads : a.kv_heads);
   p.src = p.kind == 0
-              ? a.q + (row * a.q_heads + h0) * D
-              : ((p.kind == 1 || a.v == nullptr ? a.k : a.v) + (row * a.kv_heads + h0) * D);
-  p.dst = p.kind == 0 ? a.q_prepared + (row * a.q_heads + h0) * D
-                      : ((p.kind == 1 ? a.k_prepared : a.v_prepared) +
-                         (row * a.kv_heads + h0) * D);
+              ? a.q + (row * a.q_heads + p.h0) * D
+              : ((p.kind == 1 || a.v == nullptr ? a.k : a.v) + (row * a.kv_heads + p.h0) * D);
   return p;
+}
+
+// Where a token's results go and its position (negative: nowhere). A prompt's
+// K and V rows lie in row order; a chunk's lie there or in the page of their
+// position (nullptr: not stored).
+struct PrepRow {
+  int position;
+  __nv_bfloat16 *k;
+  __nv_bfloat16 *v;
+};
+template <int D>
+__device__ __forceinline__ PrepRow prep_row_of(const PrefillPrepArgs &a, int64_t row) {
+  return {__ldg(a.token_position + row), a.k_prepared + row * a.kv_heads * D,
+          a.v_prepared + row * a.kv_heads * D};
+}
+// The run that names the row: every lane looks at its share of the runs (one
+// round of loads for up to 32 of them).
+template <int D>
+__device__ __forceinline__ PrepRow prep_row_of(const ChunkPrepArgs &a, int64_t row) {
+  const ChunkRuns &runs = a.runs;
+  const int lane = int(threadIdx.x) & 31;
+  ChunkRun run;
+  bool found = false;
+  for (int base = 0; base < runs.run_count && !found; base += 32) {
+    const ChunkRun mine = chunk_run(runs, base + lane, a.cfg.batch_size);
+    const uint32_t hit =
+        __ballot_sync(0xffffffffu, row >= mine.start && row < int64_t(mine.start) + mine.count);
+    if (hit != 0) {
+      const int from = __ffs(int(hit)) - 1;
+      run.start = __shfl_sync(0xffffffffu, mine.start, from);
+      run.count = __shfl_sync(0xffffffffu, mine.count, from);
+      run.first = __shfl_sync(0xffffffffu, mine.first, from);
+      run.batch = __shfl_sync(0xffffffffu, mine.batch, from);
+      found = true;
+    }
+  }
+  PrepRow r = {-1, nullptr, nullptr};
+  if (!found) return r;
+  r.position = run.first + int(row - run.start);
+  if (a.k_prepared != nullptr) {
+    r.k = a.k_prepared + row * a.kv_heads * D;
+    r.v = a.v_prepared + row * a.kv_heads * D;
+  } else {
+    const int64_t at = chunk_store_offset(a.cfg, a.page_table, a.layer, run, r.position);
+    if (at >= 0) {
+      r.k = a.cache_k + at;
+      r.v = a.cache_v + at;
+    }
+  }
+  return r;
 }
 
 // Up to 8 warps of two pairs each, four CTAs per SM: the kernel lives on loads in
@@ -199,8 +247,10 @@ __device__ __forceinline__ PrepPair prep_pair_of(const PrefillPrepArgs &a, int64
 // soon as the current one is in shared memory.
 constexpr int kPrepWarps = 8;
 
-template <int D, int ROT, bool kIeee>
-__global__ __launch_bounds__(kPrepWarps * 32, D == 256 ? 4 : 2) void prefill_prep_kernel(PrefillPrepArgs a) {
+// Args: PrefillPrepArgs (a prompt's rows) or ChunkPrepArgs (runs of rows, K and V
+// into the cache: they then cross HBM once each way instead of twice).
+template <int D, int ROT, bool kIeee, class Args>
+__global__ __launch_bounds__(kPrepWarps * 32, D == 256 ? 4 : 2) void prefill_prep_kernel(Args a) {
   constexpr int E = D / 32;          // elements per lane and row
   constexpr int kVecs = D / 8 / 32;  // 128-bit packs per lane and row
   constexpr int kPairs = ROT / 64;   // rotated (lo, hi) element pairs per lane
@@ -227,7 +277,8 @@ __global__ __launch_bounds__(kPrepWarps * 32, D == 256 ? 4 : 2) void prefill_pre
   };
   PrepPair cur = prep_pair_of<D>(a, row, warp, pq, pk);
   fetch(cur);
-  const int position = __ldg(a.token_position + row);
+  const PrepRow to = prep_row_of<D>(a, row);
+  const int position = to.position;
   if (position < 0) return;
 
   // RoPE factors of the token for this lane's rotated elements
@@ -318,16 +369,22 @@ __global__ __launch_bounds__(kPrepWarps * 32, D == 256 ? 4 : 2) void prefill_pre
     }
     __syncwarp();
     // 4. de-interleave and out
+    __nv_bfloat16 *dst = now.kind == 0 ? a.q_prepared + (row * a.q_heads + now.h0) * D
+                                       : (now.kind == 1 ? to.k : to.v);
+    if (now.kind != 0 && dst != nullptr) dst += now.h0 * D;
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
+      if constexpr (std::is_same_v<Args, ChunkPrepArgs>) {
+        if (dst == nullptr) break;
+      }
       const int pv = lane + 32 * v;
       const uint4 w0 = reinterpret_cast<const uint4 *>(mine)[pv];
       const uint4 w1 = reinterpret_cast<const uint4 *>(mine + L::kRegion)[pv];
-      reinterpret_cast<uint4 *>(now.dst)[pv] =
+      reinterpret_cast<uint4 *>(dst)[pv] =
           make_uint4(prmt(w0.x, w0.y, 0x5410u), prmt(w0.z, w0.w, 0x5410u),
                      prmt(w1.x, w1.y, 0x5410u), prmt(w1.z, w1.w, 0x5410u));
       if (now.second) {
-        reinterpret_cast<uint4 *>(now.dst + D)[pv] =
+        reinterpret_cast<uint4 *>(dst + D)[pv] =
             make_uint4(prmt(w0.x, w0.y, 0x7632u), prmt(w0.z, w0.w, 0x7632u),
                        prmt(w1.x, w1.y, 0x7632u), prmt(w1.z, w1.w, 0x7632u));
       }
@@ -466,10 +523,104 @@ cudaError_t prefill_prep_bf16(const PrefillPrepArgs &a, cudaStream_t stream) {
   return dispatch_geometry(
       a.head_dim, a.rotary_dim, a.norm_mode, [&](auto d, auto rot, auto ieee) {
         prefill_prep_kernel<decltype(d)::value, decltype(rot)::value,
-                            decltype(ieee)::value>
+                            decltype(ieee)::value, PrefillPrepArgs>
             <<<unsigned(a.rows), warps * 32, 0, stream>>>(a);
         return cudaGetLastError();
       });
+}
+
+// Checks of the append's and the write's arguments that do not need the device.
+cudaError_t validate_chunk_append(const ChunkPrepArgs &a) {
+  const Gemma4KvCacheConfig &c = a.cfg;
+  const bool to_rows = a.k_prepared != nullptr;
+  if (!valid_chunk_runs(a.runs) || a.q_prepared == nullptr || a.q == nullptr ||
+      a.k == nullptr || a.q_norm_weight == nullptr || a.k_norm_weight == nullptr ||
+      a.cos == nullptr || a.sin == nullptr || a.q_heads <= 0 || c.num_heads <= 0 ||
+      c.batch_size <= 0 || a.q_heads % c.num_heads != 0 ||
+      (a.k_prepared == nullptr) != (a.v_prepared == nullptr) ||
+      !((c.head_dim == 256 && a.rotary_dim == 256) ||
+        (c.head_dim == 512 && a.rotary_dim == 128)) ||
+      (a.norm_mode != B200KV_NORM_IEEE && a.norm_mode != B200KV_NORM_RSQRT_APPROX)) {
+    return cudaErrorInvalidValue;
+  }
+  if (!to_rows && (!valid_cache_config(c, a.layer) || a.cache_k == nullptr ||
+                   a.cache_v == nullptr || a.page_table == nullptr)) {
+    return cudaErrorInvalidValue;
+  }
+  const uintptr_t align =
+      reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) |
+      reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.q_prepared) |
+      reinterpret_cast<uintptr_t>(a.k_prepared) | reinterpret_cast<uintptr_t>(a.v_prepared) |
+      (to_rows ? 0 : reinterpret_cast<uintptr_t>(a.cache_k) | reinterpret_cast<uintptr_t>(a.cache_v));
+  return (align & 15u) == 0 ? cudaSuccess : cudaErrorInvalidValue;  // rows move as 128-bit packs
+}
+
+cudaError_t chunk_append_bf16(const ChunkPrepArgs &a, cudaStream_t stream) {
+  const cudaError_t valid = validate_chunk_append(a);
+  if (valid != cudaSuccess) return valid;
+  if (a.runs.run_count == 0 || a.runs.rows == 0) return cudaSuccess;
+  const int pairs = (a.q_heads + 1) / 2 + 2 * ((a.kv_heads + 1) / 2);
+  const int warps = std::max(1, std::min(kPrepWarps, (pairs + 1) / 2));
+  return dispatch_geometry(
+      a.cfg.head_dim, a.rotary_dim, a.norm_mode, [&](auto d, auto rot, auto ieee) {
+        prefill_prep_kernel<decltype(d)::value, decltype(rot)::value,
+                            decltype(ieee)::value, ChunkPrepArgs>
+            <<<unsigned(a.runs.rows), warps * 32, 0, stream>>>(a);
+        return cudaGetLastError();
+      });
+}
+
+namespace {
+// Prepared rows of the runs into the cache: a CTA per (row of a run, run), the
+// row's heads are contiguous in both places.
+__global__ __launch_bounds__(256) void chunk_write_kernel(
+    __nv_bfloat16 *cache_k, __nv_bfloat16 *cache_v, Gemma4KvCacheConfig c,
+    ChunkRuns runs, const int32_t *page_table, int32_t layer,
+    const __nv_bfloat16 *k, const __nv_bfloat16 *v) {
+  const ChunkRun run = chunk_run(runs, int(blockIdx.y), c.batch_size);
+  const int r = int(blockIdx.x);
+  if (r >= run.count) return;
+  const int64_t at = chunk_store_offset(c, page_table, layer, run, run.first + r);
+  if (at < 0) return;
+  const int vecs = c.num_heads * c.head_dim / 8;
+  const uint4 *src_k = reinterpret_cast<const uint4 *>(k) + int64_t(run.start + r) * vecs;
+  const uint4 *src_v = reinterpret_cast<const uint4 *>(v) + int64_t(run.start + r) * vecs;
+  uint4 *dst_k = reinterpret_cast<uint4 *>(cache_k + at);
+  uint4 *dst_v = reinterpret_cast<uint4 *>(cache_v + at);
+  for (int i = int(threadIdx.x); i < vecs; i += int(blockDim.x)) {
+    const uint4 kk = __ldg(src_k + i);
+    const uint4 vv = __ldg(src_v + i);
+    dst_k[i] = kk;
+    dst_v[i] = vv;
+  }
+}
+}  // namespace
+
+cudaError_t validate_chunk_write(const ChunkPrepArgs &a) {
+  const Gemma4KvCacheConfig &c = a.cfg;
+  if (!valid_chunk_runs(a.runs) || !valid_cache_config(c, a.layer) ||
+      a.cache_k == nullptr || a.cache_v == nullptr || a.page_table == nullptr ||
+      a.k_prepared == nullptr || a.v_prepared == nullptr ||
+      (int64_t(c.num_heads) * c.head_dim) % 8 != 0) {
+    return cudaErrorInvalidValue;
+  }
+  const uintptr_t align = reinterpret_cast<uintptr_t>(a.k_prepared) |
+                          reinterpret_cast<uintptr_t>(a.v_prepared) |
+                          reinterpret_cast<uintptr_t>(a.cache_k) |
+                          reinterpret_cast<uintptr_t>(a.cache_v);
+  return (align & 15u) == 0 ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t chunk_write_bf16(const ChunkPrepArgs &a, cudaStream_t stream) {
+  const cudaError_t valid = validate_chunk_write(a);
+  if (valid != cudaSuccess) return valid;
+  if (a.runs.run_count == 0 || a.runs.rows == 0) return cudaSuccess;
+  const int vecs = a.cfg.num_heads * a.cfg.head_dim / 8;
+  const int threads = vecs >= 256 ? 256 : ((vecs + 31) / 32) * 32;
+  chunk_write_kernel<<<dim3(unsigned(a.runs.max_row_count), unsigned(a.runs.run_count)), threads,
+                       0, stream>>>(a.cache_k, a.cache_v, a.cfg, a.runs, a.page_table, a.layer,
+                                    a.k_prepared, a.v_prepared);
+  return cudaGetLastError();
 }
 
 namespace {

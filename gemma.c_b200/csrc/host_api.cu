@@ -1260,6 +1260,132 @@ int b200kv_decode_step_plan(const B200KvLayerStepArgs *layers, int32_t layer_cou
   return cudaSuccess;
 }
 
+// ---------------------------------------------------------------------------
+// Runs of new tokens
+// ---------------------------------------------------------------------------
+namespace {
+b200kv::ChunkRuns chunk_runs(const B200KvChunkArgs *s) {
+  b200kv::ChunkRuns r;
+  r.seq_batch = s->seq_batch;
+  r.first_position = s->first_position;
+  r.row_count = s->row_count;
+  r.row_start = s->row_start;
+  r.run_count = s->run_count;
+  r.max_row_count = s->max_row_count;
+  r.rows = s->rows;
+  return r;
+}
+
+b200kv::ChunkPrepArgs chunk_prep_args(const B200KvChunkArgs *s) {
+  using bf = __nv_bfloat16;
+  b200kv::ChunkPrepArgs a;
+  a.q_prepared = reinterpret_cast<bf *>(s->q);
+  a.k_prepared = reinterpret_cast<bf *>(s->k_rows);
+  a.v_prepared = reinterpret_cast<bf *>(s->v_rows);
+  a.q = reinterpret_cast<const bf *>(s->raw_q);
+  a.k = reinterpret_cast<const bf *>(s->raw_k);
+  a.v = reinterpret_cast<const bf *>(s->raw_v);
+  a.q_norm_weight = reinterpret_cast<const bf *>(s->q_norm_weight);
+  a.k_norm_weight = reinterpret_cast<const bf *>(s->k_norm_weight);
+  a.cos = s->cos;
+  a.sin = s->sin;
+  a.rows = s->rows;
+  a.q_heads = s->q_heads;
+  a.kv_heads = s->cache_config.num_heads;
+  a.head_dim = s->cache_config.head_dim;
+  a.rotary_dim = s->rotary_dim;
+  a.norm_mode = s->norm_mode;
+  a.runs = chunk_runs(s);
+  a.cache_k = reinterpret_cast<bf *>(s->cache_k);
+  a.cache_v = reinterpret_cast<bf *>(s->cache_v);
+  a.cfg = s->cache_config;
+  a.page_table = s->page_table;
+  a.layer = s->cache_layer;
+  return a;
+}
+
+b200kv::ChunkAttentionArgs chunk_attention_args(const B200KvChunkArgs *s) {
+  using bf = __nv_bfloat16;
+  b200kv::ChunkAttentionArgs a;
+  a.out = reinterpret_cast<bf *>(s->out);
+  a.lse = s->lse;
+  a.q = reinterpret_cast<const bf *>(s->q);
+  a.k_rows = reinterpret_cast<const bf *>(s->k_rows);
+  a.v_rows = reinterpret_cast<const bf *>(s->v_rows);
+  a.cache_k = reinterpret_cast<const bf *>(s->cache_k);
+  a.cache_v = reinterpret_cast<const bf *>(s->cache_v);
+  a.cfg = s->cache_config;
+  a.page_table = s->page_table;
+  a.runs = chunk_runs(s);
+  a.layer = s->cache_layer;
+  a.q_heads = s->q_heads;
+  // 0: the ring's own window
+  a.window = s->window_size != 0 ? s->window_size : s->cache_config.window_size;
+  a.sinks = s->sink_tokens;
+  a.softmax_scale = s->softmax_scale;
+  a.workspace = s->workspace;
+  a.workspace_bytes = s->workspace_bytes;
+  a.status = s->status;
+  return a;
+}
+}  // namespace
+
+int b200kv_chunk_append_bf16(const B200KvChunkArgs *s, b200kv_stream stream) {
+  if (s == nullptr) return cudaErrorInvalidValue;
+  if (s->run_count == 0) return cudaSuccess;
+  return b200kv::chunk_append_bf16(chunk_prep_args(s), static_cast<cudaStream_t>(stream));
+}
+
+int b200kv_chunk_attention_bf16(const B200KvChunkArgs *s, b200kv_stream stream) {
+  if (s == nullptr) return cudaErrorInvalidValue;
+  if (s->run_count == 0) return cudaSuccess;
+  return b200kv::chunk_attention_bf16(chunk_attention_args(s), static_cast<cudaStream_t>(stream));
+}
+
+size_t b200kv_chunk_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                    int32_t run_count, int32_t max_row_count,
+                                    int32_t sm_count) {
+  return b200kv::chunk_workspace_bytes(q_heads, kv_heads, head_dim, run_count, max_row_count,
+                                       sm_count);
+}
+
+int b200kv_chunk_write_bf16(const B200KvChunkArgs *s, b200kv_stream stream) {
+  if (s == nullptr) return cudaErrorInvalidValue;
+  if (s->run_count == 0) return cudaSuccess;
+  return b200kv::chunk_write_bf16(chunk_prep_args(s), static_cast<cudaStream_t>(stream));
+}
+
+int b200kv_chunk_layer_step_bf16(const B200KvChunkArgs *s, b200kv_stream stream) {
+  if (s == nullptr) return cudaErrorInvalidValue;
+  if (s->run_count == 0) return cudaSuccess;
+  const b200kv::ChunkPrepArgs prep = chunk_prep_args(s);
+  const b200kv::ChunkAttentionArgs attention = chunk_attention_args(s);
+  const bool write = s->k_rows != nullptr;
+  cudaStream_t on = static_cast<cudaStream_t>(stream);
+  B200KV_TRY(b200kv::validate_chunk_append(prep));
+  B200KV_TRY(b200kv::validate_chunk_attention(attention));
+  if (write) B200KV_TRY(b200kv::validate_chunk_write(prep));
+  B200KV_TRY(b200kv::chunk_append_bf16(prep, on));
+  B200KV_TRY(b200kv::chunk_attention_bf16(attention, on));
+  return write ? b200kv::chunk_write_bf16(prep, on) : cudaSuccess;
+}
+
+int b200kv_copy_pages_bf16(b200kv_bf16 *d_cache_k, b200kv_bf16 *d_cache_v,
+                           Gemma4KvCacheConfig config, const int32_t *d_src_page,
+                           const int32_t *d_dst_page, const int32_t *d_row_count,
+                           int32_t count, b200kv_stream stream) {
+  return b200kv::copy_pages(d_cache_k, d_cache_v, nullptr, nullptr, config, 2, d_src_page,
+                            d_dst_page, d_row_count, count, static_cast<cudaStream_t>(stream));
+}
+
+int b200kv_copy_pages_fp8(uint8_t *d_cache_k, uint8_t *d_cache_v, float *d_scale_k,
+                          float *d_scale_v, Gemma4KvCacheConfig config,
+                          const int32_t *d_src_page, const int32_t *d_dst_page,
+                          const int32_t *d_row_count, int32_t count, b200kv_stream stream) {
+  return b200kv::copy_pages(d_cache_k, d_cache_v, d_scale_k, d_scale_v, config, 1, d_src_page,
+                            d_dst_page, d_row_count, count, static_cast<cudaStream_t>(stream));
+}
+
 int b200kv_decode_ingress_bf16(const B200KvIngressArgs *s,
                                b200kv_stream stream) {
   if (s == nullptr) return cudaErrorInvalidValue;

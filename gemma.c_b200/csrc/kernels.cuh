@@ -282,6 +282,65 @@ cudaError_t prefill_attention_sm100_bf16(__nv_bfloat16 *out,
 // Synchronises; 0, or which wait of the last launch of that kernel ran out.
 int prefill_attention_sm100_fault();
 
+// Runs of new tokens of sequences in the cache (B200KvChunkArgs in the header).
+struct ChunkRuns {
+  const int32_t *seq_batch = nullptr;
+  const int32_t *first_position = nullptr;
+  const int32_t *row_count = nullptr;
+  const int32_t *row_start = nullptr;
+  int32_t run_count = 0;
+  int32_t max_row_count = 0;
+  int32_t rows = 0;
+};
+// Append and write of runs (append_prep.cu): the prompt prep's arguments (rows and
+// token_position unused; k_prepared / v_prepared nullptr: K and V into the cache)
+// plus where the rows go.
+struct ChunkPrepArgs : PrefillPrepArgs {
+  ChunkRuns runs;
+  __nv_bfloat16 *cache_k = nullptr;
+  __nv_bfloat16 *cache_v = nullptr;
+  Gemma4KvCacheConfig cfg = {};
+  const int32_t *page_table = nullptr;
+  int32_t layer = 0;
+};
+cudaError_t validate_chunk_append(const ChunkPrepArgs &args);
+cudaError_t chunk_append_bf16(const ChunkPrepArgs &args, cudaStream_t stream);
+cudaError_t validate_chunk_write(const ChunkPrepArgs &args);
+cudaError_t chunk_write_bf16(const ChunkPrepArgs &args, cudaStream_t stream);
+
+// Attention of runs over the paged cache (chunk_attention.cu).
+struct ChunkAttentionArgs {
+  __nv_bfloat16 *out = nullptr;
+  float *lse = nullptr;
+  const __nv_bfloat16 *q = nullptr;
+  const __nv_bfloat16 *k_rows = nullptr;  // nullptr: every key from the cache
+  const __nv_bfloat16 *v_rows = nullptr;
+  const __nv_bfloat16 *cache_k = nullptr;
+  const __nv_bfloat16 *cache_v = nullptr;
+  Gemma4KvCacheConfig cfg = {};
+  const int32_t *page_table = nullptr;
+  ChunkRuns runs;
+  int32_t layer = 0;
+  int32_t q_heads = 0;
+  int32_t window = 0;  // 0: none
+  int32_t sinks = 0;
+  float softmax_scale = 0.0f;
+  void *workspace = nullptr;
+  size_t workspace_bytes = 0;
+  int32_t *status = nullptr;
+};
+cudaError_t validate_chunk_attention(const ChunkAttentionArgs &args);
+cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &args, cudaStream_t stream);
+size_t chunk_workspace_bytes(int q_heads, int kv_heads, int head_dim, int run_count,
+                             int max_row_count, int sm_count);
+
+// Page copies in every layer (cache_pages.cu). row_bytes: a token's bytes in one
+// tensor; scales nullptr for a bf16 cache.
+cudaError_t copy_pages(void *cache_k, void *cache_v, float *scale_k, float *scale_v,
+                       Gemma4KvCacheConfig config, int element_bytes,
+                       const int32_t *src_page, const int32_t *dst_page,
+                       const int32_t *row_count, int32_t count, cudaStream_t stream);
+
 // FP8 e4m3 cache (fp8_cache.cu). args.cache_k / cache_v are unused.
 cudaError_t decode_append_fp8(const AppendArgs &args, uint8_t *cache_k,
                               uint8_t *cache_v, float *scale_k, float *scale_v,

@@ -595,6 +595,164 @@ int b200kv_decode_step_plan(const B200KvLayerStepArgs *layers, int32_t layer_cou
                             int32_t *forwarded);
 
 /* ------------------------------------------------------------------ *
+ * Chunks: runs of new tokens of sequences that may already have rows in the
+ * cache -- a piece of a long prompt, the tokens behind a shared prefix, the
+ * drafted tokens of a speculative step, one token. The reference has prompts
+ * from position 0 (src/gemma4_flash_attention.cuh:9-45) and single decode
+ * tokens (src/gemma4_flash_attention_decode.cu:613-977) and nothing between.
+ *
+ * Run i is the tokens at positions [first_position[i], + row_count[i]) of
+ * sequence seq_batch[i] (a row of the page table); its rows start at row
+ * row_start[i] of every packed [rows, heads, head_dim] tensor. max_row_count
+ * >= every row_count[i] (it sizes grids and workspace), rows is the number of
+ * rows of those tensors. A run whose sequence, position, count or rows are out
+ * of range, or with no rows, is skipped; rows that no run names are left as
+ * they were. The runs of one call must name distinct rows and distinct
+ * sequences' positions. run_count <= B200KV_MAX_RUNS.
+ *
+ * k_rows / v_rows ([rows, kv_heads, head_dim], both or neither):
+ *   NULL   the runs' K and V rows live in the cache: the append stores them
+ *          there, the attention reads every key from there. With a sliding ring
+ *          that needs a ring with room for the window and the run:
+ *          max_pages_per_seq * page_size >= window_size + max_row_count - 1,
+ *          else the attention returns cudaErrorInvalidValue.
+ *   given  the append leaves the prepared rows there and does not touch the
+ *          cache; the attention takes the keys from position first_position on
+ *          from there and only the older ones from the cache;
+ *          b200kv_chunk_write_bf16 then stores them (of a run longer than the
+ *          ring the rows that stay). The way for a ring as tight as the window,
+ *          whose old keys the run's own rows would overwrite.
+ * ------------------------------------------------------------------ */
+#define B200KV_MAX_RUNS 1024
+
+typedef struct B200KvChunkArgs {
+  b200kv_bf16 *q;                 /* prepared q [rows, q_heads, head_dim]: the
+                                     append's output, the attention's input */
+  b200kv_bf16 *k_rows, *v_rows;   /* see above */
+  b200kv_bf16 *out;               /* attention [rows, q_heads, head_dim] */
+  float *lse;                     /* optional [rows, q_heads], natural log */
+  b200kv_bf16 *cache_k, *cache_v;
+  Gemma4KvCacheConfig cache_config;
+  const int32_t *page_table;
+  const int32_t *seq_batch, *first_position, *row_count, *row_start;
+  const b200kv_bf16 *raw_q, *raw_k, *raw_v;  /* raw_v NULL: V from raw K */
+  const b200kv_bf16 *q_norm_weight, *k_norm_weight;
+  const float *cos, *sin;
+  void *workspace;                /* b200kv_chunk_workspace_bytes */
+  size_t workspace_bytes;
+  int32_t *status;                /* optional int32[4] */
+  int32_t run_count;
+  int32_t max_row_count;
+  int32_t rows;
+  int32_t cache_layer;
+  int32_t q_heads;
+  int32_t window_size;            /* see b200kv_chunk_attention_bf16 */
+  int32_t sink_tokens;
+  int32_t rotary_dim;
+  int32_t norm_mode;
+  float softmax_scale;
+} B200KvChunkArgs;
+
+/* RMSNorm and rotary embedding of every row of the runs (the arithmetic, and so
+ * the bits, of b200kv_decode_append_bf16 and b200kv_prefill_prep_bf16): q goes
+ * to `q`, the K and V rows into the pages or to k_rows / v_rows (above). A row
+ * whose page is not mapped is not stored; of a run longer than a ring only the
+ * rows that stay are. Geometries: head_dim 256 with rotary_dim 256, head_dim
+ * 512 with rotary_dim 128; any head counts. Row tensors 16-byte aligned. */
+int b200kv_chunk_append_bf16(const B200KvChunkArgs *args, b200kv_stream stream);
+
+/* Attention of every row of the runs over its sequence: the row at position t
+ * sees the keys at positions p <= t that have a page (or lie in k_rows), and
+ * with a window only p > t - window or p < sink_tokens. For a ring
+ * (cache_config.window_size > 0) the window is the ring's, window_size is 0 or
+ * the same and sink_tokens 0. For a linear cache window_size (0: none) and
+ * sink_tokens (0: none; needs a window) choose it; pages between the sinks and
+ * the first row's window may be given back (-1 in the page table). A row that
+ * sees no key gets zeros and an lse of -inf. Values at positions that no row of
+ * the call sees are not used, whatever they hold. head_dim 256 or 512, any
+ * number of query heads per KV head up to 64.
+ * `workspace` holds the partial results of rows whose keys several CTAs share;
+ * it need not be cleared and nothing is kept in it between calls; calls that may
+ * overlap on the GPU (two streams, two captured graphs) need one each. */
+int b200kv_chunk_attention_bf16(const B200KvChunkArgs *args, b200kv_stream stream);
+/* Bytes of `workspace` for these sizes on a GPU of sm_count SMs. 0 for sizes that
+ * make no sense. */
+size_t b200kv_chunk_workspace_bytes(int32_t q_heads, int32_t kv_heads,
+                                    int32_t head_dim, int32_t run_count,
+                                    int32_t max_row_count, int32_t sm_count);
+
+/* Stores k_rows / v_rows of the runs in the cache (see above). */
+int b200kv_chunk_write_bf16(const B200KvChunkArgs *args, b200kv_stream stream);
+
+/* Append, attention and (with k_rows / v_rows) write of one layer's chunk,
+ * enqueued in order on `stream`. Nothing is enqueued when any of the three would
+ * refuse its arguments. */
+int b200kv_chunk_layer_step_bf16(const B200KvChunkArgs *args, b200kv_stream stream);
+
+/* ------------------------------------------------------------------ *
+ * Pages as units: sharing, copying and giving them back. The reference maps
+ * sequence b to pages [b * width, (b + 1) * width) for good
+ * (src/gemma4_kv_cache.cu:108-146); these let sequences share a prefix and a
+ * pool. The host functions work on the caller's arrays (page table
+ * [batch_size, max_pages_per_seq], int32 reference counts [num_pages], 0 =
+ * free) and touch no device; they record the page copies the device still has
+ * to make. All return 0, or -1 with nothing changed.
+ *
+ * b200kv_pages_ensure   gives sequence `batch` writable pages for positions
+ *   [first, first + count): unmapped slots get the lowest free page; a page that
+ *   other sequences share is replaced by a fresh one, with a copy of the rows
+ *   below `first` recorded if the run starts inside it. -1: no page left, no
+ *   room in the table or the list.
+ * b200kv_pages_fork     makes sequence `dst` (whose slots must be unmapped) a
+ *   copy of the first `length` positions of `src` by sharing its pages.
+ * b200kv_pages_release  takes slots [first_slot, + slot_count) from `batch`;
+ *   a page nobody maps any more becomes free.
+ * b200kv_pages_compact  moves mapped pages down until they fill [0, *used): every
+ *   table entry that maps a moved page follows it.
+ * Copies are appended to h_copy_src / h_copy_dst (and h_copy_rows: how many rows
+ * of the page count) at *copy_count; capacity is the arrays' size. Within one
+ * list no page is both a source and a destination and none is a destination
+ * twice as long as the copies are made before the next call that records.
+ * Only linear caches (window_size 0) share pages: a ring rewrites its own.
+ * ------------------------------------------------------------------ */
+int32_t b200kv_pages_ensure(int32_t *h_page_table, int32_t *h_ref_count,
+                            const Gemma4KvCacheConfig *config, int32_t batch,
+                            int32_t first, int32_t count, int32_t *h_copy_src,
+                            int32_t *h_copy_dst, int32_t *h_copy_rows,
+                            int32_t capacity, int32_t *copy_count);
+int32_t b200kv_pages_fork(int32_t *h_page_table, int32_t *h_ref_count,
+                          const Gemma4KvCacheConfig *config, int32_t src,
+                          int32_t dst, int32_t length);
+int32_t b200kv_pages_release(int32_t *h_page_table, int32_t *h_ref_count,
+                             const Gemma4KvCacheConfig *config, int32_t batch,
+                             int32_t first_slot, int32_t slot_count);
+int32_t b200kv_pages_compact(int32_t *h_page_table, int32_t *h_ref_count,
+                             const Gemma4KvCacheConfig *config,
+                             int32_t *h_copy_src, int32_t *h_copy_dst,
+                             int32_t *h_copy_rows, int32_t capacity,
+                             int32_t *copy_count, int32_t *used);
+
+/* Copies pages inside a cache, in every layer, K and V, in one launch: for each
+ * i < count the first d_row_count[i] rows (d_row_count NULL: all) of page
+ * d_src_page[i] to page d_dst_page[i]; the rows behind them stay as they were.
+ * A pair with a page outside the cache, or with source = destination, is
+ * skipped; a row count is cut to [0, page_size]. No destination may be another
+ * pair's source or destination. Caches are 16-byte aligned, a row (num_heads x
+ * head_dim) is a multiple of 8 elements. The fp8 form takes the 8-bit cache of
+ * b200kv_decode_append_fp8 with its scales: rows are copied in its blocks of
+ * eight (a row count is rounded up), the page's scales with them
+ * (page_size % 8 == 0; a row count of 0 copies nothing). */
+int b200kv_copy_pages_bf16(b200kv_bf16 *d_cache_k, b200kv_bf16 *d_cache_v,
+                           Gemma4KvCacheConfig config, const int32_t *d_src_page,
+                           const int32_t *d_dst_page, const int32_t *d_row_count,
+                           int32_t count, b200kv_stream stream);
+int b200kv_copy_pages_fp8(uint8_t *d_cache_k, uint8_t *d_cache_v,
+                          float *d_scale_k, float *d_scale_v,
+                          Gemma4KvCacheConfig config, const int32_t *d_src_page,
+                          const int32_t *d_dst_page, const int32_t *d_row_count,
+                          int32_t count, b200kv_stream stream);
+
+/* ------------------------------------------------------------------ *
  * The steps either side of the KV path inside the reference's fused decode
  * layer, for `batch_count` rows of one token each and hidden size 3840
  * (GEMMA4_HIDDEN_SIZE, src/gemma4.h:6). Matrices are column-major as the

@@ -1,0 +1,183 @@
+"""Attention of runs of new tokens over the paged cache, against the definition in 64 bits (tests/chunk_cases.py)."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from tests.chunk_cases import check_attention, device_args, make_case
+from tests.gpu_util import need_gpu
+
+pytestmark = [pytest.mark.gpu, need_gpu]
+
+CASES = {
+    "one_token": dict(counts=[1], firsts=[37]),
+    "first_token_of_all": dict(counts=[1], firsts=[0]),
+    "four_tokens": dict(counts=[4], firsts=[500]),
+    "prompt_from_zero": dict(counts=[200], firsts=[0]),
+    "tile_edges": dict(counts=[64, 65, 63, 128, 1], firsts=[64, 63, 65, 0, 127]),
+    "ragged": dict(counts=[1, 130, 7, 33, 300], firsts=[900, 0, 255, 1000, 77], gap=3),
+    "long_keys_few_rows": dict(counts=[3, 1], firsts=[6000, 4097]),
+    "many_runs": dict(counts=[1 + i % 5 for i in range(70)], firsts=[(i * 53) % 400 for i in range(70)]),
+    "heads4": dict(counts=[40, 2], firsts=[300, 10], heads=4),
+    "heads1": dict(counts=[100, 5], firsts=[700, 2000], heads=1),
+    "group1": dict(counts=[70, 3], firsts=[130, 64], heads=4, group=1),
+    "group3": dict(counts=[50, 3], firsts=[130, 64], heads=2, group=3),
+    "group64": dict(counts=[5, 3], firsts=[130, 64], heads=1, group=64),
+    "dim512": dict(counts=[40, 1, 3], firsts=[300, 1000, 0], heads=1, group=16, dim=512, page=64),
+    "dim512_two_heads": dict(counts=[70], firsts=[90], heads=2, group=2, dim=512),
+    "dim512_ring": dict(counts=[90, 3], firsts=[300, 1000], heads=1, group=16, dim=512, ring=True, window=128),
+    "page1": dict(counts=[30, 2], firsts=[60, 100], page=1),
+    "page5": dict(counts=[70, 2], firsts=[131, 100], page=5),
+    "page8": dict(counts=[70, 2], firsts=[131, 100], page=8),
+    "page24": dict(counts=[70, 2], firsts=[131, 100], page=24),
+    "page64": dict(counts=[70, 2], firsts=[131, 1000], page=64),
+    "page200": dict(counts=[70, 2], firsts=[131, 1000], page=200),
+    "layer": dict(counts=[20], firsts=[100], layers=3, layer=1),
+    "ring_tight": dict(counts=[4, 1, 200, 30], firsts=[1500, 256, 100, 0], ring=True, window=256),
+    "ring_run_longer_than_window": dict(counts=[500, 20], firsts=[300, 64], ring=True, window=64),
+    "ring_slack": dict(counts=[16, 1, 9], firsts=[1000, 40, 64], ring=True, window=64, ring_slots=5, own_rows=False),
+    "ring_window1": dict(counts=[20, 1], firsts=[50, 0], ring=True, window=1),
+    "ring_page5": dict(counts=[40, 3], firsts=[333, 64], ring=True, window=61, page=5),
+    "own_rows_linear": dict(counts=[100, 3, 65], firsts=[333, 64, 0], own_rows=True),
+    "own_rows_page5": dict(counts=[100, 3, 65], firsts=[333, 64, 0], own_rows=True, page=5),
+    "window_linear": dict(counts=[100, 3], firsts=[333, 700], window=90),
+    "sinks": dict(counts=[1, 1, 1], firsts=[1000, 5, 70], window=64, sinks=4, free_middle=True),
+    "sinks_chunk": dict(counts=[150, 33], firsts=[700, 0], window=100, sinks=70, free_middle=True),
+    "sinks_beyond_run": dict(counts=[10], firsts=[3], window=4, sinks=200),
+    "sinks_own_rows": dict(counts=[150, 33], firsts=[700, 20], window=100, sinks=30, free_middle=True, own_rows=True),
+    "hole": dict(counts=[40], firsts=[200], unmap=[(0, 3), (0, 14)]),
+    "no_key_at_all": dict(counts=[2, 5], firsts=[14, 100], unmap=[(0, 0)]),
+    "peaked": dict(counts=[64, 3], firsts=[500, 800], q_scale=30.0),
+}
+
+
+@pytest.mark.parametrize("name", list(CASES))
+def test_attention_of_runs(kv, name):
+    case = make_case(len(name) * 7 + 1, **CASES[name])
+    a, t = device_args(kv, case)
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+
+
+def test_attention_without_lse(kv):
+    case = make_case(5, [3, 70], [100, 400])
+    a, t = device_args(kv, case, lse=False)
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+
+
+def test_runs_that_make_no_sense_are_skipped(kv):
+    case = make_case(6, [5, 6, 7, 8, 9, 10], [50, 60, 70, 80, 90, 100], gap=1)
+    case.seq[1] = 6          # not a sequence
+    case.first[2] = -1
+    case.count[3] = 0
+    case.start[4] = case.rows - 3
+    a, t = device_args(kv, case)
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+
+
+def test_pages_outside_the_cache_count_as_unmapped(kv):
+    case = make_case(7, [30], [100])
+    a, t = device_args(kv, case)
+    case.table[0, 2] = -1
+    t["page_table"][0, 2] = case.cfg[1]
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+
+
+def test_repeated_and_replayed_calls_give_the_same_bits(kv):
+    """A captured call (on its own stream, workspace of its own) and eager calls between its replays."""
+    case = make_case(8, [1, 130, 7, 300], [3000, 100, 255, 77])
+    a, t = device_args(kv, case)
+    b, tb = device_args(kv, case)
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    want, want_lse = t["out"].clone(), t["lse"].clone()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        kv.chunk_attention(b, stream=torch.cuda.current_stream())
+    for _ in range(5):
+        t["out"].fill_(0)
+        tb["out"].fill_(0)
+        graph.replay()
+        kv.chunk_attention(a)
+        torch.cuda.synchronize()
+        assert torch.equal(t["out"], want) and torch.equal(tb["out"], want)
+        assert torch.equal(t["lse"], want_lse) and torch.equal(tb["lse"], want_lse)
+    check_attention(case, t)
+
+
+def test_a_replayed_call_reads_the_lengths_of_the_moment(kv):
+    case = make_case(9, [20, 30], [500, 100])
+    a, t = device_args(kv, case)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kv.chunk_attention(a, stream=torch.cuda.current_stream())
+    case.count[:] = [3, 11]
+    case.first[:] = [480, 40]
+    t["row_count"].copy_(torch.from_numpy(case.count))
+    t["first_position"].copy_(torch.from_numpy(case.first))
+    graph.replay()
+    torch.cuda.synchronize()
+    check_attention(case, t)
+
+
+def test_cache_offsets_beyond_32_bits(kv):
+    """A cache of more than 2^32 bytes a tensor: the run's pages are its last ones."""
+    case = make_case(10, [20, 1], [200, 70], page=64)
+    a, t = device_args(kv, case)
+    page_elems = 64 * 8 * 256
+    pages = (1 << 32) // (page_elems * 2) + case.cfg[1] + 7
+    shift = pages - case.cfg[1]
+    for n in ("cache_k", "cache_v"):
+        big = torch.zeros(pages, page_elems, dtype=torch.bfloat16, device="cuda")
+        big[shift:] = t[n].view(-1, page_elems)
+        t[n] = big
+        setattr(a, n, big.data_ptr())
+    t["page_table"][t["page_table"] >= 0] += shift
+    a.cache_config.num_pages = pages
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+
+
+def test_long_run_against_prompt_attention(kv):
+    """The same prompt in one piece by the prompt attention and in chunks of odd length over the cache."""
+    rng = np.random.default_rng(11)
+    n, H, G, D, ps = 1500, 8, 2, 256, 16
+    q, k, v = (torch.from_numpy(rng.standard_normal((n, h, D), dtype=np.float32)).to(torch.bfloat16).cuda()
+               for h in (H * G, H, H))
+    whole = torch.empty_like(q)
+    kv.prefill_attention(whole, q, k, v, 1, n, H * G, H, D, 0, 1 / 16.0)
+    slots = -(-n // ps)
+    cfg = kv.make_kv_config(1, slots, ps, slots, 1, H, D, 0)
+    table = torch.from_numpy(rng.permutation(slots).astype(np.int32)).cuda()
+    ck, cv = (torch.full((slots * ps, H, D), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    out = torch.empty_like(q)
+    done = 0
+    for step in (1, 333, 64, 500, n):
+        m = min(step, n - done)
+        at = torch.arange(done, done + m, device="cuda")
+        place = table[at // ps].long() * ps + at % ps
+        ck[place], cv[place] = k[done:done + m], v[done:done + m]
+        a = kv.ChunkArgs()
+        ints = [torch.tensor([x], dtype=torch.int32, device="cuda") for x in (0, done, m, done)]
+        a.seq_batch, a.first_position, a.row_count, a.row_start = (x.data_ptr() for x in ints)
+        a.q, a.out, a.cache_k, a.cache_v, a.page_table = (x.data_ptr() for x in (q, out, ck, cv, table))
+        size = kv.chunk_workspace_bytes(H * G, H, D, 1, m)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        a.workspace, a.workspace_bytes, a.cache_config = ws.data_ptr(), size, cfg
+        a.run_count, a.max_row_count, a.rows, a.q_heads, a.softmax_scale = 1, m, n, H * G, 1 / 16.0
+        kv.chunk_attention(a)
+        torch.cuda.synchronize()
+        done += m
+    # two results, each off by what chunk_cases.py derives: 2 (2^-8 (A + |out|)) with A <= max |v| of the row's average
+    err = (out.float() - whole.float()).abs()
+    assert err.max().item() <= 4 * 2.0 ** -8 * float(v.float().abs().max())
+    assert err.mean().item() <= 2.0 ** -8 * float(whole.float().abs().mean()) * 2
