@@ -1,103 +1,1037 @@
-// Attention of runs of new tokens over the paged cache (B200KvChunkArgs).
+// Attention of runs of new tokens over the paged cache (B200KvChunkArgs):
 //   out[t, h] = sum_p softmax_p(scale q[t, h] . K[p, h / G]) V[p, h / G]
 // over the keys p <= t that have a page, with a window only p > t - window or
-// p < sinks. One warp per (row, query head): 16-byte packs of the head dims per
-// lane, one pass over the keys with a running maximum and sum in fp32.
+// p < sinks; G query heads share a KV head.
+//
+// Work. A tile of queries is 128 rows: 128 / G tokens of a run times the G query
+// heads of one KV head (row = token * G + head), so that K and V are read once for
+// the whole group and one token of 16 heads fills as many rows as eight tokens of
+// two. Keys come in tiles of 64: of the cache at positions that are multiples of 64,
+// of the runs' own rows counted from the run's first. An item is a (query tile, KV
+// head, part of the output dims); its keys are laid end to end with those of all
+// other items, in units of one key tile, and cut evenly: every CTA of the grid (one
+// per SM) takes one contiguous piece, whatever the lengths. A CTA that has all of an
+// item's keys writes the item's rows; a piece of an item leaves its rows' maximum,
+// sum and accumulator in the workspace, and chunk_combine_kernel joins them.
+//
+// One CTA: ten warps.
+//   warps 0-7  softmax: two groups of four warps, a thread per query row; group g
+//              takes the key tiles with number n % 2 == g
+//   warp 8     loads K and V tiles (TMA boxes that lie inside one page, or 16-byte
+//              copies where pages are no multiple of eight tokens)
+//   warp 9     one thread issues the MMAs
+// Tensor memory (512 columns): O (128 x 256 fp32), Q (128 x 256 bf16: the A operand
+// of Q K^T), and two score buffers of 64 columns; the weights go back as bf16 over
+// the scores they come from and are the A operand of P V. Shared memory holds
+// nothing but a ring of 32 KB slots (64 keys x 256 dims of K or V in 128-byte
+// swizzle): 7 slots for head_dim 256. For head_dim 512 a tile takes two K slots and
+// one V slot, the upper half of Q lies in shared memory (5 slots remain), and the
+// output dims are two parts computed by different items, each with all of Q K^T.
+// Q K^T of tile n + 1 runs under the softmax of tile n.
+//
+// Softmax: the maximum that a row's weights are scaled by is passed from tile to
+// tile (through shared memory, from one group to the other) and raised only when a
+// tile exceeds it by 2^8, so rescaling O is rare; scores, maxima, sums and O are
+// fp32, the weights are rounded to bf16 for P V (a relative 2^-9 each, which the
+// average over keys does not add up), the sum takes them unrounded.
+//
+// Keys that no row of the tile sees (before the window, behind the last row, pages
+// that are not mapped) may hold anything: their scores are replaced, and their V
+// rows cleared in shared memory before P V (0 * NaN).
+//
+// Every wait is bounded; one that runs out writes B200KV_STATUS_WAIT_TIMEOUT and
+// makes the CTA fall through to its exit, which frees the tensor memory.
 #include <algorithm>
 
 #include "chunk_common.cuh"
 #include "kernels.cuh"
+#include "umma_common.cuh"
 
 namespace b200kv {
 
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kRows = 128;                    // query rows per tile
+constexpr int kKeys = 64;                     // keys per tile
+constexpr int kPartDims = 256;                // output dims per item
+constexpr int kSlotBytes = kKeys * kPartDims * 2;
+constexpr int kBlockBytes = kKeys * 128;      // 64 keys x 64 dims
+constexpr int kQBlockBytes = kRows * 128;     // 128 rows x 64 dims
+constexpr int kMaxSlots = 7;
+constexpr int kSoftmaxWarps = 8;
+constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
+constexpr uint32_t kTmemColumns = 512;
+constexpr uint32_t kTmemQ = 256;
+constexpr uint32_t kTmemS = 384;              // + 64 * buffer
+constexpr float kRescaleSlack = 8.0f;         // log2 units
+constexpr int kInfos = 8;                     // key tiles whose description is kept
+constexpr long long kTileWaitClocks = 1ll << 26;
+// What starting an item costs next to a key tile (loading Q, reading O back), and
+// the least a CTA is given, both in key tiles: they shape the cut only.
+constexpr int kItemCost = 3;
+constexpr int kMinShare = 4;
 
-template <int D>
-__global__ __launch_bounds__(kWarps * 32) void chunk_attention_simple_kernel(ChunkAttentionArgs a) {
-  constexpr int kPacks = D / 256;
-  const Gemma4KvCacheConfig &c = a.cfg;
-  const ChunkRun run = chunk_run(a.runs, int(blockIdx.y), c.batch_size);
-  const int r = int(blockIdx.x);
-  const int head = int(blockIdx.z) * kWarps + (int(threadIdx.x) >> 5);
-  const int lane = int(threadIdx.x) & 31;
-  if (r >= run.count || head >= a.q_heads) return;
-  const int kv_head = head / (a.q_heads / c.num_heads);
-  const int t = run.first + r;
-  const int64_t row = (int64_t(run.start) + r) * a.q_heads + head;
-  float q[kPacks * 8], acc[kPacks * 8];
-  auto unpack = [](uint4 w, float *x) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+template <int kHeadDim_>
+struct ChunkTraits {
+  static constexpr int kHeadDim = kHeadDim_;
+  static constexpr int kKSlots = kHeadDim / 256;      // slots of one K tile
+  static constexpr int kParts = kHeadDim / kPartDims;
+  static constexpr int kTileSlots = kKSlots + 1;
+  static constexpr int kQHiBytes = (kHeadDim - 256) * kRows * 2;
+  static constexpr int kSlots = kHeadDim == 256 ? 7 : 5;
+  static constexpr int kTileBytes = kQHiBytes + kSlots * kSlotBytes;
+};
+
+struct ChunkParams {
+  __nv_bfloat16 *out;
+  float *lse;
+  const __nv_bfloat16 *q;
+  const __nv_bfloat16 *cache_k;
+  const __nv_bfloat16 *cache_v;
+  const __nv_bfloat16 *k_rows;
+  const __nv_bfloat16 *v_rows;
+  Gemma4KvCacheConfig cfg;
+  const int32_t *page_table;
+  ChunkRuns runs;
+  int32_t layer;
+  int32_t q_heads;
+  int32_t group;
+  int32_t tile_tokens;   // 128 / group
+  int32_t tiles_per_run; // query tiles of the longest run
+  int32_t window;
+  int32_t sinks;
+  int32_t box;           // tokens per TMA box; 0: rows are copied one by one
+  float scale_log2;
+  int4 *meta;            // per CTA: see PartialMeta
+  float *partials;       // [cta][2] x (acc [rows_cap][256], m [rows_cap], l [rows_cap])
+  int32_t rows_cap;
+  int32_t *status;
+};
+
+// The key tiles of a query tile, in this order: of the cache [0, ca) (sinks) and
+// [cb0, cb1), of the run's own rows [0, oa) (sinks) and [ob0, ob1).
+struct KeyTiles {
+  int ca, cb0, cb1, oa, ob0, ob1;
+  __device__ __forceinline__ int count() const { return ca + (cb1 - cb0) + oa + (ob1 - ob0); }
+};
+
+__device__ __forceinline__ KeyTiles key_tiles(const ChunkParams &p, int first, int t0, int t1) {
+  KeyTiles k = {};
+  const int lo = p.window > 0 ? max(0, t0 - p.window + 1) : 0;
+  const int sink_end = min(p.sinks, lo);
+  const int c_lim = p.k_rows != nullptr ? min(first, t1 + 1) : t1 + 1;
+  k.ca = div_up(min(sink_end, c_lim), kKeys);
+  if (c_lim > lo) {
+    k.cb0 = lo / kKeys;
+    k.cb1 = div_up(c_lim, kKeys);
+    k.ca = min(k.ca, k.cb0);
+  }
+  if (p.k_rows != nullptr) {
+    k.ob0 = (max(lo, first) - first) / kKeys;
+    k.ob1 = (t1 - first) / kKeys + 1;
+    k.oa = sink_end > first ? min(div_up(sink_end - first, kKeys), k.ob0) : 0;
+  }
+  return k;
+}
+
+// A piece of an item's key tiles: what one CTA does between loading Q and writing rows.
+struct Segment {
+  ChunkRun run;
+  KeyTiles keys;
+  int hp;            // part * KV heads + KV head
+  int run_index;
+  int query_tile;
+  int token0;        // first token of the tile within the run
+  int rows;          // query rows
+  int t0, t1;        // positions of the first and last row
+  int begin, end;    // key tiles [begin, end) of the item
+  int total;
+};
+
+// Walks the items of a CTA's share. Every role does so by itself.
+struct Walk {
+  long long left;
+  int hp, run, tile, offset;
+
+  __device__ __forceinline__ bool next(const ChunkParams &p, Segment &s) {
+    while (left > 0) {
+      s.run = chunk_run(p.runs, run, p.cfg.batch_size);
+      s.token0 = tile * p.tile_tokens;
+      if (s.token0 >= s.run.count) {  // the run has no such tile
+        tile = 0;
+        offset = 0;
+        if (++run == p.runs.run_count) {
+          run = 0;
+          ++hp;
+        }
+        continue;
+      }
+      const int tokens = min(p.tile_tokens, s.run.count - s.token0);
+      s.t0 = s.run.first + s.token0;
+      s.t1 = s.t0 + tokens - 1;
+      s.rows = tokens * p.group;
+      s.keys = key_tiles(p, s.run.first, s.t0, s.t1);
+      s.total = s.keys.count();
+      s.hp = hp;
+      s.run_index = run;
+      s.query_tile = tile;
+      const int cost = s.total + kItemCost;
+      const int take = int(min((long long)(cost - offset), left));
+      s.begin = max(0, offset - kItemCost);
+      s.end = max(0, offset + take - kItemCost);
+      left -= take;
+      offset += take;
+      if (offset == cost) {
+        offset = 0;
+        ++tile;
+      }
+      if (s.begin < s.end) return true;
+    }
+    return false;
+  }
+};
+
+// What the softmax needs to know about a key tile, left by the loader.
+struct TileInfo {
+  unsigned long long live;  // keys that some row of the query tile sees
+  int base;                 // position of the tile's first key
+  int edge;                 // some row does not see all 64
+};
+
+struct SmallState {
+  uint64_t full[kMaxSlots];   // the slot's tile has landed
+  uint64_t done[kMaxSlots];   // the MMAs that read the slot are complete
+  uint64_t s_full[2];         // scores of the tile in S[b] complete
+  uint64_t p_full[2];         // its weights written (and O rescaled where needed)
+  uint64_t m_full[2][4];      // row_ref[b] of 32 rows written
+  uint64_t l_full[2][4];      // row_sum of 32 rows written by the group
+  uint64_t q_full;            // Q of the segment in tensor memory
+  uint64_t o_free;            // O of the segment read back
+  TileInfo info[kInfos];
+  float row_ref[2][kRows];
+  float row_sum[2][kRows];
+  long long scan[kThreads / 32];
+  long long total;
+  Walk start;
+  uint32_t tmem_base;
+  int abort;
+};
+
+template <class T>
+constexpr int kChunkSmemBytes = T::kTileBytes + int(sizeof(SmallState));
+
+// 64 fp32 columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&r)[64]) {
+  uint32_t u[64];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = bf16_lo(u[i]);
-      x[2 * i + 1] = bf16_hi(u[i]);
+  for (int h = 0; h < 2; ++h) {
+    uint32_t *v = u + 32 * h;
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]),
+          "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+          "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]),
+          "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
+          "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr + 32u * uint32_t(h))
+        : "memory");
+  }
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) {
+    asm volatile("" : "+r"(u[i]));  // not used before the wait
+    r[i] = __uint_as_float(u[i]);
+  }
+}
+
+// One box of `box` tokens x 64 dims of a page into rows of a swizzled column block.
+__device__ __forceinline__ void tma_load_page_box(uint32_t dst, const CUtensorMap *map, int offset,
+                                                  int block, int head, int page, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(offset), "r"(block), "r"(head), "r"(page),
+      "r"(bar)
+      : "memory");
+}
+// 64 packed rows x 64 dims; rows past the tensor arrive as zeros.
+__device__ __forceinline__ void tma_load_rows_box(uint32_t dst, const CUtensorMap *map, int x, int row,
+                                                  uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// bits [0, n) of a 64-bit word, n clamped to 0 .. 64
+__device__ __forceinline__ unsigned long long low_bits(int n) {
+  return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1ull);
+}
+
+template <class T>
+__global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
+    const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap map_k,
+    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k_rows,
+    const __grid_constant__ CUtensorMap map_v_rows) {
+  constexpr int kSlots = T::kSlots;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  SmallState &small = *reinterpret_cast<SmallState *>(smem_raw + T::kTileBytes);
+  const uint32_t s_q_hi = smem_u32(smem_raw);
+  const uint32_t s_ring = s_q_hi + T::kQHiBytes;
+  const int tid = int(threadIdx.x);
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
+  const int heads = p.cfg.num_heads;
+  if ((s_q_hi & 1023u) != 0) {  // the swizzle's atoms; the window starts on such a boundary
+    if (tid == 0) set_status(p.status, B200KV_STATUS_WAIT_TIMEOUT);
+    return;
+  }
+
+  const uint32_t bar_full = smem_u32(&small.full[0]);      // + 8 slot
+  const uint32_t bar_done = smem_u32(&small.done[0]);      // + 8 slot
+  const uint32_t bar_s_full = smem_u32(&small.s_full[0]);  // + 8 b
+  const uint32_t bar_p_full = smem_u32(&small.p_full[0]);  // + 8 b
+  const uint32_t bar_m_full = smem_u32(&small.m_full[0][0]);  // + 32 b + 8 warp quarter
+  const uint32_t bar_l_full = smem_u32(&small.l_full[0][0]);  // + 32 group + 8 warp quarter
+  const uint32_t bar_q_full = smem_u32(&small.q_full);
+  const uint32_t bar_o_free = smem_u32(&small.o_free);
+  if (tid == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(bar_full + 8u * i, 1);
+      mbar_init(bar_done + 8u * i, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_s_full + 8u * b, 1);
+      mbar_init(bar_p_full + 8u * b, 4);
+      for (int w = 0; w < 4; ++w) {
+        mbar_init(bar_m_full + 32u * b + 8u * w, 1);
+        mbar_init(bar_l_full + 32u * b + 8u * w, 1);
+      }
+    }
+    mbar_init(bar_q_full, kSoftmaxWarps);
+    mbar_init(bar_o_free, kSoftmaxWarps);
+    small.abort = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&small.tmem_base)),
+                 "r"(kTmemColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // everything up to here is this kernel's own; the runs, the rows and the cache
+  // may be what the kernel before it writes
+  pdl_wait_for_predecessor();
+
+  // ---- this CTA's share: the costs of all (run, query tile) pairs, summed
+  const int pairs = p.runs.run_count * p.tiles_per_run;
+  const int per_thread = div_up(pairs, kThreads);
+  auto pair_cost = [&](int pair) -> int {
+    const ChunkRun run = chunk_run(p.runs, pair / p.tiles_per_run, p.cfg.batch_size);
+    const int token0 = (pair % p.tiles_per_run) * p.tile_tokens;
+    if (token0 >= run.count) return 0;
+    const int t0 = run.first + token0;
+    const int t1 = t0 + min(p.tile_tokens, run.count - token0) - 1;
+    return key_tiles(p, run.first, t0, t1).count() + kItemCost;
+  };
+  long long mine = 0;
+  for (int i = 0; i < per_thread; ++i) {
+    const int pair = tid * per_thread + i;
+    if (pair < pairs) mine += pair_cost(pair);
+  }
+  long long before = mine;  // inclusive scan over the warp
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += up;
+  }
+  if (lane == 31) small.scan[warp] = before;
+  __syncthreads();
+  long long warps_before = 0, per_head = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) warps_before += small.scan[w];
+    per_head += small.scan[w];
+  }
+  before += warps_before - mine;  // costs before this thread's first pair
+  const long long total = per_head * heads * T::kParts;
+  const long long ctas = max(1ll, min((long long)gridDim.x, total / kMinShare));
+  const long long c0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : 0;
+  const long long c1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
+  if (tid == 0) {
+    small.start.left = 0;
+    small.start.hp = small.start.run = small.start.tile = small.start.offset = 0;
+  }
+  __syncthreads();
+  if (c1 > c0) {
+    const int hp = int(c0 / per_head);
+    long long rem = c0 - (long long)hp * per_head;
+    if (rem >= before && rem < before + mine) {
+      rem -= before;
+      int pair = tid * per_thread;
+      for (int cost = pair_cost(pair); rem >= cost; cost = pair_cost(pair)) {
+        rem -= cost;
+        ++pair;
+      }
+      small.start.left = c1 - c0;
+      small.start.hp = hp;
+      small.start.run = pair / p.tiles_per_run;
+      small.start.tile = pair % p.tiles_per_run;
+      small.start.offset = int(rem);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = small.tmem_base;
+  volatile int *abort_flag = &small.abort;
+  Walk walk = small.start;
+
+  // Bounded wait that also gives up when another role has; false = give up.
+  auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long start = clock64();
+    for (uint32_t poll = 0;; ++poll) {
+      if (mbar_try_wait(bar, parity)) return true;
+      if ((poll & 31u) == 31u) {
+        if (*abort_flag != 0) return false;
+        if (clock64() - start > kTileWaitClocks) {
+          set_status(p.status, B200KV_STATUS_WAIT_TIMEOUT);
+          *abort_flag = 1;
+          return false;
+        }
+      }
     }
   };
+  // The slots are filled and freed in order: fill i uses slot i % kSlots for the
+  // (i / kSlots)-th time. Fill i of a tile n: i = n * kTileSlots (+ 1) for K, then V.
+  auto slot_of = [](int fill) { return uint32_t(fill % kSlots); };
+  auto parity_of = [](int fill) { return uint32_t(fill / kSlots) & 1u; };
+
+  if (warp == kSoftmaxWarps) {
+    // ------------------------------------------------------------ loader
+    int fills = 0;
+    int tile_number = 0;
+    int4 meta = make_int4(-1, 0, 0, 0);
+    Segment s;
+    bool ok = true;
+    auto claim = [&](int fill) -> bool {  // the slot's last reader is done
+      const bool free = fill < kSlots || wait(bar_done + 8u * slot_of(fill), parity_of(fill) ^ 1u);
+      return __all_sync(0xffffffffu, free);
+    };
+    while (ok && walk.next(p, s)) {
+      if (s.begin > 0) meta.w = s.end == s.total ? 1 : 2;
+      if (s.begin == 0 && s.end < s.total) {
+        meta.x = s.hp;
+        meta.y = s.run_index;
+        meta.z = s.query_tile;
+      }
+      const int head = s.hp % heads;
+      const int part = s.hp / heads;
+      for (int j = s.begin; j < s.end; ++j, ++tile_number) {
+        // where the tile lies and which of its keys anyone sees
+        int k = j;
+        bool own = false;
+        if (k < s.keys.ca) {
+        } else if ((k -= s.keys.ca) < s.keys.cb1 - s.keys.cb0) {
+          k += s.keys.cb0;
+        } else {
+          k -= s.keys.cb1 - s.keys.cb0;
+          own = true;
+          if (k >= s.keys.oa) k += s.keys.ob0 - s.keys.oa;
+        }
+        const int base = (own ? s.run.first : 0) + k * kKeys;
+        unsigned long long live = low_bits(s.t1 + 1 - base);
+        if (!own && p.k_rows != nullptr) live &= low_bits(s.run.first - base);
+        if (p.window > 0) {
+          live &= ~low_bits(s.t0 - p.window + 1 - base) | low_bits(p.sinks - base);
+        }
+        int64_t row_at[2] = {-1, -1};  // box == 0: element offset of rows lane, lane + 32
+        int page = -1, page_offset = 0;
+        const int piece = lane >> 2;   // box > 0: four lanes per box, one per 64 dims
+        unsigned long long boxes = 0;
+        if (!own && p.box > 0) {
+          if (piece * p.box < kKeys) {
+            const unsigned long long bits =
+                (p.box == 64 ? ~0ull : (1ull << p.box) - 1ull) << (piece * p.box);
+            if ((live & bits) != 0) {
+              const int position = base + piece * p.box;
+              const int logical = position / p.cfg.page_size;
+              page = chunk_page(p.cfg, p.page_table, s.run.batch, logical);
+              page_offset = position - logical * p.cfg.page_size;
+              if (page >= 0) boxes = bits;
+            }
+          }
+          const uint32_t lo = __reduce_or_sync(0xffffffffu, uint32_t(boxes));
+          const uint32_t hi = __reduce_or_sync(0xffffffffu, uint32_t(boxes >> 32));
+          boxes = (uint64_t(hi) << 32) | lo;
+          live &= boxes;
+        } else if (p.box == 0) {
 #pragma unroll
-  for (int v = 0; v < kPacks; ++v) {
-    unpack(__ldg(reinterpret_cast<const uint4 *>(a.q + row * D) + lane + 32 * v), q + 8 * v);
+          for (int i = 0; i < 2; ++i) {
+            const int r = lane + 32 * i;
+            if (((live >> r) & 1ull) == 0) continue;
+            if (own) {
+              row_at[i] = ((int64_t(s.run.start) + k * kKeys + r) * heads + head) * T::kHeadDim;
+            } else {
+              const int logical = (base + r) / p.cfg.page_size;
+              const int at = chunk_page(p.cfg, p.page_table, s.run.batch, logical);
+              if (at >= 0) {
+                row_at[i] = cache_offset(p.cfg, p.layer, at, base + r - logical * p.cfg.page_size,
+                                         head, 0);
+              }
+            }
+          }
+          const uint32_t lo = __ballot_sync(0xffffffffu, row_at[0] >= 0);
+          const uint32_t hi = __ballot_sync(0xffffffffu, row_at[1] >= 0);
+          live &= (uint64_t(hi) << 32) | lo;
+        }
+        const bool edge = live != ~0ull || base + kKeys - 1 > s.t0 ||
+                          (p.window > 0 && base <= s.t1 - p.window && base + kKeys > p.sinks);
+        if (lane == 0) small.info[tile_number % kInfos] = {live, base, edge ? 1 : 0};
+        __syncwarp();
+        // K slots, then the V slot
+#pragma unroll
+        for (int f = 0; f < T::kTileSlots; ++f, ++fills) {
+          const bool is_v = f == T::kKSlots;
+          const int block0 = is_v ? part * 4 : f * 4;
+          ok = claim(fills);
+          if (!ok) break;
+          const uint32_t bar = bar_full + 8u * slot_of(fills);
+          const uint32_t dst = s_ring + slot_of(fills) * kSlotBytes;
+          if (p.box == 0) {
+            const __nv_bfloat16 *from = own ? (is_v ? p.v_rows : p.k_rows) : (is_v ? p.cache_v : p.cache_k);
+            const uint32_t column = dst + uint32_t(lane >> 3) * kBlockBytes;
+#pragma unroll 8
+            for (int r = 0; r < kKeys; ++r) {
+              const int64_t at = __shfl_sync(0xffffffffu, row_at[r >> 5], r & 31);
+              if (at >= 0) {
+                cp_async16(column + uint32_t(r) * 128u + ((uint32_t(lane & 7) ^ uint32_t(r & 7)) << 4),
+                           from + at + block0 * 64 + lane * 8);
+              }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+          } else if (own) {
+            if (lane == 0) mbar_arrive_expect_tx(bar, kSlotBytes);
+            __syncwarp();
+            if (lane < 4) {
+              tma_load_rows_box(dst + uint32_t(lane) * kBlockBytes, is_v ? &map_v_rows : &map_k_rows,
+                                head * T::kHeadDim + (block0 + lane) * 64,
+                                s.run.start + k * kKeys, bar);
+            }
+          } else {
+            if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(__popcll(boxes)) * (kPartDims * 2));
+            __syncwarp();
+            if (page >= 0) {
+              tma_load_page_box(dst + uint32_t(lane & 3) * kBlockBytes + uint32_t(piece * p.box) * 128u,
+                                is_v ? &map_v : &map_k, page_offset, block0 + (lane & 3), head,
+                                p.layer * p.cfg.num_pages + page, bar);
+            }
+          }
+        }
+        if (!ok) break;
+      }
+    }
+    if (lane == 0) p.meta[blockIdx.x] = meta;
+    if (!ok || *abort_flag != 0) {
+      // nobody may be waiting for the last loads any more: see them land before the
+      // CTA gives its shared memory back
+      for (int i = max(0, fills - kSlots); i < fills; ++i) {
+        mbar_wait_bounded(bar_full + 8u * slot_of(i), parity_of(i), kTileWaitClocks);
+      }
+    }
+  } else if (warp == kSoftmaxWarps + 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t kIdescQK = umma_idesc(kKeys, false);
+      constexpr uint32_t kIdescPV = umma_idesc(kPartDims, true);
+      int n = 0;         // key tiles so far
+      int segments = 0;
+      Segment s;
+      bool ok = true;
+      // O (+)= P V: four steps of 16 keys; 8-key groups 1024 bytes apart, 64-dim
+      // blocks one column block apart (MN-major)
+      auto issue_pv = [&](int tile, bool accumulate) -> bool {
+        const int fill = tile * T::kTileSlots + T::kKSlots;
+        const uint32_t b = uint32_t(tile & 1);
+        if (!wait(bar_full + 8u * slot_of(fill), parity_of(fill))) return false;
+        if (!wait(bar_p_full + 8u * b, uint32_t(tile >> 1) & 1u)) return false;
+        tc_fence_after();
+        const uint32_t v = s_ring + slot_of(fill) * kSlotBytes;
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i) {
+          umma_bf16_a_tmem(tmem, tmem + kTmemS + b * kKeys + 8u * uint32_t(i),
+                           umma_desc(v + uint32_t(i) * 2048u, kBlockBytes >> 4, 64), kIdescPV,
+                           accumulate || i > 0);
+        }
+        umma_commit(bar_done + 8u * slot_of(fill));
+        return true;
+      };
+      while (ok && walk.next(p, s)) {
+        ok = wait(bar_q_full, uint32_t(segments & 1));
+        for (int j = s.begin; j < s.end && ok; ++j, ++n) {
+          // S[n & 1] held the weights of tile n - 2
+          if (n >= 2) {
+            const int fill = (n - 2) * T::kTileSlots + T::kKSlots;
+            ok = wait(bar_done + 8u * slot_of(fill), parity_of(fill));
+            if (!ok) break;
+          }
+          const uint32_t d = tmem + kTmemS + uint32_t(n & 1) * kKeys;
+#pragma unroll
+          for (int f = 0; f < T::kKSlots; ++f) {
+            const int fill = n * T::kTileSlots + f;
+            ok = ok && wait(bar_full + 8u * slot_of(fill), parity_of(fill));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t k = s_ring + slot_of(fill) * kSlotBytes;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {  // steps of 16 dims, four to a column block
+              const uint32_t in = uint32_t(i & 3) * 32u;
+              const uint64_t kd = umma_desc(k + uint32_t(i >> 2) * kBlockBytes + in, 1, 64);
+              if (f == 0) {
+                umma_bf16_a_tmem(d, tmem + kTmemQ + 8u * uint32_t(i), kd, kIdescQK, i > 0);
+              } else {
+                umma_bf16(d, umma_desc(s_q_hi + uint32_t(i >> 2) * kQBlockBytes + in, 1, 64), kd,
+                          kIdescQK, true);
+              }
+            }
+            umma_commit(bar_done + 8u * slot_of(fill));
+          }
+          if (!ok) break;
+          umma_commit(bar_s_full + 8u * uint32_t(n & 1));
+          if (j > s.begin) ok = issue_pv(n - 1, j - 1 > s.begin);
+          // the segment's first P V writes O anew: the last segment's rows must be out
+          if (j == s.begin && segments > 0) ok = wait(bar_o_free, uint32_t(segments - 1) & 1u);
+        }
+        if (ok) ok = issue_pv(n - 1, s.end - s.begin > 1);
+        ++segments;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int group = warp >> 2;
+    const int quarter = warp & 3;
+    const int row = tid & (kRows - 1);
+    const uint32_t lanes = uint32_t(32 * quarter) << 16;
+    const float scale = p.scale_log2;
+    int n0 = 0;        // key tiles before this segment
+    int segments = 0;
+    bool ok = true;
+    // every lane waits; the warp goes on or gives up as one
+    auto warp_wait = [&](uint32_t bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, wait(bar, parity));
+    };
+    // Q rows of a segment: this group's half of the dims into tensor memory (and,
+    // head_dim 512, its half of the upper dims into shared memory)
+    auto load_q = [&](const Segment &s) {
+      const bool active = 32 * quarter < s.rows;
+      if (active) {
+        const int token = row / p.group;
+        const __nv_bfloat16 *src =
+            p.q + ((int64_t(s.run.start) + s.token0 + token) * p.q_heads + (s.hp % heads) * p.group +
+                   (row - token * p.group)) * T::kHeadDim + 128 * group;
+        uint4 w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          w[i] = row < s.rows ? __ldg(reinterpret_cast<const uint4 *>(src) + i) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          tmem_st32(tmem + lanes + kTmemQ + 64u * uint32_t(group) + 32u * uint32_t(h),
+                    reinterpret_cast<const float *>(w + 8 * h));
+        }
+        if constexpr (T::kKSlots == 2) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint4 hi = row < s.rows ? __ldg(reinterpret_cast<const uint4 *>(src + 256) + i)
+                                          : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(smem_raw + (2 * group + (i >> 3)) * kQBlockBytes + row * 128 +
+                                       (((i & 7) ^ (row & 7)) << 4)) = hi;
+          }
+          fence_proxy_async_shared();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q_full);
+    };
+    Segment s;
+    bool more = walk.next(p, s);
+    if (more) load_q(s);
+    while (more && ok) {
+      const bool active = 32 * quarter < s.rows;  // some row of the warp is a query
+      const int token = min(row, s.rows - 1) / p.group;
+      const int t = s.t0 + token;
+      const int n1 = n0 + (s.end - s.begin);
+      float l_run = 0.0f;
+      float ref = -INFINITY;  // what l_run's weights are scaled by
+      for (int n = n0 + ((n0 ^ group) & 1); n < n1; n += 2) {
+        ok = warp_wait(bar_s_full + 8u * uint32_t(group), uint32_t(n >> 1) & 1u);
+        if (!ok) break;
+        tc_fence_after();
+        const TileInfo info = small.info[n % kInfos];
+        if (active) {
+          float sc[64];
+          const uint32_t s_at = tmem + lanes + kTmemS + uint32_t(group) * kKeys;
+          tmem_ld64(s_at, sc);
+          if (info.edge) {
+            unsigned long long sees = info.live & low_bits(t + 1 - info.base);
+            if (p.window > 0) {
+              sees &= ~low_bits(t - p.window + 1 - info.base) | low_bits(p.sinks - info.base);
+            }
+            const uint32_t lo = uint32_t(sees), hi = uint32_t(sees >> 32);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              if (((lo >> c) & 1u) == 0) sc[c] = -INFINITY;
+              if (((hi >> c) & 1u) == 0) sc[c + 32] = -INFINITY;
+            }
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 64; c += 8) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], fmaxf(sc[c + u], sc[c + 4 + u]));
+          }
+          const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+          // the reference so far: the other group's tile before this one
+          float last = -INFINITY;
+          if (n > n0) {
+            ok = warp_wait(bar_m_full + 32u * uint32_t(group ^ 1) + 8u * uint32_t(quarter),
+                           uint32_t((n - 1) >> 1) & 1u);
+            if (!ok) break;
+            last = small.row_ref[group ^ 1][row];
+          }
+          float now = last;
+          if (m_tile > last + kRescaleSlack || last == -INFINITY) now = m_tile;
+          small.row_ref[group][row] = now;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_m_full + 32u * uint32_t(group) + 8u * uint32_t(quarter));
+          if (ref != now) {
+            if (ref != -INFINITY) l_run *= ex2_approx(ref - now);
+            ref = now;
+          }
+          const float neg = now == -INFINITY ? 0.0f : -now;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float e0 = ex2_approx(fmaf(sc[2 * i], scale, neg));
+            const float e1 = ex2_approx(fmaf(sc[2 * i + 1], scale, neg));
+            sum[i & 3] += e0 + e1;
+            const __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+          }
+          l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          // tensor-memory accesses are warp-wide: the warp rescales its rows of O if
+          // any of them must, once P V of the tile before no longer adds to them
+          const bool raised = last != -INFINITY && now != last;
+          if (__any_sync(0xffffffffu, raised)) {
+            const int fill = (n - 1) * T::kTileSlots + T::kKSlots;
+            ok = warp_wait(bar_done + 8u * slot_of(fill), parity_of(fill));
+            if (!ok) break;
+            tc_fence_after();
+            const float factor = raised ? ex2_approx(last - now) : 1.0f;
+#pragma unroll 1
+            for (int c = 0; c < kPartDims; c += 32) {
+              float o[32];
+              tmem_ld32(tmem + lanes + uint32_t(c), o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] *= factor;
+              tmem_st32(tmem + lanes + uint32_t(c), o);
+            }
+          }
+          tmem_st32(s_at, reinterpret_cast<const float *>(w));
+        } else if (lane == 0) {
+          // nobody reads it, but the barrier's phases go by the tile's number
+          mbar_arrive(bar_m_full + 32u * uint32_t(group) + 8u * uint32_t(quarter));
+        }
+        if (info.live != ~0ull) {
+          const int fill = n * T::kTileSlots + T::kKSlots;
+          ok = warp_wait(bar_full + 8u * slot_of(fill), parity_of(fill));
+          if (!ok) break;
+          uint8_t *v = smem_raw + T::kQHiBytes + slot_of(fill) * kSlotBytes + (lane >> 3) * kBlockBytes +
+                       (lane & 7) * 16;
+          for (int r = quarter; r < kKeys; r += 4) {
+            if (((info.live >> r) & 1ull) == 0) *reinterpret_cast<uint4 *>(v + r * 128) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_shared();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p_full + 8u * uint32_t(group));
+      }
+      if (!ok) break;
+
+      // ---- the segment's end: Q of the next one, then this one's rows
+      const int last = n1 - 1;
+      const bool owner = (last & 1) == group;
+      if (!owner) {
+        ok = warp_wait(bar_s_full + 8u * uint32_t(last & 1), uint32_t(last >> 1) & 1u);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const Segment done = s;
+      more = walk.next(p, s);
+      if (more) load_q(s);
+      if (active) {
+        if (!owner) {
+          ok = warp_wait(bar_m_full + 32u * uint32_t(group ^ 1) + 8u * uint32_t(quarter),
+                         uint32_t(last >> 1) & 1u);
+          if (!ok) break;
+          const float now = small.row_ref[group ^ 1][row];
+          if (ref != now) {
+            l_run = ref == -INFINITY ? 0.0f : l_run * ex2_approx(ref - now);
+            ref = now;
+          }
+        }
+      }
+      const int fill = last * T::kTileSlots + T::kKSlots;
+      ok = warp_wait(bar_done + 8u * slot_of(fill), parity_of(fill));
+      if (!ok) break;
+      tc_fence_after();
+      if (active) small.row_sum[group][row] = l_run;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_l_full + 32u * uint32_t(group) + 8u * uint32_t(quarter));
+      ok = warp_wait(bar_l_full + 32u * uint32_t(group ^ 1) + 8u * uint32_t(quarter),
+                     uint32_t(segments & 1));
+      if (!ok) break;
+      const bool whole = done.begin == 0 && done.end == done.total;
+      const bool writes = active && row < done.rows;
+      const float l_row = active ? small.row_sum[0][row] + small.row_sum[1][row] : 0.0f;
+      const float inv = whole ? (l_row > 0.0f ? 1.0f / l_row : 0.0f) : 1.0f;
+      const int part = done.hp / heads;
+      const int64_t at = (int64_t(done.run.start) + done.token0 + token) * p.q_heads +
+                         (done.hp % heads) * p.group + (row - token * p.group);
+      float *piece = p.partials + (int64_t(blockIdx.x) * 2 + (done.begin == 0 ? 1 : 0)) *
+                                      (int64_t(p.rows_cap) * (kPartDims + 2));
+      // 64 columns at a time; the second half frees O before its stores
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        const int column = 128 * group + 64 * h;
+        float o[64];
+        if (active) tmem_ld64(tmem + lanes + uint32_t(column), o);
+        if (h == 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_o_free);
+        }
+        if (writes && whole) {
+          uint4 *dst = reinterpret_cast<uint4 *>(p.out + at * T::kHeadDim + part * kPartDims + column);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const __nv_bfloat162 b2 =
+                  __floats2bfloat162_rn(o[8 * i + 2 * j] * inv, o[8 * i + 2 * j + 1] * inv);
+              w[j] = *reinterpret_cast<const uint32_t *>(&b2);
+            }
+            dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else if (writes) {
+          float4 *acc = reinterpret_cast<float4 *>(piece + row * kPartDims + column);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
+      if (writes && group == 0) {
+        if (!whole) {
+          piece[p.rows_cap * kPartDims + row] = ref;
+          piece[p.rows_cap * (kPartDims + 1) + row] = l_row;
+        } else if (p.lse != nullptr && part == 0) {
+          p.lse[at] = l_row > 0.0f ? (ref + log2f(l_row)) * 0.6931471805599453f : -INFINITY;
+        }
+      }
+      n0 = n1;
+      ++segments;
+    }
   }
-#pragma unroll
-  for (int i = 0; i < kPacks * 8; ++i) acc[i] = 0.0f;
-  const float scale = a.softmax_scale * 1.4426950408889634f;
-  float m = -INFINITY, l = 0.0f;
-  const int lo = a.window > 0 ? max(0, t - a.window + 1) : 0;
-  for (int p = 0; p <= t; ++p) {
-    if (p < lo && p >= a.sinks) {
-      p = lo - 1;
-      continue;
-    }
-    const __nv_bfloat16 *k, *v;
-    if (a.k_rows != nullptr && p >= run.first) {
-      const int64_t at = ((int64_t(run.start) + p - run.first) * c.num_heads + kv_head) * D;
-      k = a.k_rows + at;
-      v = a.v_rows + at;
-    } else {
-      const int page = chunk_page(c, a.page_table, run.batch, p / c.page_size);
-      if (page < 0) continue;
-      const int64_t at = cache_offset(c, a.layer, page, p % c.page_size, kv_head, 0);
-      k = a.cache_k + at;
-      v = a.cache_v + at;
-    }
-    float s = 0.0f;
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < kPacks; ++i) {
-      unpack(__ldg(reinterpret_cast<const uint4 *>(k) + lane + 32 * i), x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s = fmaf(q[8 * i + j], x[j], s);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= scale;
-    const float new_m = fmaxf(m, s);
-    const float corr = m == -INFINITY ? 0.0f : ex2_approx(m - new_m);
-    const float w = ex2_approx(s - new_m);
-    l = l * corr + w;
-    m = new_m;
-#pragma unroll
-    for (int i = 0; i < kPacks; ++i) {
-      unpack(__ldg(reinterpret_cast<const uint4 *>(v) + lane + 32 * i), x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[8 * i + j] = fmaf(w, x[j], acc[8 * i + j] * corr);
-    }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(kTmemColumns)
+                 : "memory");
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+}
+
+// Joins the partial rows of items that several CTAs share. Block (i, y): the item
+// whose first key tiles CTA i has (meta.x >= 0: KV head and part; meta.y, meta.z: run
+// and query tile); the pieces behind it are the first of CTA i + 1, i + 2, ... up to
+// the one that has the item's end (meta.w 1; 2: goes on). A warp per row:
+//   M = max m, out = sum 2^(m - M) acc / sum 2^(m - M) l, lse = (M + log2 sum) ln 2
+constexpr int kCombineWarps = 8;
+__global__ __launch_bounds__(kCombineWarps * 32) void chunk_combine_kernel(ChunkParams p, int head_dim) {
+  pdl_wait_for_predecessor();
+  const int4 meta = p.meta[blockIdx.x];
+  if (meta.x < 0) return;
+  const int warp = int(threadIdx.x) >> 5;
+  const int lane = int(threadIdx.x) & 31;
+  int pieces = 0;  // behind the first
+  for (int base = int(blockIdx.x) + 1;; base += 32) {
+    const int state = base + lane < int(gridDim.x) ? p.meta[base + lane].w : 1;
+    const uint32_t end = __ballot_sync(0xffffffffu, state != 2);
+    if (end != 0) {
+      pieces += __ffs(int(end));
+      break;
+    }
+    pieces += 32;
+  }
+  pieces = min(pieces, int(gridDim.x) - 1 - int(blockIdx.x));
+  const ChunkRun run = chunk_run(p.runs, meta.y, p.cfg.batch_size);
+  const int token0 = meta.z * p.tile_tokens;
+  const int rows = min(p.tile_tokens, run.count - token0) * p.group;
+  const int head = meta.x % p.cfg.num_heads;
+  const int part = meta.x / p.cfg.num_heads;
+  const int64_t slot_floats = int64_t(p.rows_cap) * (kPartDims + 2);
+  const float *first = p.partials + (int64_t(blockIdx.x) * 2 + 1) * slot_floats;
+  const float *rest = p.partials + (int64_t(blockIdx.x) + 1) * 2 * slot_floats;
+  for (int row = int(blockIdx.y) * kCombineWarps + warp; row < rows; row += int(gridDim.y) * kCombineWarps) {
+    auto piece = [&](int i) { return i == 0 ? first : rest + int64_t(i - 1) * 2 * slot_floats; };
+    float m = -INFINITY;
+    for (int i = lane; i <= pieces; i += 32) m = fmaxf(m, piece(i)[p.rows_cap * kPartDims + row]);
 #pragma unroll
-  for (int v = 0; v < kPacks; ++v) {
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.0f;
+    float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int i = 0; i <= pieces; ++i) {
+      const float *from = piece(i);
+      const float mi = from[p.rows_cap * kPartDims + row];
+      const float li = from[p.rows_cap * (kPartDims + 1) + row];
+      const float4 a = *reinterpret_cast<const float4 *>(from + row * kPartDims + lane * 8);
+      const float4 b = *reinterpret_cast<const float4 *>(from + row * kPartDims + lane * 8 + 4);
+      // a piece without a visible key has accumulated zeros
+      const float f = mi == -INFINITY ? 0.0f : ex2_approx(mi - m);
+      l = fmaf(f, li, l);
+      acc[0] = fmaf(f, a.x, acc[0]);
+      acc[1] = fmaf(f, a.y, acc[1]);
+      acc[2] = fmaf(f, a.z, acc[2]);
+      acc[3] = fmaf(f, a.w, acc[3]);
+      acc[4] = fmaf(f, b.x, acc[4]);
+      acc[5] = fmaf(f, b.y, acc[5]);
+      acc[6] = fmaf(f, b.z, acc[6]);
+      acc[7] = fmaf(f, b.w, acc[7]);
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const int64_t at = (int64_t(run.start) + token0 + row / p.group) * p.q_heads + head * p.group +
+                       row % p.group;
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(acc[8 * v + 2 * i] * inv, acc[8 * v + 2 * i + 1] * inv);
-      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    for (int j = 0; j < 4; ++j) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+      w[j] = *reinterpret_cast<const uint32_t *>(&h);
     }
-    reinterpret_cast<uint4 *>(a.out + row * D)[lane + 32 * v] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4 *>(p.out + at * head_dim + part * kPartDims)[lane] =
+        make_uint4(w[0], w[1], w[2], w[3]);
+    if (p.lse != nullptr && part == 0 && lane == 0) {
+      p.lse[at] = l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+    }
   }
-  if (a.lse != nullptr && lane == 0) {
-    a.lse[row] = l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+// Tokens per box: the largest power of two up to a key tile that divides the page
+// (a box then lies in one page); less than eight rows do not fill a swizzle atom.
+int box_tokens(int page_size) {
+  int box = kKeys;
+  while (page_size % box != 0) box /= 2;
+  return box >= 8 ? box : 0;
+}
+
+bool make_cache_map(CUtensorMap *map, const __nv_bfloat16 *base, const Gemma4KvCacheConfig &c, int box) {
+  EncodeTiledFn encode = encode_tiled_fn();
+  if (encode == nullptr) return false;
+  const cuuint64_t row = cuuint64_t(c.num_heads) * c.head_dim * 2;
+  // [page][head][block of 64 dims][offset in page][64 dims]
+  const cuuint64_t dims[5] = {64, cuuint64_t(c.page_size), cuuint64_t(c.head_dim / 64),
+                              cuuint64_t(c.num_heads), cuuint64_t(c.num_layers) * c.num_pages};
+  const cuuint64_t strides[4] = {row, 128, cuuint64_t(c.head_dim) * 2, row * c.page_size};
+  const cuuint32_t boxes[5] = {64, cuuint32_t(box), 1, 1, 1};
+  const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<__nv_bfloat16 *>(base), dims,
+                strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool make_rows_map(CUtensorMap *map, const __nv_bfloat16 *base, int rows, int row_elems) {
+  EncodeTiledFn encode = encode_tiled_fn();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[2] = {cuuint64_t(row_elems), cuuint64_t(rows)};
+  const cuuint64_t strides[1] = {cuuint64_t(row_elems) * 2};
+  const cuuint32_t box[2] = {64, cuuint32_t(kKeys)};
+  const cuuint32_t steps[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<__nv_bfloat16 *>(base), dims,
+                strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Query rows a partial result can have, and the workspace of one CTA: its meta word
+// and two partial results.
+int partial_rows(int group, int max_row_count) {
+  const int tokens = std::min(kRows / group, max_row_count);
+  return div_up(tokens * group, 8) * 8;
+}
+int64_t workspace_per_cta(int group, int max_row_count) {
+  return 16 + int64_t(partial_rows(group, max_row_count)) * (kPartDims + 2) * 4 * 2;
+}
+
+template <class T>
+cudaError_t launch_chunk(const ChunkAttentionArgs &a, int ctas, cudaStream_t stream) {
+  static_assert(kChunkSmemBytes<T> <= 227 * 1024, "the ring and the small state must fit one SM");
+  const Gemma4KvCacheConfig &c = a.cfg;
+  ChunkParams p = {};
+  p.out = a.out;
+  p.lse = a.lse;
+  p.q = a.q;
+  p.cache_k = a.cache_k;
+  p.cache_v = a.cache_v;
+  p.k_rows = a.k_rows;
+  p.v_rows = a.v_rows;
+  p.cfg = c;
+  p.page_table = a.page_table;
+  p.runs = a.runs;
+  p.layer = a.layer;
+  p.q_heads = a.q_heads;
+  p.group = a.q_heads / c.num_heads;
+  p.tile_tokens = kRows / p.group;
+  p.tiles_per_run = div_up(std::min(a.runs.max_row_count, a.runs.rows), p.tile_tokens);
+  p.window = a.window;
+  p.sinks = a.sinks;
+  p.box = box_tokens(c.page_size);
+  p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  p.rows_cap = partial_rows(p.group, a.runs.max_row_count);
+  p.meta = static_cast<int4 *>(a.workspace);
+  p.partials = reinterpret_cast<float *>(p.meta + ctas);
+  p.status = a.status;
+  CUtensorMap map_k = {}, map_v = {}, map_k_rows = {}, map_v_rows = {};
+  if (p.box > 0 && (!make_cache_map(&map_k, a.cache_k, c, p.box) ||
+                    !make_cache_map(&map_v, a.cache_v, c, p.box))) {
+    return cudaErrorInvalidValue;
   }
+  if (p.box > 0 && a.k_rows != nullptr &&
+      (!make_rows_map(&map_k_rows, a.k_rows, a.runs.rows, c.num_heads * c.head_dim) ||
+       !make_rows_map(&map_v_rows, a.v_rows, a.runs.rows, c.num_heads * c.head_dim))) {
+    return cudaErrorInvalidValue;
+  }
+  cudaError_t st = cudaFuncSetAttribute(chunk_attention_kernel<T>,
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize, kChunkSmemBytes<T>);
+  if (st != cudaSuccess) return st;
+  st = launch_pdl(chunk_attention_kernel<T>, dim3(unsigned(ctas)), dim3(kThreads),
+                  size_t(kChunkSmemBytes<T>), stream, p, map_k, map_v, map_k_rows, map_v_rows);
+  if (st != cudaSuccess) return st;
+  const unsigned row_blocks = unsigned(std::min(4, div_up(p.rows_cap, kCombineWarps)));
+  return launch_pdl(chunk_combine_kernel, dim3(unsigned(ctas), row_blocks), dim3(kCombineWarps * 32), 0,
+                    stream, p, int(c.head_dim));
 }
 
 }  // namespace
@@ -109,7 +1043,7 @@ size_t chunk_workspace_bytes(int q_heads, int kv_heads, int head_dim, int run_co
       sm_count <= 0) {
     return 0;
   }
-  return 16;
+  return size_t(workspace_per_cta(q_heads / kv_heads, max_row_count)) * size_t(sm_count);
 }
 
 cudaError_t validate_chunk_attention(const ChunkAttentionArgs &a) {
@@ -117,9 +1051,17 @@ cudaError_t validate_chunk_attention(const ChunkAttentionArgs &a) {
   if (!valid_chunk_runs(a.runs) || !valid_cache_config(c, a.layer) || a.out == nullptr ||
       a.q == nullptr || a.cache_k == nullptr || a.cache_v == nullptr || a.page_table == nullptr ||
       (a.k_rows == nullptr) != (a.v_rows == nullptr) || a.workspace == nullptr ||
-      a.workspace_bytes < 16 || a.q_heads <= 0 || a.q_heads % c.num_heads != 0 || a.q_heads / c.num_heads > 64 ||
+      a.q_heads <= 0 || a.q_heads % c.num_heads != 0 || a.q_heads / c.num_heads > 64 ||
       (c.head_dim != 256 && c.head_dim != 512) || a.window < 0 || a.sinks < 0 ||
       (a.sinks > 0 && a.window == 0) || !(a.softmax_scale > 0.0f)) {
+    return cudaErrorInvalidValue;
+  }
+  // (run, query tile) pairs that every CTA adds up
+  if (int64_t(a.runs.run_count) * div_up(a.runs.max_row_count, kRows / (a.q_heads / c.num_heads)) >
+      (1 << 24)) {
+    return cudaErrorInvalidValue;
+  }
+  if (int64_t(a.workspace_bytes) < workspace_per_cta(a.q_heads / c.num_heads, a.runs.max_row_count)) {
     return cudaErrorInvalidValue;
   }
   // a ring has its own window and keeps no first tokens; without the runs' rows
@@ -142,14 +1084,17 @@ cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &a, cudaStream_t strea
   const cudaError_t valid = validate_chunk_attention(a);
   if (valid != cudaSuccess) return valid;
   if (a.runs.run_count == 0 || a.runs.rows == 0) return cudaSuccess;
-  const dim3 grid(unsigned(a.runs.max_row_count), unsigned(a.runs.run_count),
-                  unsigned(div_up(a.q_heads, kWarps)));
-  if (a.cfg.head_dim == 256) {
-    chunk_attention_simple_kernel<256><<<grid, kWarps * 32, 0, stream>>>(a);
-  } else {
-    chunk_attention_simple_kernel<512><<<grid, kWarps * 32, 0, stream>>>(a);
-  }
-  return cudaGetLastError();
+  int device = 0, sms = 0;
+  cudaError_t st = cudaGetDevice(&device);
+  if (st != cudaSuccess) return st;
+  st = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  if (st != cudaSuccess) return st;
+  // one CTA per SM, or as many as the workspace has room for
+  const int64_t room = int64_t(a.workspace_bytes) /
+                       workspace_per_cta(a.q_heads / a.cfg.num_heads, a.runs.max_row_count);
+  const int ctas = int(std::min<int64_t>(sms, room));
+  return a.cfg.head_dim == 256 ? launch_chunk<ChunkTraits<256>>(a, ctas, stream)
+                               : launch_chunk<ChunkTraits<512>>(a, ctas, stream);
 }
 
 }  // namespace b200kv

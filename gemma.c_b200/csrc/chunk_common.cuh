@@ -7,6 +7,9 @@
 
 namespace b200kv {
 
+// Positions below this leave room for a key tile's arithmetic in 32 bits.
+constexpr int32_t kMaxPosition = 2147483647 - 1024;
+
 // One run as the device sees it; count 0 where the call skips it.
 struct ChunkRun {
   int32_t batch = 0;
@@ -26,7 +29,7 @@ __device__ __forceinline__ ChunkRun chunk_run(const ChunkRuns &r, int i, int bat
   const bool ok = batch >= 0 && batch < batch_size && first >= 0 && count > 0 &&
                   count <= r.max_row_count && start >= 0 &&
                   int64_t(start) + count <= r.rows &&
-                  int64_t(first) + count <= 2147483647ll;
+                  first <= kMaxPosition - count;
   if (!ok) return run;
   run.batch = batch;
   run.first = first;

@@ -45,10 +45,9 @@
 // through to the common exit, which waits (bounded) for the loads in flight and
 // frees the tensor memory. CTAs that start later return at once. The host clears
 // the word before each launch and reads it through prefill_attention_sm100_fault().
-#include <cuda.h>
-
 #include "common.cuh"
 #include "kernels.cuh"
+#include "umma_common.cuh"
 
 namespace b200kv {
 
@@ -93,107 +92,6 @@ struct Sm100PrefillParams {
   float scale_log2;
 };
 
-// Shared-memory matrix descriptor for a 128-byte-swizzled tile: start address
-// and the two strides in 16-byte units, descriptor version 1, layout type 2.
-__device__ __forceinline__ uint64_t umma_desc(uint32_t smem_addr,
-                                              uint32_t leading_units,
-                                              uint32_t stride_units) {
-  const uint32_t lo = ((smem_addr >> 4) & 0x3fffu) | (leading_units << 16);
-  const uint32_t hi = (stride_units & 0x3fffu) | (1u << 14) | (2u << 29);
-  return (uint64_t(hi) << 32) | lo;
-}
-
-// Instruction descriptor: fp32 accumulate, bf16 x bf16, M = 128.
-__host__ __device__ constexpr uint32_t umma_idesc(uint32_t n, bool b_mn_major) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn_major ? (1u << 16) : 0u) |
-         ((n >> 3) << 17) | ((128u >> 4) << 24);
-}
-
-__device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc,
-                                          uint64_t b_desc, uint32_t idesc,
-                                          bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(uint32_t(accumulate))
-      : "memory");
-}
-// The same with the A operand in tensor memory: lane = row, each 32-bit column
-// two consecutive bf16 of the contraction dimension (8 columns per K = 16).
-__device__ __forceinline__ void umma_bf16_a_tmem(uint32_t d_tmem, uint32_t a_tmem,
-                                                 uint64_t b_desc, uint32_t idesc,
-                                                 bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(uint32_t(accumulate))
-      : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *r) {
-  uint32_t u[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]),
-        "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]),
-        "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
-        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]),
-        "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]),
-        "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
-      : "r"(taddr)
-      : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) r[i] = __uint_as_float(u[i]);
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float *r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(__float_as_uint(r[0])), "r"(__float_as_uint(r[1])),
-      "r"(__float_as_uint(r[2])), "r"(__float_as_uint(r[3])),
-      "r"(__float_as_uint(r[4])), "r"(__float_as_uint(r[5])),
-      "r"(__float_as_uint(r[6])), "r"(__float_as_uint(r[7])),
-      "r"(__float_as_uint(r[8])), "r"(__float_as_uint(r[9])),
-      "r"(__float_as_uint(r[10])), "r"(__float_as_uint(r[11])),
-      "r"(__float_as_uint(r[12])), "r"(__float_as_uint(r[13])),
-      "r"(__float_as_uint(r[14])), "r"(__float_as_uint(r[15])),
-      "r"(__float_as_uint(r[16])), "r"(__float_as_uint(r[17])),
-      "r"(__float_as_uint(r[18])), "r"(__float_as_uint(r[19])),
-      "r"(__float_as_uint(r[20])), "r"(__float_as_uint(r[21])),
-      "r"(__float_as_uint(r[22])), "r"(__float_as_uint(r[23])),
-      "r"(__float_as_uint(r[24])), "r"(__float_as_uint(r[25])),
-      "r"(__float_as_uint(r[26])), "r"(__float_as_uint(r[27])),
-      "r"(__float_as_uint(r[28])), "r"(__float_as_uint(r[29])),
-      "r"(__float_as_uint(r[30])), "r"(__float_as_uint(r[31]))
-      : "memory");
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
-      "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-      "r"(r[14]), "r"(r[15])
-      : "memory");
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
 // One box of 128 rows x 64 elements of a [batch][token][elements] tensor into a
 // swizzled column block; bytes counted on the mbarrier (rows past the sequence
 // arrive as zeros and count all the same).
@@ -204,41 +102,6 @@ __device__ __forceinline__ void tma_load_block(uint32_t dst, const CUtensorMap *
       "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
-}
-
-// kCount fp32 columns of this thread's lane (kCount = 32 or 16)
-template <int kCount>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float *r) {
-  if constexpr (kCount == 32) {
-    tmem_ld32(taddr, r);
-  } else {
-    uint32_t u[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]),
-          "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]),
-          "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
-        : "r"(taddr)
-        : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) r[i] = __uint_as_float(u[i]);
-  }
-}
-// kCount packed bf16 pairs into this thread's lane (kCount = 16 or 8)
-template <int kCount>
-__device__ __forceinline__ void tmem_st_packed(uint32_t taddr, const uint32_t *r) {
-  if constexpr (kCount == 16) {
-    tmem_st16(taddr, r);
-  } else {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
-        "r"(r[7])
-        : "memory");
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-  }
 }
 
 struct Barriers {
@@ -635,26 +498,6 @@ __global__ __launch_bounds__(kThreads, 1) void prefill_attention_sm100_kernel(
                  "r"(kTmemColumns)
                  : "memory");
   }
-}
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
-                                   const cuuint64_t *, const cuuint64_t *,
-                                   const cuuint32_t *, const cuuint32_t *,
-                                   CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled_fn() {
-  static EncodeTiledFn fn = [] {
-    void *ptr = nullptr;
-    cudaDriverEntryPointQueryResult result;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault,
-                                &result) != cudaSuccess ||
-        result != cudaDriverEntryPointSuccess) {
-      return EncodeTiledFn(nullptr);
-    }
-    return reinterpret_cast<EncodeTiledFn>(ptr);
-  }();
-  return fn;
 }
 
 // [batch][token][heads * head_dim] bf16, boxes of box_rows tokens x 64 elements,

@@ -606,8 +606,8 @@ int b200kv_decode_step_plan(const B200KvLayerStepArgs *layers, int32_t layer_cou
  * row_start[i] of every packed [rows, heads, head_dim] tensor. max_row_count
  * >= every row_count[i] (it sizes grids and workspace), rows is the number of
  * rows of those tensors. A run whose sequence, position, count or rows are out
- * of range, or with no rows, is skipped; rows that no run names are left as
- * they were. The runs of one call must name distinct rows and distinct
+ * of range (positions end below 2^31 - 1024), or with no rows, is skipped; rows
+ * that no run names are left as they were. The runs of one call must name distinct rows and distinct
  * sequences' positions. run_count <= B200KV_MAX_RUNS.
  *
  * k_rows / v_rows ([rows, kv_heads, head_dim], both or neither):
@@ -670,7 +670,8 @@ int b200kv_chunk_append_bf16(const B200KvChunkArgs *args, b200kv_stream stream);
  * the first row's window may be given back (-1 in the page table). A row that
  * sees no key gets zeros and an lse of -inf. Values at positions that no row of
  * the call sees are not used, whatever they hold. head_dim 256 or 512, any
- * number of query heads per KV head up to 64.
+ * number G of query heads per KV head up to 64; run_count *
+ * ceil(max_row_count / floor(128 / G)) <= 2^24.
  * `workspace` holds the partial results of rows whose keys several CTAs share;
  * it need not be cleared and nothing is kept in it between calls; calls that may
  * overlap on the GPU (two streams, two captured graphs) need one each. */
