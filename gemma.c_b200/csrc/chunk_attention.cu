@@ -55,7 +55,12 @@ constexpr int kRows = 128;                    // query rows per tile
 constexpr int kKeys = 64;                     // keys per tile
 constexpr int kPartDims = 256;                // output dims per item
 constexpr int kSlotBytes = kKeys * kPartDims * 2;
-constexpr int kBlockBytes = kKeys * 128;      // 64 keys x 64 dims
+// A slot is laid down in groups of eight keys: [key / 8][block of 64 dims][key % 8]
+// [64 dims], 128-byte swizzle. The 8 x 64 atoms of the MMA operands then have one
+// stride between key groups whatever the page size, and one TMA box brings all the
+// groups and blocks that lie in a page.
+constexpr int kGroupBytes = 8 * kPartDims * 2;
+constexpr int kBlockBytes = 8 * 128;
 constexpr int kQBlockBytes = kRows * 128;     // 128 rows x 64 dims
 constexpr int kMaxSlots = 7;
 constexpr int kSoftmaxWarps = 8;
@@ -247,23 +252,23 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&r)[64]) {
   }
 }
 
-// One box of `box` tokens x 64 dims of a page into rows of a swizzled column block.
-__device__ __forceinline__ void tma_load_page_box(uint32_t dst, const CUtensorMap *map, int offset,
-                                                  int block, int head, int page, uint32_t bar) {
+// One box of a page: `box` tokens x 256 dims, token groups of eight from `token_group`.
+__device__ __forceinline__ void tma_load_page_box(uint32_t dst, const CUtensorMap *map, int block,
+                                                  int token_group, int head, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
       "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(offset), "r"(block), "r"(head), "r"(page),
-      "r"(bar)
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(0), "r"(block), "r"(token_group),
+      "r"(head), "r"(bar)
       : "memory");
 }
-// 64 packed rows x 64 dims; rows past the tensor arrive as zeros.
-__device__ __forceinline__ void tma_load_rows_box(uint32_t dst, const CUtensorMap *map, int x, int row,
-                                                  uint32_t bar) {
+// Eight packed rows x 256 dims; rows past the tensor arrive as zeros.
+__device__ __forceinline__ void tma_load_rows_box(uint32_t dst, const CUtensorMap *map, int block,
+                                                  int row, int head, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(block), "r"(head), "r"(bar)
       : "memory");
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
@@ -454,8 +459,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           live &= ~low_bits(s.t0 - p.window + 1 - base) | low_bits(p.sinks - base);
         }
         int64_t row_at[2] = {-1, -1};  // box == 0: element offset of rows lane, lane + 32
-        int page = -1, page_offset = 0;
-        const int piece = lane >> 2;   // box > 0: four lanes per box, one per 64 dims
+        int token_group = -1;          // box > 0: the lane's box of the cache
+        const int piece = lane;
         unsigned long long boxes = 0;
         if (!own && p.box > 0) {
           if (piece * p.box < kKeys) {
@@ -464,9 +469,12 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
             if ((live & bits) != 0) {
               const int position = base + piece * p.box;
               const int logical = position / p.cfg.page_size;
-              page = chunk_page(p.cfg, p.page_table, s.run.batch, logical);
-              page_offset = position - logical * p.cfg.page_size;
-              if (page >= 0) boxes = bits;
+              const int page = chunk_page(p.cfg, p.page_table, s.run.batch, logical);
+              if (page >= 0) {
+                token_group = int((int64_t(p.layer) * p.cfg.num_pages + page) * (p.cfg.page_size / 8) +
+                                  (position - logical * p.cfg.page_size) / 8);
+                boxes = bits;
+              }
             }
           }
           const uint32_t lo = __reduce_or_sync(0xffffffffu, uint32_t(boxes));
@@ -508,12 +516,13 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           const uint32_t dst = s_ring + slot_of(fills) * kSlotBytes;
           if (p.box == 0) {
             const __nv_bfloat16 *from = own ? (is_v ? p.v_rows : p.k_rows) : (is_v ? p.cache_v : p.cache_k);
-            const uint32_t column = dst + uint32_t(lane >> 3) * kBlockBytes;
+            const uint32_t column = dst + uint32_t(lane >> 3) * kBlockBytes;  // + row
 #pragma unroll 8
             for (int r = 0; r < kKeys; ++r) {
               const int64_t at = __shfl_sync(0xffffffffu, row_at[r >> 5], r & 31);
               if (at >= 0) {
-                cp_async16(column + uint32_t(r) * 128u + ((uint32_t(lane & 7) ^ uint32_t(r & 7)) << 4),
+                cp_async16(column + uint32_t(r >> 3) * kGroupBytes + uint32_t(r & 7) * 128u +
+                               ((uint32_t(lane & 7) ^ uint32_t(r & 7)) << 4),
                            from + at + block0 * 64 + lane * 8);
               }
             }
@@ -524,18 +533,16 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           } else if (own) {
             if (lane == 0) mbar_arrive_expect_tx(bar, kSlotBytes);
             __syncwarp();
-            if (lane < 4) {
-              tma_load_rows_box(dst + uint32_t(lane) * kBlockBytes, is_v ? &map_v_rows : &map_k_rows,
-                                head * T::kHeadDim + (block0 + lane) * 64,
-                                s.run.start + k * kKeys, bar);
+            if (lane < kKeys / 8) {
+              tma_load_rows_box(dst + uint32_t(lane) * kGroupBytes, is_v ? &map_v_rows : &map_k_rows,
+                                block0, s.run.start + k * kKeys + lane * 8, head, bar);
             }
           } else {
             if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(__popcll(boxes)) * (kPartDims * 2));
             __syncwarp();
-            if (page >= 0) {
-              tma_load_page_box(dst + uint32_t(lane & 3) * kBlockBytes + uint32_t(piece * p.box) * 128u,
-                                is_v ? &map_v : &map_k, page_offset, block0 + (lane & 3), head,
-                                p.layer * p.cfg.num_pages + page, bar);
+            if (token_group >= 0) {
+              tma_load_page_box(dst + uint32_t(piece * p.box / 8) * kGroupBytes, is_v ? &map_v : &map_k,
+                                block0, token_group, head, bar);
             }
           }
         }
@@ -559,8 +566,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       int segments = 0;
       Segment s;
       bool ok = true;
-      // O (+)= P V: four steps of 16 keys; 8-key groups 1024 bytes apart, 64-dim
-      // blocks one column block apart (MN-major)
+      // O (+)= P V: four steps of 16 keys (MN-major)
       auto issue_pv = [&](int tile, bool accumulate) -> bool {
         const int fill = tile * T::kTileSlots + T::kKSlots;
         const uint32_t b = uint32_t(tile & 1);
@@ -571,7 +577,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
 #pragma unroll
         for (int i = 0; i < kKeys / 16; ++i) {
           umma_bf16_a_tmem(tmem, tmem + kTmemS + b * kKeys + 8u * uint32_t(i),
-                           umma_desc(v + uint32_t(i) * 2048u, kBlockBytes >> 4, 64), kIdescPV,
+                           umma_desc(v + uint32_t(i) * 2u * kGroupBytes, kBlockBytes >> 4,
+                                     kGroupBytes >> 4), kIdescPV,
                            accumulate || i > 0);
         }
         umma_commit(bar_done + 8u * slot_of(fill));
@@ -597,7 +604,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
 #pragma unroll
             for (int i = 0; i < 16; ++i) {  // steps of 16 dims, four to a column block
               const uint32_t in = uint32_t(i & 3) * 32u;
-              const uint64_t kd = umma_desc(k + uint32_t(i >> 2) * kBlockBytes + in, 1, 64);
+              const uint64_t kd = umma_desc(k + uint32_t(i >> 2) * kBlockBytes + in, 1,
+                                            kGroupBytes >> 4);
               if (f == 0) {
                 umma_bf16_a_tmem(d, tmem + kTmemQ + 8u * uint32_t(i), kd, kIdescQK, i > 0);
               } else {
@@ -762,7 +770,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           uint8_t *v = smem_raw + T::kQHiBytes + slot_of(fill) * kSlotBytes + (lane >> 3) * kBlockBytes +
                        (lane & 7) * 16;
           for (int r = quarter; r < kKeys; r += 4) {
-            if (((info.live >> r) & 1ull) == 0) *reinterpret_cast<uint4 *>(v + r * 128) = make_uint4(0, 0, 0, 0);
+            if (((info.live >> r) & 1ull) == 0) {
+              *reinterpret_cast<uint4 *>(v + (r >> 3) * kGroupBytes + (r & 7) * 128) = make_uint4(0, 0, 0, 0);
+            }
           }
           fence_proxy_async_shared();
         }
@@ -952,25 +962,28 @@ bool make_cache_map(CUtensorMap *map, const __nv_bfloat16 *base, const Gemma4KvC
   EncodeTiledFn encode = encode_tiled_fn();
   if (encode == nullptr) return false;
   const cuuint64_t row = cuuint64_t(c.num_heads) * c.head_dim * 2;
-  // [page][head][block of 64 dims][offset in page][64 dims]
-  const cuuint64_t dims[5] = {64, cuuint64_t(c.page_size), cuuint64_t(c.head_dim / 64),
-                              cuuint64_t(c.num_heads), cuuint64_t(c.num_layers) * c.num_pages};
-  const cuuint64_t strides[4] = {row, 128, cuuint64_t(c.head_dim) * 2, row * c.page_size};
-  const cuuint32_t boxes[5] = {64, cuuint32_t(box), 1, 1, 1};
+  // [head][group of 8 tokens][block of 64 dims][token of the group][64 dims]: the
+  // pages of all layers are one row of tokens, of which a box takes whole groups
+  const cuuint64_t dims[5] = {64, 8, cuuint64_t(c.head_dim / 64),
+                              cuuint64_t(c.num_layers) * c.num_pages * (c.page_size / 8),
+                              cuuint64_t(c.num_heads)};
+  const cuuint64_t strides[4] = {row, 128, row * 8, cuuint64_t(c.head_dim) * 2};
+  const cuuint32_t boxes[5] = {64, 8, kPartDims / 64, cuuint32_t(box / 8), 1};
   const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<__nv_bfloat16 *>(base), dims,
                 strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool make_rows_map(CUtensorMap *map, const __nv_bfloat16 *base, int rows, int row_elems) {
+bool make_rows_map(CUtensorMap *map, const __nv_bfloat16 *base, int rows, int heads, int head_dim) {
   EncodeTiledFn encode = encode_tiled_fn();
   if (encode == nullptr) return false;
-  const cuuint64_t dims[2] = {cuuint64_t(row_elems), cuuint64_t(rows)};
-  const cuuint64_t strides[1] = {cuuint64_t(row_elems) * 2};
-  const cuuint32_t box[2] = {64, cuuint32_t(kKeys)};
-  const cuuint32_t steps[2] = {1, 1};
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<__nv_bfloat16 *>(base), dims,
+  const cuuint64_t row = cuuint64_t(heads) * head_dim * 2;
+  const cuuint64_t dims[4] = {64, cuuint64_t(rows), cuuint64_t(head_dim / 64), cuuint64_t(heads)};
+  const cuuint64_t strides[3] = {row, 128, cuuint64_t(head_dim) * 2};
+  const cuuint32_t box[4] = {64, 8, kPartDims / 64, 1};
+  const cuuint32_t steps[4] = {1, 1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16 *>(base), dims,
                 strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1019,8 +1032,8 @@ cudaError_t launch_chunk(const ChunkAttentionArgs &a, int ctas, cudaStream_t str
     return cudaErrorInvalidValue;
   }
   if (p.box > 0 && a.k_rows != nullptr &&
-      (!make_rows_map(&map_k_rows, a.k_rows, a.runs.rows, c.num_heads * c.head_dim) ||
-       !make_rows_map(&map_v_rows, a.v_rows, a.runs.rows, c.num_heads * c.head_dim))) {
+      (!make_rows_map(&map_k_rows, a.k_rows, a.runs.rows, c.num_heads, c.head_dim) ||
+       !make_rows_map(&map_v_rows, a.v_rows, a.runs.rows, c.num_heads, c.head_dim))) {
     return cudaErrorInvalidValue;
   }
   cudaError_t st = cudaFuncSetAttribute(chunk_attention_kernel<T>,
