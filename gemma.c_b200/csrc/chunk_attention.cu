@@ -559,71 +559,78 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     }
   } else if (warp == kSoftmaxWarps + 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t kIdescQK = umma_idesc(kKeys, false);
-      constexpr uint32_t kIdescPV = umma_idesc(kPartDims, true);
-      int n = 0;         // key tiles so far
-      int segments = 0;
-      Segment s;
-      bool ok = true;
-      // O (+)= P V: four steps of 16 keys (MN-major)
-      auto issue_pv = [&](int tile, bool accumulate) -> bool {
-        const int fill = tile * T::kTileSlots + T::kKSlots;
-        const uint32_t b = uint32_t(tile & 1);
-        if (!wait(bar_full + 8u * slot_of(fill), parity_of(fill))) return false;
-        if (!wait(bar_p_full + 8u * b, uint32_t(tile >> 1) & 1u)) return false;
-        tc_fence_after();
-        const uint32_t v = s_ring + slot_of(fill) * kSlotBytes;
+    constexpr uint32_t kIdescQK = umma_idesc(kKeys, false);
+    constexpr uint32_t kIdescPV = umma_idesc(kPartDims, true);
+    // descriptor words of a slot's tile: K (K-major; the leading stride is not used)
+    // and V (MN-major), and of the upper half of Q
+    constexpr uint32_t kLoK = 1u << 16;
+    constexpr uint32_t kLoV = uint32_t(kBlockBytes >> 4) << 16;
+    constexpr uint32_t kHiSlot = uint32_t(kGroupBytes >> 4) | (1u << 14) | (2u << 29);
+    constexpr uint32_t kHiQ = 64u | (1u << 14) | (2u << 29);
+    const bool leader = elect_one();
+    int n = 0;  // key tiles so far
+    int segments = 0;
+    Segment s;
+    bool ok = true;
+    auto warp_wait = [&](uint32_t bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, wait(bar, parity));
+    };
+    // O (+)= P V: four steps of 16 keys
+    auto issue_pv = [&](int tile, bool accumulate) -> bool {
+      const int fill = tile * T::kTileSlots + T::kKSlots;
+      const uint32_t b = uint32_t(tile & 1);
+      if (!warp_wait(bar_full + 8u * slot_of(fill), parity_of(fill))) return false;
+      if (!warp_wait(bar_p_full + 8u * b, uint32_t(tile >> 1) & 1u)) return false;
+      tc_fence_after();
+      const uint32_t v = ((s_ring + slot_of(fill) * kSlotBytes) >> 4) | kLoV;
+      const uint32_t w = tmem + kTmemS + b * kKeys;
 #pragma unroll
-        for (int i = 0; i < kKeys / 16; ++i) {
-          umma_bf16_a_tmem(tmem, tmem + kTmemS + b * kKeys + 8u * uint32_t(i),
-                           umma_desc(v + uint32_t(i) * 2u * kGroupBytes, kBlockBytes >> 4,
-                                     kGroupBytes >> 4), kIdescPV,
-                           accumulate || i > 0);
-        }
-        umma_commit(bar_done + 8u * slot_of(fill));
-        return true;
-      };
-      while (ok && walk.next(p, s)) {
-        ok = wait(bar_q_full, uint32_t(segments & 1));
-        for (int j = s.begin; j < s.end && ok; ++j, ++n) {
-          // S[n & 1] held the weights of tile n - 2
-          if (n >= 2) {
-            const int fill = (n - 2) * T::kTileSlots + T::kKSlots;
-            ok = wait(bar_done + 8u * slot_of(fill), parity_of(fill));
-            if (!ok) break;
-          }
-          const uint32_t d = tmem + kTmemS + uint32_t(n & 1) * kKeys;
-#pragma unroll
-          for (int f = 0; f < T::kKSlots; ++f) {
-            const int fill = n * T::kTileSlots + f;
-            ok = ok && wait(bar_full + 8u * slot_of(fill), parity_of(fill));
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t k = s_ring + slot_of(fill) * kSlotBytes;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {  // steps of 16 dims, four to a column block
-              const uint32_t in = uint32_t(i & 3) * 32u;
-              const uint64_t kd = umma_desc(k + uint32_t(i >> 2) * kBlockBytes + in, 1,
-                                            kGroupBytes >> 4);
-              if (f == 0) {
-                umma_bf16_a_tmem(d, tmem + kTmemQ + 8u * uint32_t(i), kd, kIdescQK, i > 0);
-              } else {
-                umma_bf16(d, umma_desc(s_q_hi + uint32_t(i >> 2) * kQBlockBytes + in, 1, 64), kd,
-                          kIdescQK, true);
-              }
-            }
-            umma_commit(bar_done + 8u * slot_of(fill));
-          }
-          if (!ok) break;
-          umma_commit(bar_s_full + 8u * uint32_t(n & 1));
-          if (j > s.begin) ok = issue_pv(n - 1, j - 1 > s.begin);
-          // the segment's first P V writes O anew: the last segment's rows must be out
-          if (j == s.begin && segments > 0) ok = wait(bar_o_free, uint32_t(segments - 1) & 1u);
-        }
-        if (ok) ok = issue_pv(n - 1, s.end - s.begin > 1);
-        ++segments;
+      for (int i = 0; i < kKeys / 16; ++i) {
+        umma_bf16_a_tmem_warp(tmem, w + 8u * uint32_t(i), v + uint32_t(i) * (2u * kGroupBytes >> 4),
+                              kHiSlot, kIdescPV, accumulate || i > 0, leader);
       }
+      umma_commit_warp(bar_done + 8u * slot_of(fill), leader);
+      return true;
+    };
+    while (ok && walk.next(p, s)) {
+      ok = warp_wait(bar_q_full, uint32_t(segments & 1));
+      for (int j = s.begin; j < s.end && ok; ++j, ++n) {
+        // S[n & 1] held the weights of tile n - 2
+        if (n >= 2) {
+          const int fill = (n - 2) * T::kTileSlots + T::kKSlots;
+          ok = warp_wait(bar_done + 8u * slot_of(fill), parity_of(fill));
+          if (!ok) break;
+        }
+        const uint32_t d = tmem + kTmemS + uint32_t(n & 1) * kKeys;
+#pragma unroll
+        for (int f = 0; f < T::kKSlots; ++f) {
+          const int fill = n * T::kTileSlots + f;
+          ok = ok && warp_wait(bar_full + 8u * slot_of(fill), parity_of(fill));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t k = ((s_ring + slot_of(fill) * kSlotBytes) >> 4) | kLoK;
+          const uint32_t q_hi = (s_q_hi >> 4) | kLoK;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {  // steps of 16 dims, four to a block
+            const uint32_t at = uint32_t(i >> 2) * (kBlockBytes >> 4) + uint32_t(i & 3) * 2u;
+            if (f == 0) {
+              umma_bf16_a_tmem_warp(d, tmem + kTmemQ + 8u * uint32_t(i), k + at, kHiSlot, kIdescQK,
+                                    i > 0, leader);
+            } else {
+              umma_bf16_warp(d, q_hi + uint32_t(i >> 2) * (kQBlockBytes >> 4) + uint32_t(i & 3) * 2u,
+                             kHiQ, k + at, kHiSlot, kIdescQK, true, leader);
+            }
+          }
+          umma_commit_warp(bar_done + 8u * slot_of(fill), leader);
+        }
+        if (!ok) break;
+        umma_commit_warp(bar_s_full + 8u * uint32_t(n & 1), leader);
+        if (j > s.begin) ok = issue_pv(n - 1, j - 1 > s.begin);
+        // the segment's first P V writes O anew: the last segment's rows must be out
+        if (j == s.begin && segments > 0) ok = warp_wait(bar_o_free, uint32_t(segments - 1) & 1u);
+      }
+      if (ok) ok = issue_pv(n - 1, s.end - s.begin > 1);
+      ++segments;
     }
   } else {
     // ------------------------------------------------------------ softmax

@@ -44,6 +44,47 @@ __device__ __forceinline__ void umma_bf16_a_tmem(uint32_t d_tmem, uint32_t a_tme
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(uint32_t(accumulate))
       : "memory");
 }
+// The same two for a whole warp that issues through one lane (`leader` true in one
+// lane): the operands are then computed once for the warp, not in a divergent
+// branch, which is what an issue every 32 clocks takes. The descriptors come as a
+// low word (address, leading stride) to which constants can be added (addresses are
+// below 2^14 units of 16 bytes, so nothing carries out of the field) and a high word.
+__device__ __forceinline__ void umma_bf16_warp(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi,
+                                               uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                               bool accumulate, bool leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+      "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(uint32_t(accumulate)),
+      "r"(uint32_t(leader))
+      : "memory");
+}
+__device__ __forceinline__ void umma_bf16_a_tmem_warp(uint32_t d_tmem, uint32_t a_tmem,
+                                                      uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                                      bool accumulate, bool leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(uint32_t(accumulate)), "r"(uint32_t(leader))
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_warp(uint32_t bar, bool leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar),
+      "r"(uint32_t(leader))
+      : "memory");
+}
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(pred));
+  return pred != 0;
+}
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile(
       "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
