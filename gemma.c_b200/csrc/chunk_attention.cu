@@ -14,12 +14,14 @@
 // item's keys writes the item's rows; a piece of an item leaves its rows' maximum,
 // sum and accumulator in the workspace, and chunk_combine_kernel joins them.
 //
-// One CTA: ten warps.
+// One CTA: eleven warps.
 //   warps 0-7  softmax: two groups of four warps, a thread per query row; group g
 //              takes the key tiles with number n % 2 == g
-//   warp 8     loads K and V tiles (TMA boxes that lie inside one page, or 16-byte
-//              copies where pages are no multiple of eight tokens)
-//   warp 9     one thread issues the MMAs
+//   warps 8, 9 load K and V tiles (TMA boxes that lie inside one page, or 16-byte
+//              copies where pages are no multiple of eight tokens); a box costs its
+//              warp about 130 clocks, a page-table entry a round trip, so the tensors
+//              have a warp each and look a tile ahead
+//   warp 10    issues the MMAs
 // Tensor memory (512 columns): O (128 x 256 fp32), Q (128 x 256 bf16: the A operand
 // of Q K^T), and two score buffers of 64 columns; the weights go back as bf16 over
 // the scores they come from and are the A operand of P V. Shared memory holds
@@ -64,7 +66,7 @@ constexpr int kBlockBytes = 8 * 128;
 constexpr int kQBlockBytes = kRows * 128;     // 128 rows x 64 dims
 constexpr int kMaxSlots = 7;
 constexpr int kSoftmaxWarps = 8;
-constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
+constexpr int kThreads = (kSoftmaxWarps + 3) * 32;
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kTmemQ = 256;
 constexpr uint32_t kTmemS = 384;              // + 64 * buffer
@@ -87,6 +89,21 @@ struct ChunkTraits {
   static constexpr int kTileBytes = kQHiBytes + kSlots * kSlotBytes;
 };
 
+// Division of 0 .. 2^31 - 1 by a fixed number: the quotient's high part by a 32-bit
+// multiplication (Granlund and Montgomery's round-up method).
+struct FastDiv {
+  uint32_t d, m, shift;
+  __device__ __forceinline__ int quotient(int n) const {
+    return int((__umulhi(uint32_t(n), m) + uint32_t(n)) >> shift);
+  }
+  static FastDiv by(uint32_t d) {
+    FastDiv f = {d, 0, 0};
+    while ((1ull << f.shift) < d) ++f.shift;
+    f.m = uint32_t(((1ull << 32) * ((1ull << f.shift) - d)) / d + 1);
+    return f;
+  }
+};
+
 struct ChunkParams {
   __nv_bfloat16 *out;
   float *lse;
@@ -106,6 +123,8 @@ struct ChunkParams {
   int32_t window;
   int32_t sinks;
   int32_t box;           // tokens per TMA box; 0: rows are copied one by one
+  FastDiv page_div;      // by page_size
+  FastDiv slot_div;      // by max_pages_per_seq
   float scale_log2;
   int4 *meta;            // per CTA: see PartialMeta
   float *partials;       // [cta][2] x (acc [rows_cap][256], m [rows_cap], l [rows_cap])
@@ -196,6 +215,18 @@ struct Walk {
   }
 };
 
+// chunk_page without its divisions.
+__device__ __forceinline__ int logical_to_page(const ChunkParams &p, int batch, int logical) {
+  const int slots = p.cfg.max_pages_per_seq;
+  if (p.cfg.window_size == 0) {
+    if (logical >= slots) return -1;
+  } else {
+    logical -= p.slot_div.quotient(logical) * slots;
+  }
+  const int page = __ldg(p.page_table + int64_t(batch) * slots + logical);
+  return page < p.cfg.num_pages ? page : -1;
+}
+
 // What the softmax needs to know about a key tile, left by the loader.
 struct TileInfo {
   unsigned long long live;  // keys that some row of the query tile sees
@@ -207,7 +238,7 @@ struct SmallState {
   uint64_t full[kMaxSlots];   // the slot's tile has landed
   uint64_t done[kMaxSlots];   // the MMAs that read the slot are complete
   uint64_t s_full[2];         // scores of the tile in S[b] complete
-  uint64_t p_full[2];         // its weights written (and O rescaled where needed)
+  uint64_t p_full[2][2];      // half of its weights written (and O rescaled where needed)
   uint64_t m_full[2][4];      // row_ref[b] of 32 rows written
   uint64_t l_full[2][4];      // row_sum of 32 rows written by the group
   uint64_t q_full;            // Q of the segment in tensor memory
@@ -302,7 +333,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   const uint32_t bar_full = smem_u32(&small.full[0]);      // + 8 slot
   const uint32_t bar_done = smem_u32(&small.done[0]);      // + 8 slot
   const uint32_t bar_s_full = smem_u32(&small.s_full[0]);  // + 8 b
-  const uint32_t bar_p_full = smem_u32(&small.p_full[0]);  // + 8 b
+  const uint32_t bar_p_full = smem_u32(&small.p_full[0][0]);  // + 16 b + 8 half
   const uint32_t bar_m_full = smem_u32(&small.m_full[0][0]);  // + 32 b + 8 warp quarter
   const uint32_t bar_l_full = smem_u32(&small.l_full[0][0]);  // + 32 group + 8 warp quarter
   const uint32_t bar_q_full = smem_u32(&small.q_full);
@@ -314,7 +345,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_s_full + 8u * b, 1);
-      mbar_init(bar_p_full + 8u * b, 4);
+      mbar_init(bar_p_full + 16u * b, 4);
+      mbar_init(bar_p_full + 16u * b + 8u, 4);
       for (int w = 0; w < 4; ++w) {
         mbar_init(bar_m_full + 32u * b + 8u * w, 1);
         mbar_init(bar_l_full + 32u * b + 8u * w, 1);
@@ -420,144 +452,168 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   auto slot_of = [](int fill) { return uint32_t(fill % kSlots); };
   auto parity_of = [](int fill) { return uint32_t(fill / kSlots) & 1u; };
 
-  if (warp == kSoftmaxWarps) {
-    // ------------------------------------------------------------ loader
-    int fills = 0;
-    int tile_number = 0;
-    int4 meta = make_int4(-1, 0, 0, 0);
+  if (warp == kSoftmaxWarps || warp == kSoftmaxWarps + 1) {
+    // ------------------------------------------------------------ loaders of K and V
+    const bool is_v = warp == kSoftmaxWarps + 1;
+    // A key tile as the loader sees it: where it lies, which of its keys somebody sees
+    // (pages aside), and this lane's page-table entries, asked for a tile ahead.
+    struct Tile {
+      unsigned long long live;
+      int base, t0, t1;
+      int head, part;
+      int row0;      // of the own rows; -1: in the cache
+      int page[2];   // box > 0: of the lane's box; else of rows lane and lane + 32
+      int offset[2]; // in the page
+    };
     Segment s;
-    bool ok = true;
+    int j = 0;
+    s.end = 0;
+    int4 meta = make_int4(-1, 0, 0, 0);
+    auto look_up = [&](Tile &t) -> bool {
+      if (j >= s.end) {
+        if (!walk.next(p, s)) return false;
+        j = s.begin;
+        if (s.begin > 0) meta.w = s.end == s.total ? 1 : 2;
+        if (s.begin == 0 && s.end < s.total) {
+          meta.x = s.hp;
+          meta.y = s.run_index;
+          meta.z = s.query_tile;
+        }
+      }
+      int k = j++;
+      bool own = false;
+      if (k < s.keys.ca) {
+      } else if ((k -= s.keys.ca) < s.keys.cb1 - s.keys.cb0) {
+        k += s.keys.cb0;
+      } else {
+        k -= s.keys.cb1 - s.keys.cb0;
+        own = true;
+        if (k >= s.keys.oa) k += s.keys.ob0 - s.keys.oa;
+      }
+      t.head = s.hp % heads;
+      t.part = s.hp / heads;
+      t.t0 = s.t0;
+      t.t1 = s.t1;
+      t.base = (own ? s.run.first : 0) + k * kKeys;
+      t.row0 = own ? s.run.start + k * kKeys : -1;
+      t.live = low_bits(s.t1 + 1 - t.base);
+      if (!own && p.k_rows != nullptr) t.live &= low_bits(s.run.first - t.base);
+      if (p.window > 0) {
+        t.live &= ~low_bits(s.t0 - p.window + 1 - t.base) | low_bits(p.sinks - t.base);
+      }
+      t.page[0] = t.page[1] = -1;
+      if (!own) {
+        const int step = p.box > 0 ? p.box : 32;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int at = p.box > 0 ? lane * p.box : lane + 32 * i;
+          if (at >= kKeys || (p.box > 0 && i == 1)) continue;
+          const unsigned long long bits =
+              p.box > 0 ? (step == 64 ? ~0ull : ((1ull << step) - 1ull) << at) : 1ull << at;
+          if ((t.live & bits) == 0) continue;
+          const int logical = p.page_div.quotient(t.base + at);
+          t.offset[i] = t.base + at - logical * p.cfg.page_size;
+          t.page[i] = logical_to_page(p, s.run.batch, logical);
+        }
+      }
+      return true;
+    };
     auto claim = [&](int fill) -> bool {  // the slot's last reader is done
       const bool free = fill < kSlots || wait(bar_done + 8u * slot_of(fill), parity_of(fill) ^ 1u);
       return __all_sync(0xffffffffu, free);
     };
-    while (ok && walk.next(p, s)) {
-      if (s.begin > 0) meta.w = s.end == s.total ? 1 : 2;
-      if (s.begin == 0 && s.end < s.total) {
-        meta.x = s.hp;
-        meta.y = s.run_index;
-        meta.z = s.query_tile;
+    Tile t, ahead;
+    bool more = look_up(t);
+    bool ok = true;
+    int n = 0;
+    for (; more && ok; ++n) {
+      const bool more_ahead = look_up(ahead);
+      const bool own = t.row0 >= 0;
+      unsigned long long mapped = ~0ull;  // keys whose page exists
+      if (!own && p.box > 0) {
+        unsigned long long bits = 0;
+        if (t.page[0] >= 0) {
+          bits = p.box == 64 ? ~0ull : ((1ull << p.box) - 1ull) << (lane * p.box);
+        }
+        const uint32_t lo = __reduce_or_sync(0xffffffffu, uint32_t(bits));
+        const uint32_t hi = __reduce_or_sync(0xffffffffu, uint32_t(bits >> 32));
+        mapped = (uint64_t(hi) << 32) | lo;
+      } else if (!own) {
+        const uint32_t lo = __ballot_sync(0xffffffffu, t.page[0] >= 0);
+        const uint32_t hi = __ballot_sync(0xffffffffu, t.page[1] >= 0);
+        mapped = (uint64_t(hi) << 32) | lo;
       }
-      const int head = s.hp % heads;
-      const int part = s.hp / heads;
-      for (int j = s.begin; j < s.end; ++j, ++tile_number) {
-        // where the tile lies and which of its keys anyone sees
-        int k = j;
-        bool own = false;
-        if (k < s.keys.ca) {
-        } else if ((k -= s.keys.ca) < s.keys.cb1 - s.keys.cb0) {
-          k += s.keys.cb0;
-        } else {
-          k -= s.keys.cb1 - s.keys.cb0;
-          own = true;
-          if (k >= s.keys.oa) k += s.keys.ob0 - s.keys.oa;
+      const unsigned long long live = t.live & mapped;
+#pragma unroll
+      for (int f = 0; f < T::kKSlots; ++f) {
+        if (is_v && f > 0) break;
+        const int fill = n * T::kTileSlots + (is_v ? T::kKSlots : f);
+        const int block0 = is_v ? t.part * 4 : f * 4;
+        ok = claim(fill);
+        if (!ok) break;
+        if (!is_v && f == 0 && lane == 0) {
+          const bool edge = live != ~0ull || t.base + kKeys - 1 > t.t0 ||
+                            (p.window > 0 && t.base <= t.t1 - p.window && t.base + kKeys > p.sinks);
+          small.info[n % kInfos] = {live, t.base, edge ? 1 : 0};
         }
-        const int base = (own ? s.run.first : 0) + k * kKeys;
-        unsigned long long live = low_bits(s.t1 + 1 - base);
-        if (!own && p.k_rows != nullptr) live &= low_bits(s.run.first - base);
-        if (p.window > 0) {
-          live &= ~low_bits(s.t0 - p.window + 1 - base) | low_bits(p.sinks - base);
-        }
-        int64_t row_at[2] = {-1, -1};  // box == 0: element offset of rows lane, lane + 32
-        int token_group = -1;          // box > 0: the lane's box of the cache
-        const int piece = lane;
-        unsigned long long boxes = 0;
-        if (!own && p.box > 0) {
-          if (piece * p.box < kKeys) {
-            const unsigned long long bits =
-                (p.box == 64 ? ~0ull : (1ull << p.box) - 1ull) << (piece * p.box);
-            if ((live & bits) != 0) {
-              const int position = base + piece * p.box;
-              const int logical = position / p.cfg.page_size;
-              const int page = chunk_page(p.cfg, p.page_table, s.run.batch, logical);
-              if (page >= 0) {
-                token_group = int((int64_t(p.layer) * p.cfg.num_pages + page) * (p.cfg.page_size / 8) +
-                                  (position - logical * p.cfg.page_size) / 8);
-                boxes = bits;
-              }
-            }
-          }
-          const uint32_t lo = __reduce_or_sync(0xffffffffu, uint32_t(boxes));
-          const uint32_t hi = __reduce_or_sync(0xffffffffu, uint32_t(boxes >> 32));
-          boxes = (uint64_t(hi) << 32) | lo;
-          live &= boxes;
-        } else if (p.box == 0) {
+        const uint32_t bar = bar_full + 8u * slot_of(fill);
+        const uint32_t dst = s_ring + slot_of(fill) * kSlotBytes;
+        if (p.box == 0) {
+          const __nv_bfloat16 *from = own ? (is_v ? p.v_rows : p.k_rows) : (is_v ? p.cache_v : p.cache_k);
+          int64_t row_at[2];  // element offset of rows lane, lane + 32
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int r = lane + 32 * i;
-            if (((live >> r) & 1ull) == 0) continue;
-            if (own) {
-              row_at[i] = ((int64_t(s.run.start) + k * kKeys + r) * heads + head) * T::kHeadDim;
-            } else {
-              const int logical = (base + r) / p.cfg.page_size;
-              const int at = chunk_page(p.cfg, p.page_table, s.run.batch, logical);
-              if (at >= 0) {
-                row_at[i] = cache_offset(p.cfg, p.layer, at, base + r - logical * p.cfg.page_size,
-                                         head, 0);
-              }
-            }
+            row_at[i] = -1;
+            if (((live >> (lane + 32 * i)) & 1ull) == 0) continue;
+            row_at[i] = own ? ((int64_t(t.row0) + lane + 32 * i) * heads + t.head) * T::kHeadDim
+                            : cache_offset(p.cfg, p.layer, t.page[i], t.offset[i], t.head, 0);
           }
-          const uint32_t lo = __ballot_sync(0xffffffffu, row_at[0] >= 0);
-          const uint32_t hi = __ballot_sync(0xffffffffu, row_at[1] >= 0);
-          live &= (uint64_t(hi) << 32) | lo;
-        }
-        const bool edge = live != ~0ull || base + kKeys - 1 > s.t0 ||
-                          (p.window > 0 && base <= s.t1 - p.window && base + kKeys > p.sinks);
-        if (lane == 0) small.info[tile_number % kInfos] = {live, base, edge ? 1 : 0};
-        __syncwarp();
-        // K slots, then the V slot
-#pragma unroll
-        for (int f = 0; f < T::kTileSlots; ++f, ++fills) {
-          const bool is_v = f == T::kKSlots;
-          const int block0 = is_v ? part * 4 : f * 4;
-          ok = claim(fills);
-          if (!ok) break;
-          const uint32_t bar = bar_full + 8u * slot_of(fills);
-          const uint32_t dst = s_ring + slot_of(fills) * kSlotBytes;
-          if (p.box == 0) {
-            const __nv_bfloat16 *from = own ? (is_v ? p.v_rows : p.k_rows) : (is_v ? p.cache_v : p.cache_k);
-            const uint32_t column = dst + uint32_t(lane >> 3) * kBlockBytes;  // + row
+          const uint32_t column = dst + uint32_t(lane >> 3) * kBlockBytes;
 #pragma unroll 8
-            for (int r = 0; r < kKeys; ++r) {
-              const int64_t at = __shfl_sync(0xffffffffu, row_at[r >> 5], r & 31);
-              if (at >= 0) {
-                cp_async16(column + uint32_t(r >> 3) * kGroupBytes + uint32_t(r & 7) * 128u +
-                               ((uint32_t(lane & 7) ^ uint32_t(r & 7)) << 4),
-                           from + at + block0 * 64 + lane * 8);
-              }
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_proxy_async_shared();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
-          } else if (own) {
-            if (lane == 0) mbar_arrive_expect_tx(bar, kSlotBytes);
-            __syncwarp();
-            if (lane < kKeys / 8) {
-              tma_load_rows_box(dst + uint32_t(lane) * kGroupBytes, is_v ? &map_v_rows : &map_k_rows,
-                                block0, s.run.start + k * kKeys + lane * 8, head, bar);
-            }
-          } else {
-            if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(__popcll(boxes)) * (kPartDims * 2));
-            __syncwarp();
-            if (token_group >= 0) {
-              tma_load_page_box(dst + uint32_t(piece * p.box / 8) * kGroupBytes, is_v ? &map_v : &map_k,
-                                block0, token_group, head, bar);
+          for (int r = 0; r < kKeys; ++r) {
+            const int64_t at = __shfl_sync(0xffffffffu, row_at[r >> 5], r & 31);
+            if (at >= 0) {
+              cp_async16(column + uint32_t(r >> 3) * kGroupBytes + uint32_t(r & 7) * 128u +
+                             ((uint32_t(lane & 7) ^ uint32_t(r & 7)) << 4),
+                         from + at + block0 * 64 + lane * 8);
             }
           }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar);
+        } else if (own) {
+          if (lane == 0) mbar_arrive_expect_tx(bar, kSlotBytes);
+          __syncwarp();
+          if (lane < kKeys / 8) {
+            tma_load_rows_box(dst + uint32_t(lane) * kGroupBytes, is_v ? &map_v_rows : &map_k_rows,
+                              block0, t.row0 + lane * 8, t.head, bar);
+          }
+        } else {
+          if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(__popcll(mapped)) * (kPartDims * 2));
+          __syncwarp();
+          if (t.page[0] >= 0) {
+            const int token_group = (p.layer * p.cfg.num_pages + t.page[0]) * (p.cfg.page_size / 8) +
+                                    t.offset[0] / 8;
+            tma_load_page_box(dst + uint32_t(lane * p.box / 8) * kGroupBytes, is_v ? &map_v : &map_k,
+                              block0, token_group, t.head, bar);
+          }
         }
-        if (!ok) break;
       }
+      t = ahead;
+      more = more_ahead;
     }
-    if (lane == 0) p.meta[blockIdx.x] = meta;
+    if (!is_v && lane == 0) p.meta[blockIdx.x] = meta;
     if (!ok || *abort_flag != 0) {
       // nobody may be waiting for the last loads any more: see them land before the
       // CTA gives its shared memory back
-      for (int i = max(0, fills - kSlots); i < fills; ++i) {
-        mbar_wait_bounded(bar_full + 8u * slot_of(i), parity_of(i), kTileWaitClocks);
+      for (int i = max(0, (n + 1) * T::kTileSlots - 2 * kSlots); i < n * T::kTileSlots; ++i) {
+        if ((i % T::kTileSlots == T::kKSlots) == is_v) {
+          mbar_wait_bounded(bar_full + 8u * slot_of(i), parity_of(i), kTileWaitClocks);
+        }
       }
     }
-  } else if (warp == kSoftmaxWarps + 1) {
+  } else if (warp == kSoftmaxWarps + 2) {
     // ------------------------------------------------------------ MMA issuer
     constexpr uint32_t kIdescQK = umma_idesc(kKeys, false);
     constexpr uint32_t kIdescPV = umma_idesc(kPartDims, true);
@@ -580,12 +636,14 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       const int fill = tile * T::kTileSlots + T::kKSlots;
       const uint32_t b = uint32_t(tile & 1);
       if (!warp_wait(bar_full + 8u * slot_of(fill), parity_of(fill))) return false;
-      if (!warp_wait(bar_p_full + 8u * b, uint32_t(tile >> 1) & 1u)) return false;
-      tc_fence_after();
       const uint32_t v = ((s_ring + slot_of(fill) * kSlotBytes) >> 4) | kLoV;
       const uint32_t w = tmem + kTmemS + b * kKeys;
 #pragma unroll
       for (int i = 0; i < kKeys / 16; ++i) {
+        if (i % 2 == 0) {  // the weights come in halves
+          if (!warp_wait(bar_p_full + 16u * b + 4u * uint32_t(i), uint32_t(tile >> 1) & 1u)) return false;
+          tc_fence_after();
+        }
         umma_bf16_a_tmem_warp(tmem, w + 8u * uint32_t(i), v + uint32_t(i) * (2u * kGroupBytes >> 4),
                               kHiSlot, kIdescPV, accumulate || i > 0, leader);
       }
@@ -648,22 +706,45 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     };
     // Q rows of a segment: this group's half of the dims into tensor memory (and,
     // head_dim 512, its half of the upper dims into shared memory)
-    auto load_q = [&](const Segment &s) {
+    // What is kept of a segment while its tiles go by.
+    struct Rows {
+      int64_t at;    // output row of this thread's query
+      int rows;      // of the tile
+      int t;         // this row's position
+      int tiles;
+      int part;
+      int piece;     // 0, 1: which of the CTA's partial results; -1: the item is whole
+    };
+    auto load_q = [&](Rows &kept) -> bool {
+      Segment s;
+      if (!walk.next(p, s)) return false;
+      {
+        const int token = min(row, s.rows - 1) / p.group;
+        kept.rows = s.rows;
+        kept.t = s.t0 + token;
+        kept.tiles = s.end - s.begin;
+        kept.part = s.hp / heads;
+        kept.piece = s.begin > 0 ? 0 : (s.end < s.total ? 1 : -1);
+        kept.at = (int64_t(s.run.start) + s.token0 + token) * p.q_heads + (s.hp % heads) * p.group +
+                  (row - token * p.group);
+      }
       const bool active = 32 * quarter < s.rows;
       if (active) {
-        const int token = row / p.group;
-        const __nv_bfloat16 *src =
-            p.q + ((int64_t(s.run.start) + s.token0 + token) * p.q_heads + (s.hp % heads) * p.group +
-                   (row - token * p.group)) * T::kHeadDim + 128 * group;
-        uint4 w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          w[i] = row < s.rows ? __ldg(reinterpret_cast<const uint4 *>(src) + i) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
+        const __nv_bfloat16 *src = p.q + kept.at * T::kHeadDim + 128 * group;
+#pragma unroll 1
         for (int h = 0; h < 2; ++h) {
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint4 v = row < kept.rows ? __ldg(reinterpret_cast<const uint4 *>(src) + 8 * h + i)
+                                            : make_uint4(0, 0, 0, 0);
+            w[4 * i] = v.x;
+            w[4 * i + 1] = v.y;
+            w[4 * i + 2] = v.z;
+            w[4 * i + 3] = v.w;
+          }
           tmem_st32(tmem + lanes + kTmemQ + 64u * uint32_t(group) + 32u * uint32_t(h),
-                    reinterpret_cast<const float *>(w + 8 * h));
+                    reinterpret_cast<const float *>(w));
         }
         if constexpr (T::kKSlots == 2) {
 #pragma unroll
@@ -679,15 +760,14 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_q_full);
+      return true;
     };
-    Segment s;
-    bool more = walk.next(p, s);
-    if (more) load_q(s);
+    Rows now_rows, next_rows;
+    bool more = load_q(now_rows);
     while (more && ok) {
-      const bool active = 32 * quarter < s.rows;  // some row of the warp is a query
-      const int token = min(row, s.rows - 1) / p.group;
-      const int t = s.t0 + token;
-      const int n1 = n0 + (s.end - s.begin);
+      const bool active = 32 * quarter < now_rows.rows;  // some row of the warp is a query
+      const int t = now_rows.t;
+      const int n1 = n0 + now_rows.tiles;
       float l_run = 0.0f;
       float ref = -INFINITY;  // what l_run's weights are scaled by
       for (int n = n0 + ((n0 ^ group) & 1); n < n1; n += 2) {
@@ -695,9 +775,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         if (!ok) break;
         tc_fence_after();
         const TileInfo info = small.info[n % kInfos];
+        float sc[64];
+        const uint32_t s_at = tmem + lanes + kTmemS + uint32_t(group) * kKeys;
         if (active) {
-          float sc[64];
-          const uint32_t s_at = tmem + lanes + kTmemS + uint32_t(group) * kKeys;
           tmem_ld64(s_at, sc);
           if (info.edge) {
             unsigned long long sees = info.live & low_bits(t + 1 - info.base);
@@ -735,18 +815,6 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
             if (ref != -INFINITY) l_run *= ex2_approx(ref - now);
             ref = now;
           }
-          const float neg = now == -INFINITY ? 0.0f : -now;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          uint32_t w[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float e0 = ex2_approx(fmaf(sc[2 * i], scale, neg));
-            const float e1 = ex2_approx(fmaf(sc[2 * i + 1], scale, neg));
-            sum[i & 3] += e0 + e1;
-            const __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
-            w[i] = *reinterpret_cast<const uint32_t *>(&h);
-          }
-          l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           // tensor-memory accesses are warp-wide: the warp rescales its rows of O if
           // any of them must, once P V of the tile before no longer adds to them
           const bool raised = last != -INFINITY && now != last;
@@ -765,7 +833,6 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
               tmem_st32(tmem + lanes + uint32_t(c), o);
             }
           }
-          tmem_st32(s_at, reinterpret_cast<const float *>(w));
         } else if (lane == 0) {
           // nobody reads it, but the barrier's phases go by the tile's number
           mbar_arrive(bar_m_full + 32u * uint32_t(group) + 8u * uint32_t(quarter));
@@ -783,9 +850,28 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           }
           fence_proxy_async_shared();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p_full + 8u * uint32_t(group));
+        // the weights in two halves: P V starts on the first under the second
+        const float neg = ref == -INFINITY ? 0.0f : -ref;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (active) {
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float e0 = ex2_approx(fmaf(sc[32 * h + 2 * i], scale, neg));
+              const float e1 = ex2_approx(fmaf(sc[32 * h + 2 * i + 1], scale, neg));
+              sum[i & 3] += e0 + e1;
+              const __nv_bfloat162 b2 = __floats2bfloat162_rn(e0, e1);
+              w[i] = *reinterpret_cast<const uint32_t *>(&b2);
+            }
+            tmem_st16(s_at + 16u * uint32_t(h), w);
+            l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_p_full + 16u * uint32_t(group) + 8u * uint32_t(h));
+        }
       }
       if (!ok) break;
 
@@ -797,9 +883,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         if (!ok) break;
         tc_fence_after();
       }
-      const Segment done = s;
-      more = walk.next(p, s);
-      if (more) load_q(s);
+      more = load_q(next_rows);
       if (active) {
         if (!owner) {
           ok = warp_wait(bar_m_full + 32u * uint32_t(group ^ 1) + 8u * uint32_t(quarter),
@@ -822,14 +906,11 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       ok = warp_wait(bar_l_full + 32u * uint32_t(group ^ 1) + 8u * uint32_t(quarter),
                      uint32_t(segments & 1));
       if (!ok) break;
-      const bool whole = done.begin == 0 && done.end == done.total;
-      const bool writes = active && row < done.rows;
+      const bool whole = now_rows.piece < 0;
+      const bool writes = active && row < now_rows.rows;
       const float l_row = active ? small.row_sum[0][row] + small.row_sum[1][row] : 0.0f;
       const float inv = whole ? (l_row > 0.0f ? 1.0f / l_row : 0.0f) : 1.0f;
-      const int part = done.hp / heads;
-      const int64_t at = (int64_t(done.run.start) + done.token0 + token) * p.q_heads +
-                         (done.hp % heads) * p.group + (row - token * p.group);
-      float *piece = p.partials + (int64_t(blockIdx.x) * 2 + (done.begin == 0 ? 1 : 0)) *
+      float *piece = p.partials + (int64_t(blockIdx.x) * 2 + (whole ? 0 : now_rows.piece)) *
                                       (int64_t(p.rows_cap) * (kPartDims + 2));
       // 64 columns at a time; the second half frees O before its stores
 #pragma unroll 1
@@ -843,7 +924,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           if (lane == 0) mbar_arrive(bar_o_free);
         }
         if (writes && whole) {
-          uint4 *dst = reinterpret_cast<uint4 *>(p.out + at * T::kHeadDim + part * kPartDims + column);
+          uint4 *dst = reinterpret_cast<uint4 *>(p.out + now_rows.at * T::kHeadDim + now_rows.part * kPartDims +
+                                                column);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             uint32_t w[4];
@@ -865,11 +947,12 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         if (!whole) {
           piece[p.rows_cap * kPartDims + row] = ref;
           piece[p.rows_cap * (kPartDims + 1) + row] = l_row;
-        } else if (p.lse != nullptr && part == 0) {
-          p.lse[at] = l_row > 0.0f ? (ref + log2f(l_row)) * 0.6931471805599453f : -INFINITY;
+        } else if (p.lse != nullptr && now_rows.part == 0) {
+          p.lse[now_rows.at] = l_row > 0.0f ? (ref + log2f(l_row)) * 0.6931471805599453f : -INFINITY;
         }
       }
       n0 = n1;
+      now_rows = next_rows;
       ++segments;
     }
   }
@@ -1028,6 +1111,8 @@ cudaError_t launch_chunk(const ChunkAttentionArgs &a, int ctas, cudaStream_t str
   p.window = a.window;
   p.sinks = a.sinks;
   p.box = box_tokens(c.page_size);
+  p.page_div = FastDiv::by(uint32_t(c.page_size));
+  p.slot_div = FastDiv::by(uint32_t(c.max_pages_per_seq));
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   p.rows_cap = partial_rows(p.group, a.runs.max_row_count);
   p.meta = static_cast<int4 *>(a.workspace);
