@@ -19,8 +19,10 @@
 //              takes the key tiles with number n % 2 == g
 //   warps 8, 9 load K and V tiles (TMA boxes that lie inside one page, or 16-byte
 //              copies where pages are no multiple of eight tokens); a box costs its
-//              warp about 130 clocks, a page-table entry a round trip, so the tensors
-//              have a warp each and look a tile ahead
+//              warp about 130 clocks and a page-table entry a round trip, so the
+//              tensors have a warp each, which looks up 32 boxes at a time and those
+//              a batch ahead. The K warp also tells the others what a segment (this
+//              CTA's piece of an item) and a key tile are.
 //   warp 10    issues the MMAs
 // Tensor memory (512 columns): O (128 x 256 fp32), Q (128 x 256 bf16: the A operand
 // of Q K^T), and two score buffers of 64 columns; the weights go back as bf16 over
@@ -71,7 +73,11 @@ constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kTmemQ = 256;
 constexpr uint32_t kTmemS = 384;              // + 64 * buffer
 constexpr float kRescaleSlack = 8.0f;         // log2 units
-constexpr int kInfos = 8;                     // key tiles whose description is kept
+// Key tiles and segments whose description is kept. The K warp describes tile n
+// only when K of tile n - 1 has a slot, which takes P V of tile n - 5 to be complete
+// (with either ring), so what is read for that tile and its segment has been read.
+constexpr int kInfos = 8;
+constexpr int kSegments = 8;
 constexpr long long kTileWaitClocks = 1ll << 26;
 // What starting an item costs next to a key tile (loading Q, reading O back), and
 // the least a CTA is given, both in key tiles: they shape the cut only.
@@ -172,14 +178,23 @@ struct Segment {
   int total;
 };
 
-// Walks the items of a CTA's share. Every role does so by itself.
+// Walks the items of a CTA's share (the two loader warps do, each by itself). The
+// lanes hold 32 runs at a time.
 struct Walk {
   long long left;
   int hp, run, tile, offset;
 
-  __device__ __forceinline__ bool next(const ChunkParams &p, Segment &s) {
+  __device__ __forceinline__ bool next(const ChunkParams &p, Segment &s, ChunkRun &mine, int &first_run) {
     while (left > 0) {
-      s.run = chunk_run(p.runs, run, p.cfg.batch_size);
+      if (run < first_run || run >= first_run + 32) {
+        first_run = run & ~31;
+        mine = chunk_run(p.runs, first_run + (int(threadIdx.x) & 31), p.cfg.batch_size);
+      }
+      const int from = run - first_run;
+      s.run.count = __shfl_sync(0xffffffffu, mine.count, from);
+      s.run.first = __shfl_sync(0xffffffffu, mine.first, from);
+      s.run.start = __shfl_sync(0xffffffffu, mine.start, from);
+      s.run.batch = __shfl_sync(0xffffffffu, mine.batch, from);
       s.token0 = tile * p.tile_tokens;
       if (s.token0 >= s.run.count) {  // the run has no such tile
         tile = 0;
@@ -215,23 +230,22 @@ struct Walk {
   }
 };
 
-// chunk_page without its divisions.
-__device__ __forceinline__ int logical_to_page(const ChunkParams &p, int batch, int logical) {
-  const int slots = p.cfg.max_pages_per_seq;
-  if (p.cfg.window_size == 0) {
-    if (logical >= slots) return -1;
-  } else {
-    logical -= p.slot_div.quotient(logical) * slots;
-  }
-  const int page = __ldg(p.page_table + int64_t(batch) * slots + logical);
-  return page < p.cfg.num_pages ? page : -1;
-}
-
 // What the softmax needs to know about a key tile, left by the loader.
 struct TileInfo {
   unsigned long long live;  // keys that some row of the query tile sees
   int base;                 // position of the tile's first key
   int edge;                 // some row does not see all 64
+};
+
+// What the softmax and the MMA warp need to know about a segment.
+struct SegmentInfo {
+  int tiles;   // key tiles; 0: there is no further segment
+  int rows;    // query rows
+  int t0;      // position of the first
+  int row0;    // its token's row in the packed tensors
+  int hp;      // part * KV heads + KV head
+  int piece;   // 0, 1: which of the CTA's partial results; -1: the item is whole
+  int pad[2];
 };
 
 struct SmallState {
@@ -243,7 +257,9 @@ struct SmallState {
   uint64_t l_full[2][4];      // row_sum of 32 rows written by the group
   uint64_t q_full;            // Q of the segment in tensor memory
   uint64_t o_free;            // O of the segment read back
+  uint64_t seg_full[kSegments];
   TileInfo info[kInfos];
+  SegmentInfo segment[kSegments];
   float row_ref[2][kRows];
   float row_sum[2][kRows];
   long long scan[kThreads / 32];
@@ -338,6 +354,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   const uint32_t bar_l_full = smem_u32(&small.l_full[0][0]);  // + 32 group + 8 warp quarter
   const uint32_t bar_q_full = smem_u32(&small.q_full);
   const uint32_t bar_o_free = smem_u32(&small.o_free);
+  const uint32_t bar_seg_full = smem_u32(&small.seg_full[0]);  // + 8 (segment % kSegments)
   if (tid == 0) {
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(bar_full + 8u * i, 1);
@@ -354,6 +371,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     }
     mbar_init(bar_q_full, kSoftmaxWarps);
     mbar_init(bar_o_free, kSoftmaxWarps);
+    for (int i = 0; i < kSegments; ++i) mbar_init(bar_seg_full + 8u * i, 1);
     small.abort = 0;
     mbar_fence_init();
   }
@@ -455,154 +473,221 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   if (warp == kSoftmaxWarps || warp == kSoftmaxWarps + 1) {
     // ------------------------------------------------------------ loaders of K and V
     const bool is_v = warp == kSoftmaxWarps + 1;
-    // A key tile as the loader sees it: where it lies, which of its keys somebody sees
-    // (pages aside), and this lane's page-table entries, asked for a tile ahead.
-    struct Tile {
-      unsigned long long live;
-      int base, t0, t1;
-      int head, part;
-      int row0;      // of the own rows; -1: in the cache
-      int page[2];   // box > 0: of the lane's box; else of rows lane and lane + 32
-      int offset[2]; // in the page
-    };
-    Segment s;
-    int j = 0;
-    s.end = 0;
+    const __nv_bfloat16 *cache = is_v ? p.cache_v : p.cache_k;
+    const __nv_bfloat16 *rows = is_v ? p.v_rows : p.k_rows;
+    const CUtensorMap *map = is_v ? &map_v : &map_k;
+    const CUtensorMap *map_rows = is_v ? &map_v_rows : &map_k_rows;
+    const int box_shift = p.box > 0 ? 31 - __clz(p.box) : 0;
+    const int tile_boxes = p.box > 0 ? kKeys >> box_shift : 0;  // boxes of a key tile
+    const int batch_tiles = p.box > 0 ? 32 / tile_boxes : 1;    // key tiles of a look-up
+    const int page_groups = p.cfg.page_size / 8;
+    const int layer_group = p.layer * p.cfg.num_pages * page_groups;
+    int slot = is_v ? T::kKSlots : 0;
+    uint32_t phase = 0;  // of the slot's current use
+    int n = 0, segments = 0;
     int4 meta = make_int4(-1, 0, 0, 0);
-    auto look_up = [&](Tile &t) -> bool {
-      if (j >= s.end) {
-        if (!walk.next(p, s)) return false;
-        j = s.begin;
+    ChunkRun mine;
+    int first_run = -32;
+    Segment s;
+    bool ok = true;
+    auto tell_segment = [&](int tiles) {
+      if (is_v) return;
+      if (lane == 0) {
+        SegmentInfo &info = small.segment[segments % kSegments];
+        info.tiles = tiles;
+        info.rows = s.rows;
+        info.t0 = s.t0;
+        info.row0 = s.run.start + s.token0;
+        info.hp = s.hp;
+        info.piece = s.begin > 0 ? 0 : (s.end < s.total ? 1 : -1);
+        mbar_arrive(bar_seg_full + 8u * uint32_t(segments % kSegments));
+      }
+      ++segments;
+    };
+    while (ok && walk.next(p, s, mine, first_run)) {
+      const int head = s.hp % heads;
+      const int part = s.hp / heads;
+      tell_segment(s.end - s.begin);
+      if (!is_v) {
         if (s.begin > 0) meta.w = s.end == s.total ? 1 : 2;
         if (s.begin == 0 && s.end < s.total) {
           meta.x = s.hp;
           meta.y = s.run_index;
           meta.z = s.query_tile;
         }
-      }
-      int k = j++;
-      bool own = false;
-      if (k < s.keys.ca) {
-      } else if ((k -= s.keys.ca) < s.keys.cb1 - s.keys.cb0) {
-        k += s.keys.cb0;
-      } else {
-        k -= s.keys.cb1 - s.keys.cb0;
-        own = true;
-        if (k >= s.keys.oa) k += s.keys.ob0 - s.keys.oa;
-      }
-      t.head = s.hp % heads;
-      t.part = s.hp / heads;
-      t.t0 = s.t0;
-      t.t1 = s.t1;
-      t.base = (own ? s.run.first : 0) + k * kKeys;
-      t.row0 = own ? s.run.start + k * kKeys : -1;
-      t.live = low_bits(s.t1 + 1 - t.base);
-      if (!own && p.k_rows != nullptr) t.live &= low_bits(s.run.first - t.base);
-      if (p.window > 0) {
-        t.live &= ~low_bits(s.t0 - p.window + 1 - t.base) | low_bits(p.sinks - t.base);
-      }
-      t.page[0] = t.page[1] = -1;
-      if (!own) {
-        const int step = p.box > 0 ? p.box : 32;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int at = p.box > 0 ? lane * p.box : lane + 32 * i;
-          if (at >= kKeys || (p.box > 0 && i == 1)) continue;
-          const unsigned long long bits =
-              p.box > 0 ? (step == 64 ? ~0ull : ((1ull << step) - 1ull) << at) : 1ull << at;
-          if ((t.live & bits) == 0) continue;
-          const int logical = p.page_div.quotient(t.base + at);
-          t.offset[i] = t.base + at - logical * p.cfg.page_size;
-          t.page[i] = logical_to_page(p, s.run.batch, logical);
+        // the query rows of the segment, which the softmax warps will ask for
+        const int tokens = s.t1 - s.t0 + 1;
+        for (int i = lane; i < tokens; i += 32) {
+          const __nv_bfloat16 *q = p.q + ((int64_t(s.run.start) + s.token0 + i) * p.q_heads +
+                                          head * p.group) * T::kHeadDim;
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(q),
+                       "r"(p.group * T::kHeadDim * 2)
+                       : "memory");
         }
       }
-      return true;
-    };
-    auto claim = [&](int fill) -> bool {  // the slot's last reader is done
-      const bool free = fill < kSlots || wait(bar_done + 8u * slot_of(fill), parity_of(fill) ^ 1u);
-      return __all_sync(0xffffffffu, free);
-    };
-    Tile t, ahead;
-    bool more = look_up(t);
-    bool ok = true;
-    int n = 0;
-    for (; more && ok; ++n) {
-      const bool more_ahead = look_up(ahead);
-      const bool own = t.row0 >= 0;
-      unsigned long long mapped = ~0ull;  // keys whose page exists
-      if (!own && p.box > 0) {
-        unsigned long long bits = 0;
-        if (t.page[0] >= 0) {
-          bits = p.box == 64 ? ~0ull : ((1ull << p.box) - 1ull) << (lane * p.box);
-        }
-        const uint32_t lo = __reduce_or_sync(0xffffffffu, uint32_t(bits));
-        const uint32_t hi = __reduce_or_sync(0xffffffffu, uint32_t(bits >> 32));
-        mapped = (uint64_t(hi) << 32) | lo;
-      } else if (!own) {
-        const uint32_t lo = __ballot_sync(0xffffffffu, t.page[0] >= 0);
-        const uint32_t hi = __ballot_sync(0xffffffffu, t.page[1] >= 0);
-        mapped = (uint64_t(hi) << 32) | lo;
-      }
-      const unsigned long long live = t.live & mapped;
-#pragma unroll
-      for (int f = 0; f < T::kKSlots; ++f) {
-        if (is_v && f > 0) break;
-        const int fill = n * T::kTileSlots + (is_v ? T::kKSlots : f);
-        const int block0 = is_v ? t.part * 4 : f * 4;
-        ok = claim(fill);
-        if (!ok) break;
-        if (!is_v && f == 0 && lane == 0) {
-          const bool edge = live != ~0ull || t.base + kKeys - 1 > t.t0 ||
-                            (p.window > 0 && t.base <= t.t1 - p.window && t.base + kKeys > p.sinks);
-          small.info[n % kInfos] = {live, t.base, edge ? 1 : 0};
-        }
-        const uint32_t bar = bar_full + 8u * slot_of(fill);
-        const uint32_t dst = s_ring + slot_of(fill) * kSlotBytes;
-        if (p.box == 0) {
-          const __nv_bfloat16 *from = own ? (is_v ? p.v_rows : p.k_rows) : (is_v ? p.cache_v : p.cache_k);
-          int64_t row_at[2];  // element offset of rows lane, lane + 32
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            row_at[i] = -1;
-            if (((live >> (lane + 32 * i)) & 1ull) == 0) continue;
-            row_at[i] = own ? ((int64_t(t.row0) + lane + 32 * i) * heads + t.head) * T::kHeadDim
-                            : cache_offset(p.cfg, p.layer, t.page[i], t.offset[i], t.head, 0);
+      int j = s.begin;
+      while (j < s.end && ok) {
+        // the contiguous key tiles from j on
+        int k = j, stop;
+        bool own = false;
+        if (k < s.keys.ca) {
+          stop = s.keys.ca;
+        } else if ((k -= s.keys.ca) < s.keys.cb1 - s.keys.cb0) {
+          k += s.keys.cb0;
+          stop = s.keys.cb1;
+        } else {
+          k -= s.keys.cb1 - s.keys.cb0;
+          own = true;
+          stop = s.keys.oa;
+          if (k >= s.keys.oa) {
+            k += s.keys.ob0 - s.keys.oa;
+            stop = s.keys.ob1;
           }
-          const uint32_t column = dst + uint32_t(lane >> 3) * kBlockBytes;
-#pragma unroll 8
-          for (int r = 0; r < kKeys; ++r) {
-            const int64_t at = __shfl_sync(0xffffffffu, row_at[r >> 5], r & 31);
-            if (at >= 0) {
-              cp_async16(column + uint32_t(r >> 3) * kGroupBytes + uint32_t(r & 7) * 128u +
-                             ((uint32_t(lane & 7) ^ uint32_t(r & 7)) << 4),
-                         from + at + block0 * 64 + lane * 8);
+        }
+        const int count = min(stop - k, s.end - j);
+        j += count;
+        const int origin = own ? s.run.first : 0;
+        const int limit = !own && p.k_rows != nullptr ? min(s.run.first, s.t1 + 1) : s.t1 + 1;
+        // keys of the tile that some row sees, pages aside
+        auto seen = [&](int base) -> unsigned long long {
+          unsigned long long live = low_bits(limit - base);
+          if (p.window > 0) {
+            live &= ~low_bits(s.t0 - p.window + 1 - base) | low_bits(p.sinks - base);
+          }
+          return live;
+        };
+        // box > 0: token group of box `lane` of the 32 from position `at` on, -1
+        // without a page; asked for raw, checked when it is used
+        int raw = -1, raw_offset = 0;
+        auto ask = [&](int at) {
+          raw = -1;
+          const int position = at + (lane << box_shift);
+          if (position >= limit) return;
+          int logical = p.page_div.quotient(position);
+          raw_offset = (position - logical * p.cfg.page_size) >> 3;
+          const int slots = p.cfg.max_pages_per_seq;
+          if (p.cfg.window_size == 0) {
+            if (logical >= slots) return;
+          } else {
+            logical -= p.slot_div.quotient(logical) * slots;
+          }
+          raw = __ldg(p.page_table + int64_t(s.run.batch) * slots + logical);
+        };
+        int group_of_box = -1;
+        int in_batch = batch_tiles;  // the current batch is used up
+        if (!own && p.box > 0) ask(k * kKeys);
+        for (int i = 0; i < count; ++i, ++n) {
+          const int base = origin + (k + i) * kKeys;
+          unsigned long long live = ~0ull;
+          if (base + kKeys > limit || (p.window > 0 && base <= s.t0 - p.window)) live = seen(base);
+          int group = -1;  // of this lane's box of the tile
+          if (!own && p.box > 0) {
+            if (in_batch == batch_tiles) {
+              group_of_box = raw >= 0 && raw < p.cfg.num_pages
+                                 ? layer_group + raw * page_groups + raw_offset
+                                 : -1;
+              in_batch = 0;
+              ask(base + 32 * p.box);
+            }
+            group = __shfl_sync(0xffffffffu, group_of_box, (in_batch * tile_boxes + lane) & 31);
+            ++in_batch;
+            if (lane >= tile_boxes ||
+                ((live >> (lane << box_shift)) & (p.box == 64 ? ~0ull : (1ull << p.box) - 1ull)) == 0) {
+              group = -1;
+            }
+            const uint32_t boxes = __ballot_sync(0xffffffffu, group >= 0);
+            if (boxes != (tile_boxes == 32 ? ~0u : (1u << tile_boxes) - 1u)) {
+              unsigned long long mapped = 0;
+              for (int b = 0; b < tile_boxes; ++b) {
+                if ((boxes >> b) & 1u) mapped |= low_bits(p.box) << (b << box_shift);
+              }
+              live &= mapped;
             }
           }
-          asm volatile("cp.async.wait_all;" ::: "memory");
-          fence_proxy_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar);
-        } else if (own) {
-          if (lane == 0) mbar_arrive_expect_tx(bar, kSlotBytes);
-          __syncwarp();
-          if (lane < kKeys / 8) {
-            tma_load_rows_box(dst + uint32_t(lane) * kGroupBytes, is_v ? &map_v_rows : &map_k_rows,
-                              block0, t.row0 + lane * 8, t.head, bar);
+          int page[2], offset[2];  // box == 0: of rows lane and lane + 32
+          if (p.box == 0 && !own) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              page[r] = -1;
+              const int at = lane + 32 * r;
+              if (((live >> at) & 1ull) != 0) {
+                const int logical = p.page_div.quotient(base + at);
+                offset[r] = base + at - logical * p.cfg.page_size;
+                page[r] = chunk_page(p.cfg, p.page_table, s.run.batch, logical);
+              }
+            }
+            const uint32_t lo = __ballot_sync(0xffffffffu, page[0] >= 0);
+            const uint32_t hi = __ballot_sync(0xffffffffu, page[1] >= 0);
+            live &= (uint64_t(hi) << 32) | lo;
           }
-        } else {
-          if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(__popcll(mapped)) * (kPartDims * 2));
-          __syncwarp();
-          if (t.page[0] >= 0) {
-            const int token_group = (p.layer * p.cfg.num_pages + t.page[0]) * (p.cfg.page_size / 8) +
-                                    t.offset[0] / 8;
-            tma_load_page_box(dst + uint32_t(lane * p.box / 8) * kGroupBytes, is_v ? &map_v : &map_k,
-                              block0, token_group, t.head, bar);
+#pragma unroll
+          for (int f = 0; f < T::kKSlots; ++f) {
+            if (is_v && f > 0) break;
+            const int block0 = is_v ? part * 4 : f * 4;
+            // the slot's last reader is done (a slot's first use waits for nothing)
+            ok = __all_sync(0xffffffffu, wait(bar_done + 8u * uint32_t(slot), phase ^ 1u));
+            if (!ok) break;
+            if (!is_v && f == 0 && lane == 0) {
+              const bool edge = live != ~0ull || base + kKeys - 1 > s.t0 ||
+                                (p.window > 0 && base <= s.t1 - p.window && base + kKeys > p.sinks);
+              small.info[n % kInfos] = {live, base, edge ? 1 : 0};
+            }
+            const uint32_t bar = bar_full + 8u * uint32_t(slot);
+            const uint32_t dst = s_ring + uint32_t(slot) * kSlotBytes;
+            if (p.box == 0) {
+              int64_t row_at[2];  // element offset of rows lane, lane + 32
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                row_at[r] = -1;
+                const int at = lane + 32 * r;
+                if (((live >> at) & 1ull) == 0) continue;
+                row_at[r] = own ? ((int64_t(s.run.start) + (k + i) * kKeys + at) * heads + head) * T::kHeadDim
+                                : cache_offset(p.cfg, p.layer, page[r], offset[r], head, 0);
+              }
+              const __nv_bfloat16 *from = own ? rows : cache;
+              const uint32_t column = dst + uint32_t(lane >> 3) * kBlockBytes;
+#pragma unroll 8
+              for (int r = 0; r < kKeys; ++r) {
+                const int64_t at = __shfl_sync(0xffffffffu, row_at[r >> 5], r & 31);
+                if (at >= 0) {
+                  cp_async16(column + uint32_t(r >> 3) * kGroupBytes + uint32_t(r & 7) * 128u +
+                                 ((uint32_t(lane & 7) ^ uint32_t(r & 7)) << 4),
+                             from + at + block0 * 64 + lane * 8);
+                }
+              }
+              asm volatile("cp.async.wait_all;" ::: "memory");
+              fence_proxy_async_shared();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar);
+            } else if (own) {
+              if (lane == 0) mbar_arrive_expect_tx(bar, kSlotBytes);
+              __syncwarp();
+              if (lane < kKeys / 8) {
+                tma_load_rows_box(dst + uint32_t(lane) * kGroupBytes, map_rows, block0,
+                                  s.run.start + (k + i) * kKeys + lane * 8, head, bar);
+              }
+            } else {
+              const uint32_t boxes = __ballot_sync(0xffffffffu, group >= 0);
+              if (lane == 0) {
+                mbar_arrive_expect_tx(bar, uint32_t(__popc(boxes) << box_shift) * (kPartDims * 2));
+              }
+              __syncwarp();
+              if (group >= 0) {
+                tma_load_page_box(dst + (uint32_t(lane << box_shift) >> 3) * kGroupBytes, map, block0, group,
+                                  head, bar);
+              }
+            }
+            slot += is_v ? T::kTileSlots : (f + 1 < T::kKSlots ? 1 : T::kTileSlots - T::kKSlots + 1);
+            if (slot >= kSlots) {
+              slot -= kSlots;
+              phase ^= 1u;
+            }
           }
+          if (!ok) break;
         }
       }
-      t = ahead;
-      more = more_ahead;
     }
+    if (ok) tell_segment(0);
     if (!is_v && lane == 0) p.meta[blockIdx.x] = meta;
     if (!ok || *abort_flag != 0) {
       // nobody may be waiting for the last loads any more: see them land before the
@@ -624,49 +709,66 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     constexpr uint32_t kHiSlot = uint32_t(kGroupBytes >> 4) | (1u << 14) | (2u << 29);
     constexpr uint32_t kHiQ = 64u | (1u << 14) | (2u << 29);
     const bool leader = elect_one();
-    int n = 0;  // key tiles so far
-    int segments = 0;
-    Segment s;
-    bool ok = true;
     auto warp_wait = [&](uint32_t bar, uint32_t parity) -> bool {
       return __all_sync(0xffffffffu, wait(bar, parity));
     };
-    // O (+)= P V: four steps of 16 keys
-    auto issue_pv = [&](int tile, bool accumulate) -> bool {
-      const int fill = tile * T::kTileSlots + T::kKSlots;
-      const uint32_t b = uint32_t(tile & 1);
-      if (!warp_wait(bar_full + 8u * slot_of(fill), parity_of(fill))) return false;
-      const uint32_t v = ((s_ring + slot_of(fill) * kSlotBytes) >> 4) | kLoV;
+    // position in the ring of K of the next tile to score and of V of the next to add
+    struct Cursor {
+      uint32_t slot, phase;
+      __device__ __forceinline__ void advance(uint32_t by) {
+        slot += by;
+        if (slot >= kSlots) {
+          slot -= kSlots;
+          phase ^= 1u;
+        }
+      }
+    };
+    Cursor k_at = {0, 0}, v_at = {uint32_t(T::kKSlots), 0};
+    Cursor v_last = v_at;  // of the tile before v_at's
+    int n = 0;             // key tiles so far
+    int segments = 0;
+    bool ok = true;
+    // O (+)= P V of tile n - 1: four steps of 16 keys
+    auto issue_pv = [&](bool accumulate) -> bool {
+      const uint32_t b = uint32_t(n - 1) & 1u;
+      const uint32_t parity = uint32_t((n - 1) >> 1) & 1u;
+      if (!warp_wait(bar_full + 8u * v_at.slot, v_at.phase)) return false;
+      const uint32_t v = ((s_ring + v_at.slot * kSlotBytes) >> 4) | kLoV;
       const uint32_t w = tmem + kTmemS + b * kKeys;
 #pragma unroll
       for (int i = 0; i < kKeys / 16; ++i) {
         if (i % 2 == 0) {  // the weights come in halves
-          if (!warp_wait(bar_p_full + 16u * b + 4u * uint32_t(i), uint32_t(tile >> 1) & 1u)) return false;
+          if (!warp_wait(bar_p_full + 16u * b + 4u * uint32_t(i), parity)) return false;
           tc_fence_after();
         }
         umma_bf16_a_tmem_warp(tmem, w + 8u * uint32_t(i), v + uint32_t(i) * (2u * kGroupBytes >> 4),
                               kHiSlot, kIdescPV, accumulate || i > 0, leader);
       }
-      umma_commit_warp(bar_done + 8u * slot_of(fill), leader);
+      umma_commit_warp(bar_done + 8u * v_at.slot, leader);
+      v_last = v_at;
+      v_at.advance(T::kTileSlots);
       return true;
     };
-    while (ok && walk.next(p, s)) {
+    for (; ok; ++segments) {
+      ok = warp_wait(bar_seg_full + 8u * uint32_t(segments % kSegments),
+                     uint32_t(segments / kSegments) & 1u);
+      if (!ok) break;
+      const int tiles = small.segment[segments % kSegments].tiles;
+      if (tiles == 0) break;
       ok = warp_wait(bar_q_full, uint32_t(segments & 1));
-      for (int j = s.begin; j < s.end && ok; ++j, ++n) {
-        // S[n & 1] held the weights of tile n - 2
+      for (int j = 0; j < tiles && ok; ++j) {
+        // S[n & 1] held the weights of tile n - 2, the last whose P V was issued
         if (n >= 2) {
-          const int fill = (n - 2) * T::kTileSlots + T::kKSlots;
-          ok = warp_wait(bar_done + 8u * slot_of(fill), parity_of(fill));
+          ok = warp_wait(bar_done + 8u * v_last.slot, v_last.phase);
           if (!ok) break;
         }
         const uint32_t d = tmem + kTmemS + uint32_t(n & 1) * kKeys;
 #pragma unroll
         for (int f = 0; f < T::kKSlots; ++f) {
-          const int fill = n * T::kTileSlots + f;
-          ok = ok && warp_wait(bar_full + 8u * slot_of(fill), parity_of(fill));
+          ok = ok && warp_wait(bar_full + 8u * k_at.slot, k_at.phase);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t k = ((s_ring + slot_of(fill) * kSlotBytes) >> 4) | kLoK;
+          const uint32_t k = ((s_ring + k_at.slot * kSlotBytes) >> 4) | kLoK;
           const uint32_t q_hi = (s_q_hi >> 4) | kLoK;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {  // steps of 16 dims, four to a block
@@ -679,16 +781,20 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
                              kHiQ, k + at, kHiSlot, kIdescQK, true, leader);
             }
           }
-          umma_commit_warp(bar_done + 8u * slot_of(fill), leader);
+          umma_commit_warp(bar_done + 8u * k_at.slot, leader);
+          k_at.advance(f + 1 < T::kKSlots ? 1 : T::kTileSlots - T::kKSlots + 1);
         }
         if (!ok) break;
         umma_commit_warp(bar_s_full + 8u * uint32_t(n & 1), leader);
-        if (j > s.begin) ok = issue_pv(n - 1, j - 1 > s.begin);
-        // the segment's first P V writes O anew: the last segment's rows must be out
-        if (j == s.begin && segments > 0) ok = warp_wait(bar_o_free, uint32_t(segments - 1) & 1u);
+        if (j > 0) {
+          ok = issue_pv(j > 1);
+        } else if (segments > 0) {
+          // the segment's first P V writes O anew: the last segment's rows must be out
+          ok = warp_wait(bar_o_free, uint32_t(segments - 1) & 1u);
+        }
+        ++n;
       }
-      if (ok) ok = issue_pv(n - 1, s.end - s.begin > 1);
-      ++segments;
+      if (ok) ok = issue_pv(tiles > 1);
     }
   } else {
     // ------------------------------------------------------------ softmax
@@ -704,30 +810,35 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     auto warp_wait = [&](uint32_t bar, uint32_t parity) -> bool {
       return __all_sync(0xffffffffu, wait(bar, parity));
     };
-    // Q rows of a segment: this group's half of the dims into tensor memory (and,
-    // head_dim 512, its half of the upper dims into shared memory)
+    const int token = row / p.group;           // of the query tile
+    const int head_of_group = row - token * p.group;
     // What is kept of a segment while its tiles go by.
     struct Rows {
       int64_t at;    // output row of this thread's query
       int rows;      // of the tile
-      int t;         // this row's position
+      int t;         // this row's position (rows behind the last: not used)
       int tiles;
       int part;
       int piece;     // 0, 1: which of the CTA's partial results; -1: the item is whole
     };
+    // Q rows of the next segment: this group's half of the dims into tensor memory
+    // (and, head_dim 512, its half of the upper dims into shared memory)
+    int asked = 0;  // segments so far
     auto load_q = [&](Rows &kept) -> bool {
-      Segment s;
-      if (!walk.next(p, s)) return false;
-      {
-        const int token = min(row, s.rows - 1) / p.group;
-        kept.rows = s.rows;
-        kept.t = s.t0 + token;
-        kept.tiles = s.end - s.begin;
-        kept.part = s.hp / heads;
-        kept.piece = s.begin > 0 ? 0 : (s.end < s.total ? 1 : -1);
-        kept.at = (int64_t(s.run.start) + s.token0 + token) * p.q_heads + (s.hp % heads) * p.group +
-                  (row - token * p.group);
+      if (!warp_wait(bar_seg_full + 8u * uint32_t(asked % kSegments),
+                     uint32_t(asked / kSegments) & 1u)) {
+        ok = false;
+        return false;
       }
+      const SegmentInfo s = small.segment[asked % kSegments];
+      ++asked;
+      if (s.tiles == 0) return false;
+      kept.rows = s.rows;
+      kept.t = s.t0 + token;
+      kept.tiles = s.tiles;
+      kept.part = s.hp / heads;
+      kept.piece = s.piece;
+      kept.at = (int64_t(s.row0) + token) * p.q_heads + (s.hp - kept.part * heads) * p.group + head_of_group;
       const bool active = 32 * quarter < s.rows;
       if (active) {
         const __nv_bfloat16 *src = p.q + kept.at * T::kHeadDim + 128 * group;
@@ -884,6 +995,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         tc_fence_after();
       }
       more = load_q(next_rows);
+      if (!ok) break;
       if (active) {
         if (!owner) {
           ok = warp_wait(bar_m_full + 32u * uint32_t(group ^ 1) + 8u * uint32_t(quarter),
