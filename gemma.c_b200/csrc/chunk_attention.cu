@@ -25,13 +25,17 @@
 //              CTA's piece of an item) and a key tile are.
 //   warp 10    issues the MMAs
 // Tensor memory (512 columns): O (128 x 256 fp32), Q (128 x 256 bf16: the A operand
-// of Q K^T), and two score buffers of 64 columns; the weights go back as bf16 over
-// the scores they come from and are the A operand of P V. Shared memory holds
-// nothing but a ring of 32 KB slots (64 keys x 256 dims of K or V in 128-byte
-// swizzle): 7 slots for head_dim 256. For head_dim 512 a tile takes two K slots and
-// one V slot, the upper half of Q lies in shared memory (5 slots remain), and the
-// output dims are two parts computed by different items, each with all of Q K^T.
-// Q K^T of tile n + 1 runs under the softmax of tile n.
+// of Q K^T), and two score buffers of 64 columns. K and V tiles go through a ring of
+// 32 KB shared-memory slots (64 keys x 256 dims, 128-byte swizzle).
+// head_dim 256: 6 slots, and two buffers (16 KB) for the bf16 weights, the A operand
+// of P V. A score buffer is free as soon as it has been read, so Q K^T runs two tiles
+// ahead of P V: the tensor pipe always has work queued, and a group of softmax warps
+// has two tiles' time for one.
+// head_dim 512: a tile takes two K slots and one V slot, the upper half of Q lies in
+// shared memory, 5 slots remain; the weights go back into tensor memory over the
+// scores they come from (in two halves: P V starts on the first under the second), so
+// Q K^T runs one tile ahead. The output dims are two parts computed by different
+// items, each with all of Q K^T.
 //
 // Softmax: the maximum that a row's weights are scaled by is passed from tile to
 // tile (through shared memory, from one group to the other) and raised only when a
@@ -66,16 +70,17 @@ constexpr int kSlotBytes = kKeys * kPartDims * 2;
 constexpr int kGroupBytes = 8 * kPartDims * 2;
 constexpr int kBlockBytes = 8 * 128;
 constexpr int kQBlockBytes = kRows * 128;     // 128 rows x 64 dims
-constexpr int kMaxSlots = 7;
+constexpr int kPTileBytes = kRows * kKeys * 2;  // weights of a tile
+constexpr int kMaxSlots = 6;
 constexpr int kSoftmaxWarps = 8;
 constexpr int kThreads = (kSoftmaxWarps + 3) * 32;
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kTmemQ = 256;
 constexpr uint32_t kTmemS = 384;              // + 64 * buffer
 constexpr float kRescaleSlack = 8.0f;         // log2 units
-// Key tiles and segments whose description is kept. The K warp describes tile n
-// only when K of tile n - 1 has a slot, which takes P V of tile n - 5 to be complete
-// (with either ring), so what is read for that tile and its segment has been read.
+// Key tiles and segments whose description is kept. The K warp describes tile n when K
+// of tile n - 1 has a slot, which takes Q K^T of tile n - 4 (n - 3 for head_dim 512) to
+// be complete and so the softmax of tile n - 6 (n - 5) to have begun.
 constexpr int kInfos = 8;
 constexpr int kSegments = 8;
 constexpr long long kTileWaitClocks = 1ll << 26;
@@ -91,8 +96,12 @@ struct ChunkTraits {
   static constexpr int kParts = kHeadDim / kPartDims;
   static constexpr int kTileSlots = kKSlots + 1;
   static constexpr int kQHiBytes = (kHeadDim - 256) * kRows * 2;
-  static constexpr int kSlots = kHeadDim == 256 ? 7 : 5;
-  static constexpr int kTileBytes = kQHiBytes + kSlots * kSlotBytes;
+  static constexpr bool kPShared = kHeadDim == 256;   // the weights in shared memory
+  static constexpr int kPBytes = kPShared ? 2 * kPTileBytes : 0;
+  static constexpr int kSlots = kHeadDim == 256 ? 6 : 5;
+  static constexpr int kLag = kPShared ? 2 : 1;       // tiles that Q K^T is ahead of P V
+  static constexpr int kRingAt = kQHiBytes + kPBytes; // shared memory: upper Q, weights, ring
+  static constexpr int kTileBytes = kRingAt + kSlots * kSlotBytes;
 };
 
 // Division of 0 .. 2^31 - 1 by a fixed number: the quotient's high part by a 32-bit
@@ -255,8 +264,11 @@ struct SmallState {
   uint64_t p_full[2][2];      // half of its weights written (and O rescaled where needed)
   uint64_t m_full[2][4];      // row_ref[b] of 32 rows written
   uint64_t l_full[2][4];      // row_sum of 32 rows written by the group
+  uint64_t s_free[2];         // kPShared: the scores in S[b] have been read
   uint64_t q_full;            // Q of the segment in tensor memory
-  uint64_t o_free;            // O of the segment read back
+  uint64_t q_free;            // its last Q K^T is complete
+  uint64_t o_full;            // its last P V is complete
+  uint64_t o_free;            // its O has been read back
   uint64_t seg_full[kSegments];
   TileInfo info[kInfos];
   SegmentInfo segment[kSegments];
@@ -322,6 +334,29 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  return fmaxf(a, fmaxf(b, c));
+}
+using f32x2 = unsigned long long;  // two fp32, each operation with the scalar one's rounding
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2_rn(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2_rn(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // bits [0, n) of a 64-bit word, n clamped to 0 .. 64
 __device__ __forceinline__ unsigned long long low_bits(int n) {
   return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1ull);
@@ -336,7 +371,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   SmallState &small = *reinterpret_cast<SmallState *>(smem_raw + T::kTileBytes);
   const uint32_t s_q_hi = smem_u32(smem_raw);
-  const uint32_t s_ring = s_q_hi + T::kQHiBytes;
+  const uint32_t s_p = s_q_hi + T::kQHiBytes;
+  const uint32_t s_ring = s_q_hi + T::kRingAt;
   const int tid = int(threadIdx.x);
   const int warp = tid >> 5;
   const int lane = tid & 31;
@@ -352,7 +388,10 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   const uint32_t bar_p_full = smem_u32(&small.p_full[0][0]);  // + 16 b + 8 half
   const uint32_t bar_m_full = smem_u32(&small.m_full[0][0]);  // + 32 b + 8 warp quarter
   const uint32_t bar_l_full = smem_u32(&small.l_full[0][0]);  // + 32 group + 8 warp quarter
+  const uint32_t bar_s_free = smem_u32(&small.s_free[0]);  // + 8 b
   const uint32_t bar_q_full = smem_u32(&small.q_full);
+  const uint32_t bar_q_free = smem_u32(&small.q_free);
+  const uint32_t bar_o_full = smem_u32(&small.o_full);
   const uint32_t bar_o_free = smem_u32(&small.o_free);
   const uint32_t bar_seg_full = smem_u32(&small.seg_full[0]);  // + 8 (segment % kSegments)
   if (tid == 0) {
@@ -369,7 +408,11 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         mbar_init(bar_l_full + 32u * b + 8u * w, 1);
       }
     }
+    mbar_init(bar_s_free, 4);
+    mbar_init(bar_s_free + 8u, 4);
     mbar_init(bar_q_full, kSoftmaxWarps);
+    mbar_init(bar_q_free, 1);
+    mbar_init(bar_o_full, 1);
     mbar_init(bar_o_free, kSoftmaxWarps);
     for (int i = 0; i < kSegments; ++i) mbar_init(bar_seg_full + 8u * i, 1);
     small.abort = 0;
@@ -725,28 +768,35 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     };
     Cursor k_at = {0, 0}, v_at = {uint32_t(T::kKSlots), 0};
     Cursor v_last = v_at;  // of the tile before v_at's
-    int n = 0;             // key tiles so far
+    int n = 0;             // tiles whose Q K^T has been issued
+    int added = 0;         // tiles whose P V has been issued
     int segments = 0;
     bool ok = true;
-    // O (+)= P V of tile n - 1: four steps of 16 keys
+    // O (+)= P V of tile `added`: four steps of 16 keys
     auto issue_pv = [&](bool accumulate) -> bool {
-      const uint32_t b = uint32_t(n - 1) & 1u;
-      const uint32_t parity = uint32_t((n - 1) >> 1) & 1u;
+      const uint32_t b = uint32_t(added) & 1u;
+      const uint32_t parity = uint32_t(added >> 1) & 1u;
       if (!warp_wait(bar_full + 8u * v_at.slot, v_at.phase)) return false;
       const uint32_t v = ((s_ring + v_at.slot * kSlotBytes) >> 4) | kLoV;
-      const uint32_t w = tmem + kTmemS + b * kKeys;
 #pragma unroll
       for (int i = 0; i < kKeys / 16; ++i) {
-        if (i % 2 == 0) {  // the weights come in halves
+        if (i == 0 || (i == 2 && !T::kPShared)) {
           if (!warp_wait(bar_p_full + 16u * b + 4u * uint32_t(i), parity)) return false;
           tc_fence_after();
         }
-        umma_bf16_a_tmem_warp(tmem, w + 8u * uint32_t(i), v + uint32_t(i) * (2u * kGroupBytes >> 4),
-                              kHiSlot, kIdescPV, accumulate || i > 0, leader);
+        const uint32_t vi = v + uint32_t(i) * (2u * kGroupBytes >> 4);
+        if constexpr (T::kPShared) {
+          umma_bf16_warp(tmem, ((s_p + b * kPTileBytes) >> 4 | kLoK) + uint32_t(i) * 2u, kHiQ, vi,
+                         kHiSlot, kIdescPV, accumulate || i > 0, leader);
+        } else {
+          umma_bf16_a_tmem_warp(tmem, tmem + kTmemS + b * kKeys + 8u * uint32_t(i), vi, kHiSlot,
+                                kIdescPV, accumulate || i > 0, leader);
+        }
       }
       umma_commit_warp(bar_done + 8u * v_at.slot, leader);
       v_last = v_at;
       v_at.advance(T::kTileSlots);
+      ++added;
       return true;
     };
     for (; ok; ++segments) {
@@ -755,46 +805,54 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       if (!ok) break;
       const int tiles = small.segment[segments % kSegments].tiles;
       if (tiles == 0) break;
+      const int first = n;
       ok = warp_wait(bar_q_full, uint32_t(segments & 1));
-      for (int j = 0; j < tiles && ok; ++j) {
-        // S[n & 1] held the weights of tile n - 2, the last whose P V was issued
-        if (n >= 2) {
-          ok = warp_wait(bar_done + 8u * v_last.slot, v_last.phase);
-          if (!ok) break;
-        }
-        const uint32_t d = tmem + kTmemS + uint32_t(n & 1) * kKeys;
-#pragma unroll
-        for (int f = 0; f < T::kKSlots; ++f) {
-          ok = ok && warp_wait(bar_full + 8u * k_at.slot, k_at.phase);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t k = ((s_ring + k_at.slot * kSlotBytes) >> 4) | kLoK;
-          const uint32_t q_hi = (s_q_hi >> 4) | kLoK;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {  // steps of 16 dims, four to a block
-            const uint32_t at = uint32_t(i >> 2) * (kBlockBytes >> 4) + uint32_t(i & 3) * 2u;
-            if (f == 0) {
-              umma_bf16_a_tmem_warp(d, tmem + kTmemQ + 8u * uint32_t(i), k + at, kHiSlot, kIdescQK,
-                                    i > 0, leader);
-            } else {
-              umma_bf16_warp(d, q_hi + uint32_t(i >> 2) * (kQBlockBytes >> 4) + uint32_t(i & 3) * 2u,
-                             kHiQ, k + at, kHiSlot, kIdescQK, true, leader);
-            }
+      // one step beyond the segment's tiles per tile that P V lags behind
+      for (int j = 0; j < tiles + T::kLag && ok; ++j) {
+        if (j < tiles) {
+          // S[n & 1] held the scores (kPShared) or the weights of tile n - 2
+          if (n >= 2) {
+            ok = T::kPShared ? warp_wait(bar_s_free + 8u * uint32_t(n & 1), uint32_t((n - 2) >> 1) & 1u)
+                             : warp_wait(bar_done + 8u * v_last.slot, v_last.phase);
+            if (!ok) break;
           }
-          umma_commit_warp(bar_done + 8u * k_at.slot, leader);
-          k_at.advance(f + 1 < T::kKSlots ? 1 : T::kTileSlots - T::kKSlots + 1);
+          const uint32_t d = tmem + kTmemS + uint32_t(n & 1) * kKeys;
+#pragma unroll
+          for (int f = 0; f < T::kKSlots; ++f) {
+            ok = ok && warp_wait(bar_full + 8u * k_at.slot, k_at.phase);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t k = ((s_ring + k_at.slot * kSlotBytes) >> 4) | kLoK;
+            const uint32_t q_hi = (s_q_hi >> 4) | kLoK;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {  // steps of 16 dims, four to a block
+              const uint32_t at = uint32_t(i >> 2) * (kBlockBytes >> 4) + uint32_t(i & 3) * 2u;
+              if (f == 0) {
+                umma_bf16_a_tmem_warp(d, tmem + kTmemQ + 8u * uint32_t(i), k + at, kHiSlot, kIdescQK,
+                                      i > 0, leader);
+              } else {
+                umma_bf16_warp(d, q_hi + uint32_t(i >> 2) * (kQBlockBytes >> 4) + uint32_t(i & 3) * 2u,
+                               kHiQ, k + at, kHiSlot, kIdescQK, true, leader);
+              }
+            }
+            umma_commit_warp(bar_done + 8u * k_at.slot, leader);
+            k_at.advance(f + 1 < T::kKSlots ? 1 : T::kTileSlots - T::kKSlots + 1);
+          }
+          if (!ok) break;
+          umma_commit_warp(bar_s_full + 8u * uint32_t(n & 1), leader);
+          if (j + 1 == tiles) umma_commit_warp(bar_q_free, leader);
+          ++n;
         }
-        if (!ok) break;
-        umma_commit_warp(bar_s_full + 8u * uint32_t(n & 1), leader);
-        if (j > 0) {
-          ok = issue_pv(j > 1);
-        } else if (segments > 0) {
+        if (j >= T::kLag) {
           // the segment's first P V writes O anew: the last segment's rows must be out
-          ok = warp_wait(bar_o_free, uint32_t(segments - 1) & 1u);
+          if (added == first && segments > 0) {
+            ok = warp_wait(bar_o_free, uint32_t(segments - 1) & 1u);
+            if (!ok) break;
+          }
+          ok = issue_pv(added > first);
         }
-        ++n;
       }
-      if (ok) ok = issue_pv(tiles > 1);
+      if (ok) umma_commit_warp(bar_o_full, leader);
     }
   } else {
     // ------------------------------------------------------------ softmax
@@ -881,16 +939,60 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       const int n1 = n0 + now_rows.tiles;
       float l_run = 0.0f;
       float ref = -INFINITY;  // what l_run's weights are scaled by
-      for (int n = n0 + ((n0 ^ group) & 1); n < n1; n += 2) {
-        ok = warp_wait(bar_s_full + 8u * uint32_t(group), uint32_t(n >> 1) & 1u);
-        if (!ok) break;
-        tc_fence_after();
-        const TileInfo info = small.info[n % kInfos];
-        float sc[64];
-        const uint32_t s_at = tmem + lanes + kTmemS + uint32_t(group) * kKeys;
-        if (active) {
+      // V rows that no row of the tile sees become zeros
+      auto clear_v = [&](int n, unsigned long long live) -> bool {
+        const int fill = n * T::kTileSlots + T::kKSlots;
+        if (!warp_wait(bar_full + 8u * slot_of(fill), parity_of(fill))) return false;
+        uint8_t *v = smem_raw + T::kRingAt + slot_of(fill) * kSlotBytes + (lane >> 3) * kBlockBytes +
+                     (lane & 7) * 16;
+        // the rows quarter, quarter + 4, ...: bits 0, 4, 8, ... of
+        unsigned long long dead = (~live >> quarter) & 0x1111111111111111ull;
+        while (dead != 0) {
+          const int r = __ffsll((long long)dead) - 1 + quarter;
+          dead &= dead - 1;
+          *reinterpret_cast<uint4 *>(v + (r >> 3) * kGroupBytes + (r & 7) * 128) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_shared();
+        return true;
+      };
+      if (!active) {
+        // no row of this warp is a query: it keeps the barriers' phases, which go by the
+        // tile's number, and clears its share of V
+        for (int n = n0 + ((n0 ^ group) & 1); n < n1; n += 2) {
+          ok = warp_wait(bar_s_full + 8u * uint32_t(group), uint32_t(n >> 1) & 1u);
+          if (!ok) break;
+          const unsigned long long live = small.info[n % kInfos].live;
+          if (live != ~0ull) ok = clear_v(n, live);
+          if (!ok) break;
+          if (T::kPShared && n >= 2) {  // not a phase ahead of the other warps' weights
+            const int fill = (n - 2) * T::kTileSlots + T::kKSlots;
+            ok = warp_wait(bar_done + 8u * slot_of(fill), parity_of(fill));
+            if (!ok) break;
+          }
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (T::kPShared) mbar_arrive(bar_s_free + 8u * uint32_t(group));
+            mbar_arrive(bar_m_full + 32u * uint32_t(group) + 8u * uint32_t(quarter));
+            mbar_arrive(bar_p_full + 16u * uint32_t(group));
+            if constexpr (!T::kPShared) mbar_arrive(bar_p_full + 16u * uint32_t(group) + 8u);
+          }
+        }
+      } else {
+        for (int n = n0 + ((n0 ^ group) & 1); n < n1; n += 2) {
+          ok = warp_wait(bar_s_full + 8u * uint32_t(group), uint32_t(n >> 1) & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          const TileInfo info = small.info[n % kInfos];
+          float sc[64];
+          const uint32_t s_at = tmem + lanes + kTmemS + uint32_t(group) * kKeys;
           tmem_ld64(s_at, sc);
+          if constexpr (T::kPShared) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_s_free + 8u * uint32_t(group));
+          }
           if (info.edge) {
+            asm volatile("" ::: "memory");  // a branch, not 64 selects on every tile
             unsigned long long sees = info.live & low_bits(t + 1 - info.base);
             if (p.window > 0) {
               sees &= ~low_bits(t - p.window + 1 - info.base) | low_bits(p.sinks - info.base);
@@ -901,14 +1003,17 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
               if (((lo >> c) & 1u) == 0) sc[c] = -INFINITY;
               if (((hi >> c) & 1u) == 0) sc[c + 32] = -INFINITY;
             }
+            if (info.live != ~0ull) ok = clear_v(n, info.live);
+            if (!ok) break;
           }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
 #pragma unroll
-          for (int c = 0; c < 64; c += 8) {
+          for (int c = 4; c < 60; c += 8) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], fmaxf(sc[c + u], sc[c + 4 + u]));
+            for (int u = 0; u < 4; ++u) mx[u] = max3(mx[u], sc[c + u], sc[c + 4 + u]);
           }
-          const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+          const float m_tile = fmaxf(max3(mx[0], mx[1], max3(mx[2], mx[3], sc[60])),
+                                     max3(sc[61], sc[62], sc[63])) * scale;
           // the reference so far: the other group's tile before this one
           float last = -INFINITY;
           if (n > n0) {
@@ -917,71 +1022,77 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
             if (!ok) break;
             last = small.row_ref[group ^ 1][row];
           }
-          float now = last;
-          if (m_tile > last + kRescaleSlack || last == -INFINITY) now = m_tile;
+          const float now = m_tile > last + kRescaleSlack || last == -INFINITY ? m_tile : last;
           small.row_ref[group][row] = now;
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_m_full + 32u * uint32_t(group) + 8u * uint32_t(quarter));
-          if (ref != now) {
-            if (ref != -INFINITY) l_run *= ex2_approx(ref - now);
+          // Raising is rare. Tensor-memory accesses are warp-wide: the warp rescales its
+          // rows of O if any of them must, once P V of the tile before no longer adds to
+          // them.
+          if (__any_sync(0xffffffffu, ref != now)) {
+            l_run = ref == -INFINITY ? 0.0f : l_run * ex2_approx(ref - now);
             ref = now;
+            const bool raised = last != -INFINITY && now != last;
+            if (__any_sync(0xffffffffu, raised)) {
+              const int fill = (n - 1) * T::kTileSlots + T::kKSlots;
+              ok = warp_wait(bar_done + 8u * slot_of(fill), parity_of(fill));
+              if (!ok) break;
+              tc_fence_after();
+              const float factor = raised ? ex2_approx(last - now) : 1.0f;
+#pragma unroll 1
+              for (int c = 0; c < kPartDims; c += 32) {
+                float o[32];
+                tmem_ld32(tmem + lanes + uint32_t(c), o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] *= factor;
+                tmem_st32(tmem + lanes + uint32_t(c), o);
+              }
+            }
           }
-          // tensor-memory accesses are warp-wide: the warp rescales its rows of O if
-          // any of them must, once P V of the tile before no longer adds to them
-          const bool raised = last != -INFINITY && now != last;
-          if (__any_sync(0xffffffffu, raised)) {
-            const int fill = (n - 1) * T::kTileSlots + T::kKSlots;
+          if (T::kPShared && n >= 2) {  // the buffer's last weights have been used
+            const int fill = (n - 2) * T::kTileSlots + T::kKSlots;
             ok = warp_wait(bar_done + 8u * slot_of(fill), parity_of(fill));
             if (!ok) break;
-            tc_fence_after();
-            const float factor = raised ? ex2_approx(last - now) : 1.0f;
-#pragma unroll 1
-            for (int c = 0; c < kPartDims; c += 32) {
-              float o[32];
-              tmem_ld32(tmem + lanes + uint32_t(c), o);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] *= factor;
-              tmem_st32(tmem + lanes + uint32_t(c), o);
-            }
           }
-        } else if (lane == 0) {
-          // nobody reads it, but the barrier's phases go by the tile's number
-          mbar_arrive(bar_m_full + 32u * uint32_t(group) + 8u * uint32_t(quarter));
-        }
-        if (info.live != ~0ull) {
-          const int fill = n * T::kTileSlots + T::kKSlots;
-          ok = warp_wait(bar_full + 8u * slot_of(fill), parity_of(fill));
-          if (!ok) break;
-          uint8_t *v = smem_raw + T::kQHiBytes + slot_of(fill) * kSlotBytes + (lane >> 3) * kBlockBytes +
-                       (lane & 7) * 16;
-          for (int r = quarter; r < kKeys; r += 4) {
-            if (((info.live >> r) & 1ull) == 0) {
-              *reinterpret_cast<uint4 *>(v + (r >> 3) * kGroupBytes + (r & 7) * 128) = make_uint4(0, 0, 0, 0);
-            }
-          }
-          fence_proxy_async_shared();
-        }
-        // the weights in two halves: P V starts on the first under the second
-        const float neg = ref == -INFINITY ? 0.0f : -ref;
+          // the weights, in packed pairs; rounded to bf16 for P V, summed unrounded
+          const float neg = now == -INFINITY ? 0.0f : -now;
+          const f32x2 neg2 = pack2(neg, neg), scale2 = pack2(scale, scale);
+          f32x2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (active) {
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int h = 0; h < 2; ++h) {
             uint32_t w[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float e0 = ex2_approx(fmaf(sc[32 * h + 2 * i], scale, neg));
-              const float e1 = ex2_approx(fmaf(sc[32 * h + 2 * i + 1], scale, neg));
-              sum[i & 3] += e0 + e1;
+              float e0, e1;
+              unpack2(fma2_rn(pack2(sc[32 * h + 2 * i], sc[32 * h + 2 * i + 1]), scale2, neg2), e0, e1);
+              e0 = ex2_approx(e0);
+              e1 = ex2_approx(e1);
+              sum[i & 1] = add2_rn(sum[i & 1], pack2(e0, e1));
               const __nv_bfloat162 b2 = __floats2bfloat162_rn(e0, e1);
               w[i] = *reinterpret_cast<const uint32_t *>(&b2);
             }
-            tmem_st16(s_at + 16u * uint32_t(h), w);
-            l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            if constexpr (T::kPShared) {  // row of 128 bytes, its 16-byte chunks swizzled
+              uint8_t *to = smem_raw + T::kQHiBytes + group * kPTileBytes + row * 128;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                *reinterpret_cast<uint4 *>(to + (((4 * h + c) ^ (row & 7)) << 4)) =
+                    make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+              }
+              if (h == 1) fence_proxy_async_shared();
+            } else {
+              tmem_st16(s_at + 16u * uint32_t(h), w);
+            }
+            if (!T::kPShared || h == 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) {
+                mbar_arrive(bar_p_full + 16u * uint32_t(group) + (T::kPShared ? 0u : 8u * uint32_t(h)));
+              }
+            }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_p_full + 16u * uint32_t(group) + 8u * uint32_t(h));
+          float a0, a1;
+          unpack2(add2_rn(sum[0], sum[1]), a0, a1);
+          l_run += a0 + a1;
         }
       }
       if (!ok) break;
@@ -989,11 +1100,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       // ---- the segment's end: Q of the next one, then this one's rows
       const int last = n1 - 1;
       const bool owner = (last & 1) == group;
-      if (!owner) {
-        ok = warp_wait(bar_s_full + 8u * uint32_t(last & 1), uint32_t(last >> 1) & 1u);
-        if (!ok) break;
-        tc_fence_after();
-      }
+      ok = warp_wait(bar_q_free, uint32_t(segments & 1));
+      if (!ok) break;
+      tc_fence_after();
       more = load_q(next_rows);
       if (!ok) break;
       if (active) {
@@ -1008,8 +1117,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           }
         }
       }
-      const int fill = last * T::kTileSlots + T::kKSlots;
-      ok = warp_wait(bar_done + 8u * slot_of(fill), parity_of(fill));
+      ok = warp_wait(bar_o_full, uint32_t(segments & 1));
       if (!ok) break;
       tc_fence_after();
       if (active) small.row_sum[group][row] = l_run;
