@@ -25,14 +25,16 @@
 //              CTA's piece of an item) and a key tile are.
 //   warp 10    issues the MMAs
 // Tensor memory (512 columns): O (128 x 256 fp32), Q (128 x 256 bf16: the A operand
-// of Q K^T), and two score buffers of 64 columns. K and V tiles go through a ring of
-// 32 KB shared-memory slots (64 keys x 256 dims, 128-byte swizzle).
-// head_dim 256: 6 slots, and two buffers (16 KB) for the bf16 weights, the A operand
-// of P V. A score buffer is free as soon as it has been read, so Q K^T runs two tiles
-// ahead of P V: the tensor pipe always has work queued, and a group of softmax warps
-// has two tiles' time for one.
+// of Q K^T), and two score buffers of 64 columns. K and V tiles go through two rings
+// of 32 KB shared-memory slots (64 keys x 256 dims, 128-byte swizzle); a segment's Q
+// comes through two slots of the K ring, ahead of its keys, and is copied to tensor
+// memory from there (tcgen05.cp), so the softmax warps never touch it.
+// head_dim 256: 3 + 3 slots, and two buffers (16 KB) for the bf16 weights, the A
+// operand of P V. A score buffer is free as soon as it has been read, so Q K^T runs
+// two tiles ahead of P V: the tensor pipe always has work queued, and a group of
+// softmax warps has two tiles' time for one.
 // head_dim 512: a tile takes two K slots and one V slot, the upper half of Q lies in
-// shared memory, 5 slots remain; the weights go back into tensor memory over the
+// shared memory, 3 + 2 slots remain; the weights go back into tensor memory over the
 // scores they come from (in two halves: P V starts on the first under the second), so
 // Q K^T runs one tile ahead. The output dims are two parts computed by different
 // items, each with all of Q K^T.
@@ -71,7 +73,7 @@ constexpr int kGroupBytes = 8 * kPartDims * 2;
 constexpr int kBlockBytes = 8 * 128;
 constexpr int kQBlockBytes = kRows * 128;     // 128 rows x 64 dims
 constexpr int kPTileBytes = kRows * kKeys * 2;  // weights of a tile
-constexpr int kMaxSlots = 6;
+constexpr int kMaxSlots = 3;                  // of a ring
 constexpr int kSoftmaxWarps = 8;
 constexpr int kThreads = (kSoftmaxWarps + 3) * 32;
 constexpr uint32_t kTmemColumns = 512;
@@ -94,14 +96,17 @@ struct ChunkTraits {
   static constexpr int kHeadDim = kHeadDim_;
   static constexpr int kKSlots = kHeadDim / 256;      // slots of one K tile
   static constexpr int kParts = kHeadDim / kPartDims;
-  static constexpr int kTileSlots = kKSlots + 1;
   static constexpr int kQHiBytes = (kHeadDim - 256) * kRows * 2;
   static constexpr bool kPShared = kHeadDim == 256;   // the weights in shared memory
   static constexpr int kPBytes = kPShared ? 2 * kPTileBytes : 0;
-  static constexpr int kSlots = kHeadDim == 256 ? 6 : 5;
+  static constexpr int kKRing = 3;
+  static constexpr int kVRing = kHeadDim == 256 ? 3 : 2;
   static constexpr int kLag = kPShared ? 2 : 1;       // tiles that Q K^T is ahead of P V
-  static constexpr int kRingAt = kQHiBytes + kPBytes; // shared memory: upper Q, weights, ring
-  static constexpr int kTileBytes = kRingAt + kSlots * kSlotBytes;
+  // shared memory: upper half of Q, weights, K ring, V ring
+  static constexpr int kPAt = kQHiBytes;
+  static constexpr int kKAt = kPAt + kPBytes;
+  static constexpr int kVAt = kKAt + kKRing * kSlotBytes;
+  static constexpr int kTileBytes = kVAt + kVRing * kSlotBytes;
 };
 
 // Division of 0 .. 2^31 - 1 by a fixed number: the quotient's high part by a 32-bit
@@ -135,6 +140,7 @@ struct ChunkParams {
   int32_t group;
   int32_t tile_tokens;   // 128 / group
   int32_t tiles_per_run; // query tiles of the longest run
+  int32_t q_box;         // tokens of a query box
   int32_t window;
   int32_t sinks;
   int32_t box;           // tokens per TMA box; 0: rows are copied one by one
@@ -258,15 +264,17 @@ struct SegmentInfo {
 };
 
 struct SmallState {
-  uint64_t full[kMaxSlots];   // the slot's tile has landed
-  uint64_t done[kMaxSlots];   // the MMAs that read the slot are complete
+  uint64_t k_full[kMaxSlots]; // the slot's tile (or half of Q) has landed
+  uint64_t k_done[kMaxSlots]; // the MMAs (or copies) that read the slot are complete
+  uint64_t v_full[kMaxSlots];
+  uint64_t v_done[kMaxSlots];
   uint64_t s_full[2];         // scores of the tile in S[b] complete
   uint64_t p_full[2][2];      // half of its weights written (and O rescaled where needed)
   uint64_t m_full[2][4];      // row_ref[b] of 32 rows written
   uint64_t l_full[2][4];      // row_sum of 32 rows written by the group
   uint64_t s_free[2];         // kPShared: the scores in S[b] have been read
-  uint64_t q_full;            // Q of the segment in tensor memory
-  uint64_t q_free;            // its last Q K^T is complete
+  uint64_t q_hi_full;         // head_dim 512: the upper half of the segment's Q has landed
+  uint64_t q_free;            // the segment's last Q K^T is complete
   uint64_t o_full;            // its last P V is complete
   uint64_t o_free;            // its O has been read back
   uint64_t seg_full[kSegments];
@@ -362,17 +370,55 @@ __device__ __forceinline__ unsigned long long low_bits(int n) {
   return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1ull);
 }
 
+// A warp's 32 rows of 128 bytes (lane = row, eight 16-byte chunks) through its 4 KB of
+// shared memory: eight lanes then store a row's whole line. to(r, c): where chunk c of
+// row r goes (called by all lanes); rows from `valid` on are not stored.
+template <class To>
+__device__ __forceinline__ void store_rows_staged(uint8_t *stage, const uint4 (&w)[8], int lane,
+                                                  int valid, To to) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    *reinterpret_cast<uint4 *>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = w[c];
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 3);
+    const int c = lane & 7;
+    const uint4 v = *reinterpret_cast<const uint4 *>(stage + r * 128 + ((c ^ (r & 7)) << 4));
+    uint4 *dst = to(r, c);
+    if (r < valid) *dst = v;
+  }
+  __syncwarp();
+}
+
+// 128 rows x 32 bytes of a swizzled block to eight columns of tensor memory.
+__device__ __forceinline__ void tmem_copy_warp(uint32_t d_tmem, uint32_t lo, uint32_t hi, bool leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t.reg .b64 d;\n\tsetp.ne.b32 q, %3, 0;\n\tmov.b64 d, {%1, %2};\n\t"
+      "@q tcgen05.cp.cta_group::1.128x256b [%0], d;\n\t}\n" ::"r"(d_tmem),
+      "r"(lo), "r"(hi), "r"(uint32_t(leader))
+      : "memory");
+}
+// One box of query rows x 64 dims: box tokens x the query heads of one KV head.
+__device__ __forceinline__ void tma_load_block(uint32_t dst, const CUtensorMap *map, int x, int head,
+                                               int row, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(row), "r"(bar)
+      : "memory");
+}
+
 template <class T>
 __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap map_k,
     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k_rows,
-    const __grid_constant__ CUtensorMap map_v_rows) {
-  constexpr int kSlots = T::kSlots;
+    const __grid_constant__ CUtensorMap map_v_rows, const __grid_constant__ CUtensorMap map_q) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   SmallState &small = *reinterpret_cast<SmallState *>(smem_raw + T::kTileBytes);
   const uint32_t s_q_hi = smem_u32(smem_raw);
-  const uint32_t s_p = s_q_hi + T::kQHiBytes;
-  const uint32_t s_ring = s_q_hi + T::kRingAt;
+  const uint32_t s_p = s_q_hi + T::kPAt;
   const int tid = int(threadIdx.x);
   const int warp = tid >> 5;
   const int lane = tid & 31;
@@ -382,22 +428,26 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     return;
   }
 
-  const uint32_t bar_full = smem_u32(&small.full[0]);      // + 8 slot
-  const uint32_t bar_done = smem_u32(&small.done[0]);      // + 8 slot
+  const uint32_t bar_k_full = smem_u32(&small.k_full[0]);  // + 8 slot
+  const uint32_t bar_k_done = smem_u32(&small.k_done[0]);  // + 8 slot
+  const uint32_t bar_v_full = smem_u32(&small.v_full[0]);  // + 8 slot
+  const uint32_t bar_v_done = smem_u32(&small.v_done[0]);  // + 8 slot
   const uint32_t bar_s_full = smem_u32(&small.s_full[0]);  // + 8 b
   const uint32_t bar_p_full = smem_u32(&small.p_full[0][0]);  // + 16 b + 8 half
   const uint32_t bar_m_full = smem_u32(&small.m_full[0][0]);  // + 32 b + 8 warp quarter
   const uint32_t bar_l_full = smem_u32(&small.l_full[0][0]);  // + 32 group + 8 warp quarter
   const uint32_t bar_s_free = smem_u32(&small.s_free[0]);  // + 8 b
-  const uint32_t bar_q_full = smem_u32(&small.q_full);
+  const uint32_t bar_q_hi_full = smem_u32(&small.q_hi_full);
   const uint32_t bar_q_free = smem_u32(&small.q_free);
   const uint32_t bar_o_full = smem_u32(&small.o_full);
   const uint32_t bar_o_free = smem_u32(&small.o_free);
   const uint32_t bar_seg_full = smem_u32(&small.seg_full[0]);  // + 8 (segment % kSegments)
   if (tid == 0) {
-    for (int i = 0; i < kSlots; ++i) {
-      mbar_init(bar_full + 8u * i, 1);
-      mbar_init(bar_done + 8u * i, 1);
+    for (int i = 0; i < kMaxSlots; ++i) {
+      mbar_init(bar_k_full + 8u * i, 1);
+      mbar_init(bar_k_done + 8u * i, 1);
+      mbar_init(bar_v_full + 8u * i, 1);
+      mbar_init(bar_v_done + 8u * i, 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_s_full + 8u * b, 1);
@@ -410,7 +460,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     }
     mbar_init(bar_s_free, 4);
     mbar_init(bar_s_free + 8u, 4);
-    mbar_init(bar_q_full, kSoftmaxWarps);
+    mbar_init(bar_q_hi_full, 1);
     mbar_init(bar_q_free, 1);
     mbar_init(bar_o_full, 1);
     mbar_init(bar_o_free, kSoftmaxWarps);
@@ -508,10 +558,19 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       }
     }
   };
-  // The slots are filled and freed in order: fill i uses slot i % kSlots for the
-  // (i / kSlots)-th time. Fill i of a tile n: i = n * kTileSlots (+ 1) for K, then V.
-  auto slot_of = [](int fill) { return uint32_t(fill % kSlots); };
-  auto parity_of = [](int fill) { return uint32_t(fill / kSlots) & 1u; };
+  // A ring's slots are filled and freed in order: a role keeps the slot of its next
+  // fill and the parity of that slot's use. V of key tile n is fill n of its ring.
+  struct Cursor {
+    uint32_t slot = 0, phase = 0;
+    __device__ __forceinline__ void advance(uint32_t slots) {
+      if (++slot == slots) {
+        slot = 0;
+        phase ^= 1u;
+      }
+    }
+  };
+  auto v_slot = [](int tile) { return uint32_t(tile % T::kVRing); };
+  auto v_parity = [](int tile) { return uint32_t(tile / T::kVRing) & 1u; };
 
   if (warp == kSoftmaxWarps || warp == kSoftmaxWarps + 1) {
     // ------------------------------------------------------------ loaders of K and V
@@ -525,8 +584,11 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     const int batch_tiles = p.box > 0 ? 32 / tile_boxes : 1;    // key tiles of a look-up
     const int page_groups = p.cfg.page_size / 8;
     const int layer_group = p.layer * p.cfg.num_pages * page_groups;
-    int slot = is_v ? T::kKSlots : 0;
-    uint32_t phase = 0;  // of the slot's current use
+    const uint32_t ring = s_q_hi + (is_v ? T::kVAt : T::kKAt);
+    const uint32_t ring_slots = is_v ? T::kVRing : T::kKRing;
+    const uint32_t bar_full = is_v ? bar_v_full : bar_k_full;
+    const uint32_t bar_done = is_v ? bar_v_done : bar_k_done;
+    Cursor at;
     int n = 0, segments = 0;
     int4 meta = make_int4(-1, 0, 0, 0);
     ChunkRun mine;
@@ -558,14 +620,38 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           meta.y = s.run_index;
           meta.z = s.query_tile;
         }
-        // the query rows of the segment, which the softmax warps will ask for
-        const int tokens = s.t1 - s.t0 + 1;
-        for (int i = lane; i < tokens; i += 32) {
-          const __nv_bfloat16 *q = p.q + ((int64_t(s.run.start) + s.token0 + i) * p.q_heads +
-                                          head * p.group) * T::kHeadDim;
-          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(q),
-                       "r"(p.group * T::kHeadDim * 2)
-                       : "memory");
+        // Q: 64-dim blocks of box_rows rows, two to a slot (rows behind the segment's are
+        // other runs', or zeros behind the last: nobody looks at what comes of them)
+        const int token = s.run.start + s.token0;
+        const uint32_t block_bytes = uint32_t(p.q_box * p.group) * 128u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          ok = ok && __all_sync(0xffffffffu, wait(bar_k_done + 8u * at.slot, at.phase ^ 1u));
+          if (!ok) break;
+          if (lane == 0) {
+            const uint32_t bar = bar_k_full + 8u * at.slot;
+            mbar_arrive_expect_tx(bar, 2u * block_bytes);
+            for (int b = 0; b < 2; ++b) {
+              tma_load_block(ring + at.slot * kSlotBytes + uint32_t(b) * kQBlockBytes, &map_q,
+                             (2 * h + b) * 64, head * p.group, token, bar);
+            }
+          }
+          __syncwarp();
+          at.advance(ring_slots);
+        }
+        if constexpr (T::kKSlots == 2) {
+          // its place is free when the last segment's Q K^T is complete
+          if (ok && segments > 1) {
+            ok = __all_sync(0xffffffffu, wait(bar_q_free, uint32_t(segments - 2) & 1u));
+          }
+          if (ok && lane == 0) {
+            mbar_arrive_expect_tx(bar_q_hi_full, 4u * block_bytes);
+            for (int b = 0; b < 4; ++b) {
+              tma_load_block(s_q_hi + uint32_t(b) * kQBlockBytes, &map_q, 256 + b * 64,
+                             head * p.group, token, bar_q_hi_full);
+            }
+          }
+          __syncwarp();
         }
       }
       int j = s.begin;
@@ -668,15 +754,15 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
             if (is_v && f > 0) break;
             const int block0 = is_v ? part * 4 : f * 4;
             // the slot's last reader is done (a slot's first use waits for nothing)
-            ok = __all_sync(0xffffffffu, wait(bar_done + 8u * uint32_t(slot), phase ^ 1u));
+            ok = __all_sync(0xffffffffu, wait(bar_done + 8u * at.slot, at.phase ^ 1u));
             if (!ok) break;
             if (!is_v && f == 0 && lane == 0) {
               const bool edge = live != ~0ull || base + kKeys - 1 > s.t0 ||
                                 (p.window > 0 && base <= s.t1 - p.window && base + kKeys > p.sinks);
               small.info[n % kInfos] = {live, base, edge ? 1 : 0};
             }
-            const uint32_t bar = bar_full + 8u * uint32_t(slot);
-            const uint32_t dst = s_ring + uint32_t(slot) * kSlotBytes;
+            const uint32_t bar = bar_full + 8u * at.slot;
+            const uint32_t dst = ring + at.slot * kSlotBytes;
             if (p.box == 0) {
               int64_t row_at[2];  // element offset of rows lane, lane + 32
 #pragma unroll
@@ -720,11 +806,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
                                   head, bar);
               }
             }
-            slot += is_v ? T::kTileSlots : (f + 1 < T::kKSlots ? 1 : T::kTileSlots - T::kKSlots + 1);
-            if (slot >= kSlots) {
-              slot -= kSlots;
-              phase ^= 1u;
-            }
+            at.advance(ring_slots);
           }
           if (!ok) break;
         }
@@ -734,11 +816,14 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     if (!is_v && lane == 0) p.meta[blockIdx.x] = meta;
     if (!ok || *abort_flag != 0) {
       // nobody may be waiting for the last loads any more: see them land before the
-      // CTA gives its shared memory back
-      for (int i = max(0, (n + 1) * T::kTileSlots - 2 * kSlots); i < n * T::kTileSlots; ++i) {
-        if ((i % T::kTileSlots == T::kKSlots) == is_v) {
-          mbar_wait_bounded(bar_full + 8u * slot_of(i), parity_of(i), kTileWaitClocks);
-        }
+      // CTA gives its shared memory back. The slots before the cursor were filled in
+      // its phase, those behind it in the phase before (a slot that never was passes:
+      // parity 1 of a fresh barrier counts as complete).
+      for (uint32_t i = 0; i < ring_slots; ++i) {
+        mbar_wait_bounded(bar_full + 8u * i, i < at.slot ? at.phase : at.phase ^ 1u, kTileWaitClocks);
+      }
+      if (T::kKSlots == 2 && !is_v && segments > 0) {
+        mbar_wait_bounded(bar_q_hi_full, uint32_t(segments - 1) & 1u, kTileWaitClocks);
       }
     }
   } else if (warp == kSoftmaxWarps + 2) {
@@ -755,33 +840,52 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     auto warp_wait = [&](uint32_t bar, uint32_t parity) -> bool {
       return __all_sync(0xffffffffu, wait(bar, parity));
     };
-    // position in the ring of K of the next tile to score and of V of the next to add
-    struct Cursor {
-      uint32_t slot, phase;
-      __device__ __forceinline__ void advance(uint32_t by) {
-        slot += by;
-        if (slot >= kSlots) {
-          slot -= kSlots;
-          phase ^= 1u;
-        }
-      }
-    };
-    Cursor k_at = {0, 0}, v_at = {uint32_t(T::kKSlots), 0};
-    Cursor v_last = v_at;  // of the tile before v_at's
-    int n = 0;             // tiles whose Q K^T has been issued
-    int added = 0;         // tiles whose P V has been issued
+    Cursor k_at, v_at;  // K of the next tile to score, V of the next to add
+    uint32_t v_last_slot = 0, v_last_phase = 0;  // V of the last tile added
+    int n = 0;          // tiles whose Q K^T has been issued
+    int added = 0;      // tiles whose P V has been issued
     int segments = 0;
     bool ok = true;
+    auto s_free_parity = [&]() { return uint32_t((n - 2) >> 1) & 1u; };
+    auto p_bar = [&](int half) { return bar_p_full + 16u * (uint32_t(added) & 1u) + 8u * uint32_t(half); };
+    auto p_parity = [&]() { return uint32_t(added >> 1) & 1u; };
+    // S[n & 1] = Q K^T of tile n: 16 steps of 16 dims per K slot, four to a block
+    auto issue_qk = [&](bool waited, bool last) -> bool {
+      const uint32_t d = tmem + kTmemS + uint32_t(n & 1) * kKeys;
+#pragma unroll
+      for (int f = 0; f < T::kKSlots; ++f) {
+        if (!(waited && f == 0) && !warp_wait(bar_k_full + 8u * k_at.slot, k_at.phase)) return false;
+        tc_fence_after();
+        const uint32_t k = ((s_q_hi + T::kKAt + k_at.slot * kSlotBytes) >> 4) | kLoK;
+        const uint32_t q_hi = (s_q_hi >> 4) | kLoK;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t at = uint32_t(i >> 2) * (kBlockBytes >> 4) + uint32_t(i & 3) * 2u;
+          if (f == 0) {
+            umma_bf16_a_tmem_warp(d, tmem + kTmemQ + 8u * uint32_t(i), k + at, kHiSlot, kIdescQK,
+                                  i > 0, leader);
+          } else {
+            umma_bf16_warp(d, q_hi + uint32_t(i >> 2) * (kQBlockBytes >> 4) + uint32_t(i & 3) * 2u,
+                           kHiQ, k + at, kHiSlot, kIdescQK, true, leader);
+          }
+        }
+        umma_commit_warp(bar_k_done + 8u * k_at.slot, leader);
+        k_at.advance(T::kKRing);
+      }
+      umma_commit_warp(bar_s_full + 8u * uint32_t(n & 1), leader);
+      if (last) umma_commit_warp(bar_q_free, leader);
+      ++n;
+      return true;
+    };
     // O (+)= P V of tile `added`: four steps of 16 keys
-    auto issue_pv = [&](bool accumulate) -> bool {
+    auto issue_pv = [&](bool waited, bool accumulate) -> bool {
       const uint32_t b = uint32_t(added) & 1u;
-      const uint32_t parity = uint32_t(added >> 1) & 1u;
-      if (!warp_wait(bar_full + 8u * v_at.slot, v_at.phase)) return false;
-      const uint32_t v = ((s_ring + v_at.slot * kSlotBytes) >> 4) | kLoV;
+      if (!waited && !warp_wait(bar_v_full + 8u * v_at.slot, v_at.phase)) return false;
+      const uint32_t v = ((s_q_hi + T::kVAt + v_at.slot * kSlotBytes) >> 4) | kLoV;
 #pragma unroll
       for (int i = 0; i < kKeys / 16; ++i) {
         if (i == 0 || (i == 2 && !T::kPShared)) {
-          if (!warp_wait(bar_p_full + 16u * b + 4u * uint32_t(i), parity)) return false;
+          if (!(waited && i == 0) && !warp_wait(p_bar(i / 2), p_parity())) return false;
           tc_fence_after();
         }
         const uint32_t vi = v + uint32_t(i) * (2u * kGroupBytes >> 4);
@@ -793,9 +897,10 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
                                 kIdescPV, accumulate || i > 0, leader);
         }
       }
-      umma_commit_warp(bar_done + 8u * v_at.slot, leader);
-      v_last = v_at;
-      v_at.advance(T::kTileSlots);
+      umma_commit_warp(bar_v_done + 8u * v_at.slot, leader);
+      v_last_slot = v_at.slot;
+      v_last_phase = v_at.phase;
+      v_at.advance(T::kVRing);
       ++added;
       return true;
     };
@@ -806,42 +911,44 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       const int tiles = small.segment[segments % kSegments].tiles;
       if (tiles == 0) break;
       const int first = n;
-      ok = warp_wait(bar_q_full, uint32_t(segments & 1));
+      // Q into tensor memory, when the last segment's Q K^T no longer reads what is there
+      if (segments > 0) ok = warp_wait(bar_q_free, uint32_t(segments - 1) & 1u);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ok = ok && warp_wait(bar_k_full + 8u * k_at.slot, k_at.phase);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t q = ((s_q_hi + T::kKAt + k_at.slot * kSlotBytes) >> 4) | kLoK;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          tmem_copy_warp(tmem + kTmemQ + 64u * uint32_t(h) + 8u * uint32_t(i),
+                         q + uint32_t(i >> 2) * (kQBlockBytes >> 4) + uint32_t(i & 3) * 2u, kHiQ, leader);
+        }
+        umma_commit_warp(bar_k_done + 8u * k_at.slot, leader);
+        k_at.advance(T::kKRing);
+      }
+      if (T::kKSlots == 2) ok = ok && warp_wait(bar_q_hi_full, uint32_t(segments & 1));
       // one step beyond the segment's tiles per tile that P V lags behind
       for (int j = 0; j < tiles + T::kLag && ok; ++j) {
+        bool ready = false;
+        if (T::kPShared && j < tiles && j >= T::kLag) {
+          // What both products wait for, asked for at once: a wait costs its latency
+          // even where nothing is waited for, and the tensor pipe has only what is
+          // queued to run under it.
+          ready = mbar_try_wait(bar_s_free + 8u * uint32_t(n & 1), s_free_parity()) &
+                  mbar_try_wait(bar_k_full + 8u * k_at.slot, k_at.phase) &
+                  mbar_try_wait(bar_v_full + 8u * v_at.slot, v_at.phase) &
+                  mbar_try_wait(p_bar(0), p_parity());
+          ready = __all_sync(0xffffffffu, ready);
+        }
         if (j < tiles) {
           // S[n & 1] held the scores (kPShared) or the weights of tile n - 2
-          if (n >= 2) {
-            ok = T::kPShared ? warp_wait(bar_s_free + 8u * uint32_t(n & 1), uint32_t((n - 2) >> 1) & 1u)
-                             : warp_wait(bar_done + 8u * v_last.slot, v_last.phase);
-            if (!ok) break;
+          if (n >= 2 && !ready) {
+            ok = T::kPShared ? warp_wait(bar_s_free + 8u * uint32_t(n & 1), s_free_parity())
+                             : warp_wait(bar_v_done + 8u * v_last_slot, v_last_phase);
           }
-          const uint32_t d = tmem + kTmemS + uint32_t(n & 1) * kKeys;
-#pragma unroll
-          for (int f = 0; f < T::kKSlots; ++f) {
-            ok = ok && warp_wait(bar_full + 8u * k_at.slot, k_at.phase);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t k = ((s_ring + k_at.slot * kSlotBytes) >> 4) | kLoK;
-            const uint32_t q_hi = (s_q_hi >> 4) | kLoK;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {  // steps of 16 dims, four to a block
-              const uint32_t at = uint32_t(i >> 2) * (kBlockBytes >> 4) + uint32_t(i & 3) * 2u;
-              if (f == 0) {
-                umma_bf16_a_tmem_warp(d, tmem + kTmemQ + 8u * uint32_t(i), k + at, kHiSlot, kIdescQK,
-                                      i > 0, leader);
-              } else {
-                umma_bf16_warp(d, q_hi + uint32_t(i >> 2) * (kQBlockBytes >> 4) + uint32_t(i & 3) * 2u,
-                               kHiQ, k + at, kHiSlot, kIdescQK, true, leader);
-              }
-            }
-            umma_commit_warp(bar_done + 8u * k_at.slot, leader);
-            k_at.advance(f + 1 < T::kKSlots ? 1 : T::kTileSlots - T::kKSlots + 1);
-          }
+          ok = ok && issue_qk(ready, j + 1 == tiles);
           if (!ok) break;
-          umma_commit_warp(bar_s_full + 8u * uint32_t(n & 1), leader);
-          if (j + 1 == tiles) umma_commit_warp(bar_q_free, leader);
-          ++n;
         }
         if (j >= T::kLag) {
           // the segment's first P V writes O anew: the last segment's rows must be out
@@ -849,7 +956,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
             ok = warp_wait(bar_o_free, uint32_t(segments - 1) & 1u);
             if (!ok) break;
           }
-          ok = issue_pv(added > first);
+          ok = issue_pv(ready, added > first);
         }
       }
       if (ok) umma_commit_warp(bar_o_full, leader);
@@ -879,10 +986,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       int part;
       int piece;     // 0, 1: which of the CTA's partial results; -1: the item is whole
     };
-    // Q rows of the next segment: this group's half of the dims into tensor memory
-    // (and, head_dim 512, its half of the upper dims into shared memory)
     int asked = 0;  // segments so far
-    auto load_q = [&](Rows &kept) -> bool {
+    auto next_segment = [&](Rows &kept) -> bool {
       if (!warp_wait(bar_seg_full + 8u * uint32_t(asked % kSegments),
                      uint32_t(asked / kSegments) & 1u)) {
         ok = false;
@@ -897,42 +1002,10 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       kept.part = s.hp / heads;
       kept.piece = s.piece;
       kept.at = (int64_t(s.row0) + token) * p.q_heads + (s.hp - kept.part * heads) * p.group + head_of_group;
-      const bool active = 32 * quarter < s.rows;
-      if (active) {
-        const __nv_bfloat16 *src = p.q + kept.at * T::kHeadDim + 128 * group;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          uint32_t w[32];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint4 v = row < kept.rows ? __ldg(reinterpret_cast<const uint4 *>(src) + 8 * h + i)
-                                            : make_uint4(0, 0, 0, 0);
-            w[4 * i] = v.x;
-            w[4 * i + 1] = v.y;
-            w[4 * i + 2] = v.z;
-            w[4 * i + 3] = v.w;
-          }
-          tmem_st32(tmem + lanes + kTmemQ + 64u * uint32_t(group) + 32u * uint32_t(h),
-                    reinterpret_cast<const float *>(w));
-        }
-        if constexpr (T::kKSlots == 2) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint4 hi = row < s.rows ? __ldg(reinterpret_cast<const uint4 *>(src + 256) + i)
-                                          : make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4 *>(smem_raw + (2 * group + (i >> 3)) * kQBlockBytes + row * 128 +
-                                       (((i & 7) ^ (row & 7)) << 4)) = hi;
-          }
-          fence_proxy_async_shared();
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_q_full);
       return true;
     };
-    Rows now_rows, next_rows;
-    bool more = load_q(now_rows);
+    Rows now_rows;
+    bool more = next_segment(now_rows);
     while (more && ok) {
       const bool active = 32 * quarter < now_rows.rows;  // some row of the warp is a query
       const int t = now_rows.t;
@@ -941,9 +1014,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       float ref = -INFINITY;  // what l_run's weights are scaled by
       // V rows that no row of the tile sees become zeros
       auto clear_v = [&](int n, unsigned long long live) -> bool {
-        const int fill = n * T::kTileSlots + T::kKSlots;
-        if (!warp_wait(bar_full + 8u * slot_of(fill), parity_of(fill))) return false;
-        uint8_t *v = smem_raw + T::kRingAt + slot_of(fill) * kSlotBytes + (lane >> 3) * kBlockBytes +
+        if (!warp_wait(bar_v_full + 8u * v_slot(n), v_parity(n))) return false;
+        uint8_t *v = smem_raw + T::kVAt + v_slot(n) * kSlotBytes + (lane >> 3) * kBlockBytes +
                      (lane & 7) * 16;
         // the rows quarter, quarter + 4, ...: bits 0, 4, 8, ... of
         unsigned long long dead = (~live >> quarter) & 0x1111111111111111ull;
@@ -965,8 +1037,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           if (live != ~0ull) ok = clear_v(n, live);
           if (!ok) break;
           if (T::kPShared && n >= 2) {  // not a phase ahead of the other warps' weights
-            const int fill = (n - 2) * T::kTileSlots + T::kKSlots;
-            ok = warp_wait(bar_done + 8u * slot_of(fill), parity_of(fill));
+            ok = warp_wait(bar_v_done + 8u * v_slot(n - 2), v_parity(n - 2));
             if (!ok) break;
           }
           __syncwarp();
@@ -1012,8 +1083,10 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
 #pragma unroll
             for (int u = 0; u < 4; ++u) mx[u] = max3(mx[u], sc[c + u], sc[c + 4 + u]);
           }
-          const float m_tile = fmaxf(max3(mx[0], mx[1], max3(mx[2], mx[3], sc[60])),
-                                     max3(sc[61], sc[62], sc[63])) * scale;
+          float m_tile = fmaxf(max3(mx[0], mx[1], max3(mx[2], mx[3], sc[60])),
+                               max3(sc[61], sc[62], sc[63])) * scale;
+          // rows behind the last hold anything: they must not make the warp rescale
+          if (row >= now_rows.rows) m_tile = 0.0f;
           // the reference so far: the other group's tile before this one
           float last = -INFINITY;
           if (n > n0) {
@@ -1034,8 +1107,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
             ref = now;
             const bool raised = last != -INFINITY && now != last;
             if (__any_sync(0xffffffffu, raised)) {
-              const int fill = (n - 1) * T::kTileSlots + T::kKSlots;
-              ok = warp_wait(bar_done + 8u * slot_of(fill), parity_of(fill));
+              ok = warp_wait(bar_v_done + 8u * v_slot(n - 1), v_parity(n - 1));
               if (!ok) break;
               tc_fence_after();
               const float factor = raised ? ex2_approx(last - now) : 1.0f;
@@ -1050,8 +1122,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
             }
           }
           if (T::kPShared && n >= 2) {  // the buffer's last weights have been used
-            const int fill = (n - 2) * T::kTileSlots + T::kKSlots;
-            ok = warp_wait(bar_done + 8u * slot_of(fill), parity_of(fill));
+            ok = warp_wait(bar_v_done + 8u * v_slot(n - 2), v_parity(n - 2));
             if (!ok) break;
           }
           // the weights, in packed pairs; rounded to bf16 for P V, summed unrounded
@@ -1072,7 +1143,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
               w[i] = *reinterpret_cast<const uint32_t *>(&b2);
             }
             if constexpr (T::kPShared) {  // row of 128 bytes, its 16-byte chunks swizzled
-              uint8_t *to = smem_raw + T::kQHiBytes + group * kPTileBytes + row * 128;
+              uint8_t *to = smem_raw + T::kPAt + group * kPTileBytes + row * 128;
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 *reinterpret_cast<uint4 *>(to + (((4 * h + c) ^ (row & 7)) << 4)) =
@@ -1097,14 +1168,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       }
       if (!ok) break;
 
-      // ---- the segment's end: Q of the next one, then this one's rows
+      // ---- the segment's end
       const int last = n1 - 1;
       const bool owner = (last & 1) == group;
-      ok = warp_wait(bar_q_free, uint32_t(segments & 1));
-      if (!ok) break;
-      tc_fence_after();
-      more = load_q(next_rows);
-      if (!ok) break;
       if (active) {
         if (!owner) {
           ok = warp_wait(bar_m_full + 32u * uint32_t(group ^ 1) + 8u * uint32_t(quarter),
@@ -1132,7 +1198,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       const float inv = whole ? (l_row > 0.0f ? 1.0f / l_row : 0.0f) : 1.0f;
       float *piece = p.partials + (int64_t(blockIdx.x) * 2 + (whole ? 0 : now_rows.piece)) *
                                       (int64_t(p.rows_cap) * (kPartDims + 2));
-      // 64 columns at a time; the second half frees O before its stores
+      // 64 columns at a time; O is free once the second half has been read. head_dim
+      // 256: through the group's weight buffer (its P V is complete; each warp has its
+      // 4 KB of it) so that a store covers whole 128-byte lines, not 32 rows of 16 bytes.
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
         const int column = 128 * group + 64 * h;
@@ -1143,24 +1211,54 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_o_free);
         }
-        if (writes && whole) {
-          uint4 *dst = reinterpret_cast<uint4 *>(p.out + now_rows.at * T::kHeadDim + now_rows.part * kPartDims +
-                                                column);
+        if (!active) continue;
+        uint8_t *stage = smem_raw + T::kPAt + group * kPTileBytes + quarter * 4096;
+        const int valid = now_rows.rows - 32 * quarter;  // rows of the warp
+        if (whole) {
+          uint4 w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            uint32_t w[4];
+            uint32_t x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const __nv_bfloat162 b2 =
                   __floats2bfloat162_rn(o[8 * i + 2 * j] * inv, o[8 * i + 2 * j + 1] * inv);
-              w[j] = *reinterpret_cast<const uint32_t *>(&b2);
+              x[j] = *reinterpret_cast<const uint32_t *>(&b2);
             }
-            dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            w[i] = make_uint4(x[0], x[1], x[2], x[3]);
           }
-        } else if (writes) {
-          float4 *acc = reinterpret_cast<float4 *>(piece + row * kPartDims + column);
+          __nv_bfloat16 *dst = p.out + now_rows.part * kPartDims + column;
+          if constexpr (T::kPShared) {
+            store_rows_staged(stage, w, lane, valid, [&](int r, int c) {
+              const int64_t at = __shfl_sync(0xffffffffu, now_rows.at, r);
+              return reinterpret_cast<uint4 *>(dst + at * T::kHeadDim) + c;
+            });
+          } else if (writes) {
+            uint4 *to = reinterpret_cast<uint4 *>(dst + now_rows.at * T::kHeadDim);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int i = 0; i < 8; ++i) to[i] = w[i];
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            uint4 w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float *x = o + 32 * q + 4 * i;
+              w[i] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                                __float_as_uint(x[3]));
+            }
+            float *dst = piece + 32 * quarter * kPartDims + column + 32 * q;
+            if constexpr (T::kPShared) {
+              store_rows_staged(stage, w, lane, valid, [&](int r, int c) {
+                return reinterpret_cast<uint4 *>(dst + r * kPartDims) + c;
+              });
+            } else if (writes) {
+              uint4 *to = reinterpret_cast<uint4 *>(dst + lane * kPartDims);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) to[i] = w[i];
+            }
+          }
         }
       }
       if (writes && group == 0) {
@@ -1172,7 +1270,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         }
       }
       n0 = n1;
-      now_rows = next_rows;
+      more = next_segment(now_rows);
       ++segments;
     }
   }
@@ -1298,6 +1396,20 @@ bool make_rows_map(CUtensorMap *map, const __nv_bfloat16 *base, int rows, int he
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_q_map(CUtensorMap *map, const __nv_bfloat16 *q, int rows, int q_heads, int head_dim,
+                int group, int box_tokens) {
+  EncodeTiledFn encode = encode_tiled_fn();
+  if (encode == nullptr) return false;
+  const cuuint64_t row = cuuint64_t(q_heads) * head_dim * 2;
+  const cuuint64_t dims[3] = {cuuint64_t(head_dim), cuuint64_t(q_heads), cuuint64_t(rows)};
+  const cuuint64_t strides[2] = {cuuint64_t(head_dim) * 2, row};
+  const cuuint32_t box[3] = {64, cuuint32_t(group), cuuint32_t(box_tokens)};
+  const cuuint32_t steps[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16 *>(q), dims,
+                strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Query rows a partial result can have, and the workspace of one CTA: its meta word
 // and two partial results.
 int partial_rows(int group, int max_row_count) {
@@ -1338,7 +1450,11 @@ cudaError_t launch_chunk(const ChunkAttentionArgs &a, int ctas, cudaStream_t str
   p.meta = static_cast<int4 *>(a.workspace);
   p.partials = reinterpret_cast<float *>(p.meta + ctas);
   p.status = a.status;
-  CUtensorMap map_k = {}, map_v = {}, map_k_rows = {}, map_v_rows = {};
+  p.q_box = std::min(p.tile_tokens, a.runs.max_row_count);
+  CUtensorMap map_q = {}, map_k = {}, map_v = {}, map_k_rows = {}, map_v_rows = {};
+  if (!make_q_map(&map_q, a.q, a.runs.rows, a.q_heads, c.head_dim, p.group, p.q_box)) {
+    return cudaErrorInvalidValue;
+  }
   if (p.box > 0 && (!make_cache_map(&map_k, a.cache_k, c, p.box) ||
                     !make_cache_map(&map_v, a.cache_v, c, p.box))) {
     return cudaErrorInvalidValue;
@@ -1352,7 +1468,8 @@ cudaError_t launch_chunk(const ChunkAttentionArgs &a, int ctas, cudaStream_t str
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, kChunkSmemBytes<T>);
   if (st != cudaSuccess) return st;
   st = launch_pdl(chunk_attention_kernel<T>, dim3(unsigned(ctas)), dim3(kThreads),
-                  size_t(kChunkSmemBytes<T>), stream, p, map_k, map_v, map_k_rows, map_v_rows);
+                  size_t(kChunkSmemBytes<T>), stream, p, map_k, map_v, map_k_rows, map_v_rows,
+                  map_q);
   if (st != cudaSuccess) return st;
   const unsigned row_blocks = unsigned(std::min(4, div_up(p.rows_cap, kCombineWarps)));
   return launch_pdl(chunk_combine_kernel, dim3(unsigned(ctas), row_blocks), dim3(kCombineWarps * 32), 0,
