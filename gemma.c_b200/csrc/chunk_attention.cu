@@ -146,6 +146,7 @@ struct ChunkParams {
   int32_t box;           // tokens per TMA box; 0: rows are copied one by one
   FastDiv page_div;      // by page_size
   FastDiv slot_div;      // by max_pages_per_seq
+  FastDiv run_div;       // by tiles_per_run
   float scale_log2;
   int4 *meta;            // per CTA: see PartialMeta
   float *partials;       // [cta][2] x (acc [rows_cap][256], m [rows_cap], l [rows_cap])
@@ -370,26 +371,23 @@ __device__ __forceinline__ unsigned long long low_bits(int n) {
   return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1ull);
 }
 
-// A warp's 32 rows of 128 bytes (lane = row, eight 16-byte chunks) through its 4 KB of
-// shared memory: eight lanes then store a row's whole line. to(r, c): where chunk c of
-// row r goes (called by all lanes); rows from `valid` on are not stored.
-template <class To>
-__device__ __forceinline__ void store_rows_staged(uint8_t *stage, const uint4 (&w)[8], int lane,
-                                                  int valid, To to) {
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// Eight 32-bit columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint4 (&w)[2]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      : "=r"(w[0].x), "=r"(w[0].y), "=r"(w[0].z), "=r"(w[0].w), "=r"(w[1].x), "=r"(w[1].y),
+        "=r"(w[1].z), "=r"(w[1].w)
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    *reinterpret_cast<uint4 *>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = w[c];
+  for (int i = 0; i < 2; ++i) {
+    asm volatile("" : "+r"(w[i].x), "+r"(w[i].y), "+r"(w[i].z), "+r"(w[i].w));  // not before the wait
   }
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = 4 * i + (lane >> 3);
-    const int c = lane & 7;
-    const uint4 v = *reinterpret_cast<const uint4 *>(stage + r * 128 + ((c ^ (r & 7)) << 4));
-    uint4 *dst = to(r, c);
-    if (r < valid) *dst = v;
-  }
-  __syncwarp();
 }
 
 // 128 rows x 32 bytes of a swizzled block to eight columns of tensor memory.
@@ -483,8 +481,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   const int pairs = p.runs.run_count * p.tiles_per_run;
   const int per_thread = div_up(pairs, kThreads);
   auto pair_cost = [&](int pair) -> int {
-    const ChunkRun run = chunk_run(p.runs, pair / p.tiles_per_run, p.cfg.batch_size);
-    const int token0 = (pair % p.tiles_per_run) * p.tile_tokens;
+    const int of_run = p.run_div.quotient(pair);
+    const ChunkRun run = chunk_run(p.runs, of_run, p.cfg.batch_size);
+    const int token0 = (pair - of_run * p.tiles_per_run) * p.tile_tokens;
     if (token0 >= run.count) return 0;
     const int t0 = run.first + token0;
     const int t1 = t0 + min(p.tile_tokens, run.count - token0) - 1;
@@ -509,17 +508,24 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     per_head += small.scan[w];
   }
   before += warps_before - mine;  // costs before this thread's first pair
+  // an even cut; 32-bit divisions where they do (nearly always)
   const long long total = per_head * heads * T::kParts;
-  const long long ctas = max(1ll, min((long long)gridDim.x, total / kMinShare));
-  const long long c0 = blockIdx.x < ctas ? total * blockIdx.x / ctas : 0;
-  const long long c1 = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
+  const long long most = min((long long)gridDim.x, (long long)kMinShare * gridDim.x > total
+                                                       ? (long long)(uint32_t(total) / kMinShare)
+                                                       : (long long)gridDim.x);
+  const int ctas = int(max(1ll, most));
+  const long long share = total < (1ll << 31) ? (long long)(uint32_t(total) / uint32_t(ctas)) : total / ctas;
+  const int extra = int(total - share * ctas);  // the first CTAs have one more
+  const int cta = int(blockIdx.x);
+  const long long c0 = cta < ctas ? share * cta + min(cta, extra) : 0;
+  const long long c1 = cta < ctas ? c0 + share + (cta < extra ? 1 : 0) : 0;
   if (tid == 0) {
     small.start.left = 0;
     small.start.hp = small.start.run = small.start.tile = small.start.offset = 0;
   }
   __syncthreads();
   if (c1 > c0) {
-    const int hp = int(c0 / per_head);
+    const int hp = total < (1ll << 31) ? int(uint32_t(c0) / uint32_t(per_head)) : int(c0 / per_head);
     long long rem = c0 - (long long)hp * per_head;
     if (rem >= before && rem < before + mine) {
       rem -= before;
@@ -530,8 +536,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       }
       small.start.left = c1 - c0;
       small.start.hp = hp;
-      small.start.run = pair / p.tiles_per_run;
-      small.start.tile = pair % p.tiles_per_run;
+      small.start.run = p.run_div.quotient(pair);
+      small.start.tile = pair - small.start.run * p.tiles_per_run;
       small.start.offset = int(rem);
     }
   }
@@ -775,7 +781,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
               }
               const __nv_bfloat16 *from = own ? rows : cache;
               const uint32_t column = dst + uint32_t(lane >> 3) * kBlockBytes;
-#pragma unroll 8
+#pragma unroll 4
               for (int r = 0; r < kKeys; ++r) {
                 const int64_t at = __shfl_sync(0xffffffffu, row_at[r >> 5], r & 31);
                 if (at >= 0) {
@@ -1198,67 +1204,69 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       const float inv = whole ? (l_row > 0.0f ? 1.0f / l_row : 0.0f) : 1.0f;
       float *piece = p.partials + (int64_t(blockIdx.x) * 2 + (whole ? 0 : now_rows.piece)) *
                                       (int64_t(p.rows_cap) * (kPartDims + 2));
-      // 64 columns at a time; O is free once the second half has been read. head_dim
-      // 256: through the group's weight buffer (its P V is complete; each warp has its
-      // 4 KB of it) so that a store covers whole 128-byte lines, not 32 rows of 16 bytes.
+      // This group's 128 columns of O, 32 lines of 128 bytes per warp at a time: 64
+      // columns as bf16, or 32 as fp32. head_dim 256: through the group's weight buffer
+      // (its P V is complete; each warp has its 4 KB of it), so that a store covers whole
+      // lines, not 32 rows of 16 bytes. Rolled loops: this code runs once per segment
+      // and costs what it takes to fetch it.
+      const int steps = whole ? 2 : 4;
+      const int step_columns = whole ? 64 : 32;
+      uint8_t *stage = smem_raw + T::kPAt + group * kPTileBytes + quarter * 4096;
+      const int valid = now_rows.rows - 32 * quarter;  // rows of the warp
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        const int column = 128 * group + 64 * h;
-        float o[64];
-        if (active) tmem_ld64(tmem + lanes + uint32_t(column), o);
-        if (h == 1) {
+      for (int h = 0; h < steps; ++h) {
+        const int column = 128 * group + step_columns * h;
+        uint8_t *line;  // this row's 128 bytes
+        if (whole) {
+          line = reinterpret_cast<uint8_t *>(p.out + now_rows.at * T::kHeadDim +
+                                             now_rows.part * kPartDims + column);
+        } else {
+          line = reinterpret_cast<uint8_t *>(piece + row * kPartDims + column);
+        }
+        if (active) {
+#pragma unroll 1
+          for (int c = 0; c < 8; c += 2) {  // two 16-byte chunks of the line
+            float o[16];
+            uint4 w[2];
+            if (whole) {
+              tmem_ld<16>(tmem + lanes + uint32_t(column + 8 * c), o);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                w[i] = make_uint4(bf16_pair(o[8 * i] * inv, o[8 * i + 1] * inv),
+                                  bf16_pair(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                                  bf16_pair(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
+                                  bf16_pair(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+              }
+            } else {
+              tmem_ld8(tmem + lanes + uint32_t(column + 4 * c), w);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if constexpr (T::kPShared) {
+                *reinterpret_cast<uint4 *>(stage + lane * 128 + (((c + i) ^ (lane & 7)) << 4)) = w[i];
+              } else if (writes) {
+                reinterpret_cast<uint4 *>(line)[c + i] = w[i];
+              }
+            }
+          }
+        }
+        if (h + 1 == steps) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_o_free);
         }
-        if (!active) continue;
-        uint8_t *stage = smem_raw + T::kPAt + group * kPTileBytes + quarter * 4096;
-        const int valid = now_rows.rows - 32 * quarter;  // rows of the warp
-        if (whole) {
-          uint4 w[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint32_t x[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const __nv_bfloat162 b2 =
-                  __floats2bfloat162_rn(o[8 * i + 2 * j] * inv, o[8 * i + 2 * j + 1] * inv);
-              x[j] = *reinterpret_cast<const uint32_t *>(&b2);
-            }
-            w[i] = make_uint4(x[0], x[1], x[2], x[3]);
+        if (T::kPShared && active) {
+          __syncwarp();
+#pragma unroll 2
+          for (int i = 0; i < 8; ++i) {  // eight lanes store a row's line
+            const int r = 4 * i + (lane >> 3);
+            const int c = lane & 7;
+            const uint4 v = *reinterpret_cast<const uint4 *>(stage + r * 128 + ((c ^ (r & 7)) << 4));
+            uint8_t *to = reinterpret_cast<uint8_t *>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(line), r));
+            if (r < valid) reinterpret_cast<uint4 *>(to)[c] = v;
           }
-          __nv_bfloat16 *dst = p.out + now_rows.part * kPartDims + column;
-          if constexpr (T::kPShared) {
-            store_rows_staged(stage, w, lane, valid, [&](int r, int c) {
-              const int64_t at = __shfl_sync(0xffffffffu, now_rows.at, r);
-              return reinterpret_cast<uint4 *>(dst + at * T::kHeadDim) + c;
-            });
-          } else if (writes) {
-            uint4 *to = reinterpret_cast<uint4 *>(dst + now_rows.at * T::kHeadDim);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) to[i] = w[i];
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint4 w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float *x = o + 32 * q + 4 * i;
-              w[i] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
-                                __float_as_uint(x[3]));
-            }
-            float *dst = piece + 32 * quarter * kPartDims + column + 32 * q;
-            if constexpr (T::kPShared) {
-              store_rows_staged(stage, w, lane, valid, [&](int r, int c) {
-                return reinterpret_cast<uint4 *>(dst + r * kPartDims) + c;
-              });
-            } else if (writes) {
-              uint4 *to = reinterpret_cast<uint4 *>(dst + lane * kPartDims);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) to[i] = w[i];
-            }
-          }
+          __syncwarp();
         }
       }
       if (writes && group == 0) {
@@ -1445,6 +1453,7 @@ cudaError_t launch_chunk(const ChunkAttentionArgs &a, int ctas, cudaStream_t str
   p.box = box_tokens(c.page_size);
   p.page_div = FastDiv::by(uint32_t(c.page_size));
   p.slot_div = FastDiv::by(uint32_t(c.max_pages_per_seq));
+  p.run_div = FastDiv::by(uint32_t(p.tiles_per_run));
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   p.rows_cap = partial_rows(p.group, a.runs.max_row_count);
   p.meta = static_cast<int4 *>(a.workspace);
