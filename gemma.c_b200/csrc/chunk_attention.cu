@@ -141,6 +141,7 @@ struct ChunkParams {
   int32_t tile_tokens;   // 128 / group
   int32_t tiles_per_run; // query tiles of the longest run
   int32_t q_box;         // tokens of a query box
+  int32_t q_slots;       // K slots that a segment's Q takes
   int32_t window;
   int32_t sinks;
   int32_t box;           // tokens per TMA box; 0: rows are copied one by one
@@ -375,21 +376,6 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
 }
-// Eight 32-bit columns of this thread's lane.
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint4 (&w)[2]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-      : "=r"(w[0].x), "=r"(w[0].y), "=r"(w[0].z), "=r"(w[0].w), "=r"(w[1].x), "=r"(w[1].y),
-        "=r"(w[1].z), "=r"(w[1].w)
-      : "r"(taddr)
-      : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    asm volatile("" : "+r"(w[i].x), "+r"(w[i].y), "+r"(w[i].z), "+r"(w[i].w));  // not before the wait
-  }
-}
-
 // 128 rows x 32 bytes of a swizzled block to eight columns of tensor memory.
 __device__ __forceinline__ void tmem_copy_warp(uint32_t d_tmem, uint32_t lo, uint32_t hi, bool leader) {
   asm volatile(
@@ -476,6 +462,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   // everything up to here is this kernel's own; the runs, the rows and the cache
   // may be what the kernel before it writes
   pdl_wait_for_predecessor();
+  // the combine's blocks may take their places; they wait for this kernel's end
+  pdl_release_successor();
 
   // ---- this CTA's share: the costs of all (run, query tile) pairs, summed
   const int pairs = p.runs.run_count * p.tiles_per_run;
@@ -626,29 +614,28 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           meta.y = s.run_index;
           meta.z = s.query_tile;
         }
-        // Q: 64-dim blocks of box_rows rows, two to a slot (rows behind the segment's are
-        // other runs', or zeros behind the last: nobody looks at what comes of them)
+        // Q: 64-dim blocks, two to a slot, or all four where the box has at most 64 rows
+        // (rows behind the segment's are other runs', or zeros behind the last, or what
+        // the slot held: nobody looks at what comes of them)
         const int token = s.run.start + s.token0;
         const uint32_t block_bytes = uint32_t(p.q_box * p.group) * 128u;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          ok = ok && __all_sync(0xffffffffu, wait(bar_k_done + 8u * at.slot, at.phase ^ 1u));
+        for (int h = 0; h < p.q_slots && ok; ++h) {
+          ok = __all_sync(0xffffffffu, wait(bar_k_done + 8u * at.slot, at.phase ^ 1u));
           if (!ok) break;
-          if (lane == 0) {
-            const uint32_t bar = bar_k_full + 8u * at.slot;
-            mbar_arrive_expect_tx(bar, 2u * block_bytes);
-            for (int b = 0; b < 2; ++b) {
-              tma_load_block(ring + at.slot * kSlotBytes + uint32_t(b) * kQBlockBytes, &map_q,
-                             (2 * h + b) * 64, head * p.group, token, bar);
-            }
-          }
+          const uint32_t blocks = 4u / uint32_t(p.q_slots);
+          if (lane == 0) mbar_arrive_expect_tx(bar_k_full + 8u * at.slot, blocks * block_bytes);
           __syncwarp();
+          if (uint32_t(lane) < blocks) {
+            tma_load_block(ring + at.slot * kSlotBytes + uint32_t(lane) * (kSlotBytes / blocks), &map_q,
+                           (int(blocks) * h + lane) * 64, head * p.group, token,
+                           bar_k_full + 8u * at.slot);
+          }
           at.advance(ring_slots);
         }
         if constexpr (T::kKSlots == 2) {
-          // its place is free when the last segment's Q K^T is complete
+          // its place is free when the last segment's rows are out (they go through it)
           if (ok && segments > 1) {
-            ok = __all_sync(0xffffffffu, wait(bar_q_free, uint32_t(segments - 2) & 1u));
+            ok = __all_sync(0xffffffffu, wait(bar_o_free, uint32_t(segments - 2) & 1u));
           }
           if (ok && lane == 0) {
             mbar_arrive_expect_tx(bar_q_hi_full, 4u * block_bytes);
@@ -919,16 +906,18 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       const int first = n;
       // Q into tensor memory, when the last segment's Q K^T no longer reads what is there
       if (segments > 0) ok = warp_wait(bar_q_free, uint32_t(segments - 1) & 1u);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        ok = ok && warp_wait(bar_k_full + 8u * k_at.slot, k_at.phase);
+      for (int h = 0; h < p.q_slots && ok; ++h) {
+        ok = warp_wait(bar_k_full + 8u * k_at.slot, k_at.phase);
         if (!ok) break;
         tc_fence_after();
+        // (with one slot a copy's 128 rows reach into what lies behind the block's 64:
+        // rows without a query)
+        const int blocks = 4 / p.q_slots;
         const uint32_t q = ((s_q_hi + T::kKAt + k_at.slot * kSlotBytes) >> 4) | kLoK;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          tmem_copy_warp(tmem + kTmemQ + 64u * uint32_t(h) + 8u * uint32_t(i),
-                         q + uint32_t(i >> 2) * (kQBlockBytes >> 4) + uint32_t(i & 3) * 2u, kHiQ, leader);
+        for (int i = 0; i < 4 * blocks; ++i) {
+          tmem_copy_warp(tmem + kTmemQ + 8u * uint32_t(4 * blocks * h + i),
+                         q + uint32_t(i >> 2) * uint32_t((kSlotBytes >> 4) / blocks) + uint32_t(i & 3) * 2u,
+                         kHiQ, leader);
         }
         umma_commit_warp(bar_k_done + 8u * k_at.slot, leader);
         k_at.advance(T::kKRing);
@@ -1205,13 +1194,14 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       float *piece = p.partials + (int64_t(blockIdx.x) * 2 + (whole ? 0 : now_rows.piece)) *
                                       (int64_t(p.rows_cap) * (kPartDims + 2));
       // This group's 128 columns of O, 32 lines of 128 bytes per warp at a time: 64
-      // columns as bf16, or 32 as fp32. head_dim 256: through the group's weight buffer
-      // (its P V is complete; each warp has its 4 KB of it), so that a store covers whole
-      // lines, not 32 rows of 16 bytes. Rolled loops: this code runs once per segment
-      // and costs what it takes to fetch it.
+      // columns as bf16, or 32 as fp32, through 4 KB of shared memory per warp so that a
+      // store covers whole lines, not 32 rows of 16 bytes: the weights' buffers (P V is
+      // complete), or for head_dim 512 the upper half of Q (so is Q K^T). Rolled loops:
+      // this code runs once per segment and costs what it takes to fetch it.
       const int steps = whole ? 2 : 4;
       const int step_columns = whole ? 64 : 32;
-      uint8_t *stage = smem_raw + T::kPAt + group * kPTileBytes + quarter * 4096;
+      static_assert(T::kPShared || T::kQHiBytes >= kSoftmaxWarps * 4096, "place for the rows");
+      uint8_t *stage = smem_raw + (T::kPShared ? T::kPAt : 0) + (4 * group + quarter) * 4096;
       const int valid = now_rows.rows - 32 * quarter;  // rows of the warp
 #pragma unroll 1
       for (int h = 0; h < steps; ++h) {
@@ -1225,37 +1215,39 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         }
         if (active) {
 #pragma unroll 1
-          for (int c = 0; c < 8; c += 2) {  // two 16-byte chunks of the line
-            float o[16];
-            uint4 w[2];
+          for (int c = 0; c < 8; c += 4) {  // four 16-byte chunks of the line
+            uint4 w[4];
             if (whole) {
-              tmem_ld<16>(tmem + lanes + uint32_t(column + 8 * c), o);
+              float o[32];
+              tmem_ld<32>(tmem + lanes + uint32_t(column + 8 * c), o);
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
+              for (int i = 0; i < 4; ++i) {
                 w[i] = make_uint4(bf16_pair(o[8 * i] * inv, o[8 * i + 1] * inv),
                                   bf16_pair(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
                                   bf16_pair(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
                                   bf16_pair(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
               }
             } else {
-              tmem_ld8(tmem + lanes + uint32_t(column + 4 * c), w);
+              float o[16];
+              tmem_ld<16>(tmem + lanes + uint32_t(column + 4 * c), o);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                w[i] = make_uint4(__float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]),
+                                  __float_as_uint(o[4 * i + 2]), __float_as_uint(o[4 * i + 3]));
+              }
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              if constexpr (T::kPShared) {
-                *reinterpret_cast<uint4 *>(stage + lane * 128 + (((c + i) ^ (lane & 7)) << 4)) = w[i];
-              } else if (writes) {
-                reinterpret_cast<uint4 *>(line)[c + i] = w[i];
-              }
+            for (int i = 0; i < 4; ++i) {
+              *reinterpret_cast<uint4 *>(stage + lane * 128 + (((c + i) ^ (lane & 7)) << 4)) = w[i];
             }
           }
         }
-        if (h + 1 == steps) {
+        if (T::kPShared && h + 1 == steps) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_o_free);
         }
-        if (T::kPShared && active) {
+        if (active) {
           __syncwarp();
 #pragma unroll 2
           for (int i = 0; i < 8; ++i) {  // eight lanes store a row's line
@@ -1268,6 +1260,12 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           }
           __syncwarp();
         }
+      }
+      if constexpr (!T::kPShared) {  // the next upper half of Q comes where the rows went through
+        fence_proxy_async_shared();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_o_free);
       }
       if (writes && group == 0) {
         if (!whole) {
@@ -1296,7 +1294,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
 // and query tile); the pieces behind it are the first of CTA i + 1, i + 2, ... up to
 // the one that has the item's end (meta.w 1; 2: goes on). A warp per row:
 //   M = max m, out = sum 2^(m - M) acc / sum 2^(m - M) l, lse = (M + log2 sum) ln 2
-constexpr int kCombineWarps = 8;
+constexpr int kCombineWarps = 4;
 __global__ __launch_bounds__(kCombineWarps * 32) void chunk_combine_kernel(ChunkParams p, int head_dim) {
   pdl_wait_for_predecessor();
   const int4 meta = p.meta[blockIdx.x];
@@ -1322,7 +1320,8 @@ __global__ __launch_bounds__(kCombineWarps * 32) void chunk_combine_kernel(Chunk
   const int64_t slot_floats = int64_t(p.rows_cap) * (kPartDims + 2);
   const float *first = p.partials + (int64_t(blockIdx.x) * 2 + 1) * slot_floats;
   const float *rest = p.partials + (int64_t(blockIdx.x) + 1) * 2 * slot_floats;
-  for (int row = int(blockIdx.y) * kCombineWarps + warp; row < rows; row += int(gridDim.y) * kCombineWarps) {
+  const int row = int(blockIdx.y) * kCombineWarps + warp;
+  if (row < rows) {
     auto piece = [&](int i) { return i == 0 ? first : rest + int64_t(i - 1) * 2 * slot_floats; };
     float m = -INFINITY;
     for (int i = lane; i <= pieces; i += 32) m = fmaxf(m, piece(i)[p.rows_cap * kPartDims + row]);
@@ -1460,6 +1459,7 @@ cudaError_t launch_chunk(const ChunkAttentionArgs &a, int ctas, cudaStream_t str
   p.partials = reinterpret_cast<float *>(p.meta + ctas);
   p.status = a.status;
   p.q_box = std::min(p.tile_tokens, a.runs.max_row_count);
+  p.q_slots = p.q_box * p.group <= kRows / 2 ? 1 : 2;
   CUtensorMap map_q = {}, map_k = {}, map_v = {}, map_k_rows = {}, map_v_rows = {};
   if (!make_q_map(&map_q, a.q, a.runs.rows, a.q_heads, c.head_dim, p.group, p.q_box)) {
     return cudaErrorInvalidValue;
@@ -1480,7 +1480,7 @@ cudaError_t launch_chunk(const ChunkAttentionArgs &a, int ctas, cudaStream_t str
                   size_t(kChunkSmemBytes<T>), stream, p, map_k, map_v, map_k_rows, map_v_rows,
                   map_q);
   if (st != cudaSuccess) return st;
-  const unsigned row_blocks = unsigned(std::min(4, div_up(p.rows_cap, kCombineWarps)));
+  const unsigned row_blocks = unsigned(div_up(p.rows_cap, kCombineWarps));
   return launch_pdl(chunk_combine_kernel, dim3(unsigned(ctas), row_blocks), dim3(kCombineWarps * 32), 0,
                     stream, p, int(c.head_dim));
 }
