@@ -86,6 +86,7 @@ constexpr float kRescaleSlack = 8.0f;         // log2 units
 constexpr int kInfos = 8;
 constexpr int kSegments = 8;
 constexpr long long kTileWaitClocks = 1ll << 26;
+constexpr uint32_t kWaitPolls = 1u << 20;     // tens of milliseconds at least; a tile takes microseconds
 // What starting an item costs next to a key tile (loading Q, reading O back), and
 // the least a CTA is given, both in key tiles: they shape the cut only.
 constexpr int kItemCost = 3;
@@ -144,6 +145,7 @@ struct ChunkParams {
   int32_t q_slots;       // K slots that a segment's Q takes
   int32_t window;
   int32_t sinks;
+  int32_t table_end;     // first position past a linear cache's table
   int32_t box;           // tokens per TMA box; 0: rows are copied one by one
   FastDiv page_div;      // by page_size
   FastDiv slot_div;      // by max_pages_per_seq
@@ -166,7 +168,7 @@ __device__ __forceinline__ KeyTiles key_tiles(const ChunkParams &p, int first, i
   KeyTiles k = {};
   const int lo = p.window > 0 ? max(0, t0 - p.window + 1) : 0;
   const int sink_end = min(p.sinks, lo);
-  const int c_lim = p.k_rows != nullptr ? min(first, t1 + 1) : t1 + 1;
+  const int c_lim = min(p.k_rows != nullptr ? min(first, t1 + 1) : t1 + 1, p.table_end);
   k.ca = div_up(min(sink_end, c_lim), kKeys);
   if (c_lim > lo) {
     k.cb0 = lo / kKeys;
@@ -177,6 +179,8 @@ __device__ __forceinline__ KeyTiles key_tiles(const ChunkParams &p, int first, i
     k.ob0 = (max(lo, first) - first) / kKeys;
     k.ob1 = (t1 - first) / kKeys + 1;
     k.oa = sink_end > first ? min(div_up(sink_end - first, kKeys), k.ob0) : 0;
+  } else if (k.ca == 0 && k.cb1 == 0) {
+    k.cb1 = 1;  // no key at all: a tile that nobody sees gives the rows their zeros
   }
   return k;
 }
@@ -198,7 +202,7 @@ struct Segment {
 // Walks the items of a CTA's share (the two loader warps do, each by itself). The
 // lanes hold 32 runs at a time.
 struct Walk {
-  long long left;
+  int left;
   int hp, run, tile, offset;
 
   __device__ __forceinline__ bool next(const ChunkParams &p, Segment &s, ChunkRun &mine, int &first_run) {
@@ -232,7 +236,7 @@ struct Walk {
       s.run_index = run;
       s.query_tile = tile;
       const int cost = s.total + kItemCost;
-      const int take = int(min((long long)(cost - offset), left));
+      const int take = min(cost - offset, left);
       s.begin = max(0, offset - kItemCost);
       s.end = max(0, offset + take - kItemCost);
       left -= take;
@@ -274,6 +278,7 @@ struct SmallState {
   uint64_t p_full[2][2];      // half of its weights written (and O rescaled where needed)
   uint64_t m_full[2][4];      // row_ref[b] of 32 rows written
   uint64_t l_full[2][4];      // row_sum of 32 rows written by the group
+  uint64_t v_raw;             // a V tile that still has rows to be cleared has landed
   uint64_t s_free[2];         // kPShared: the scores in S[b] have been read
   uint64_t q_hi_full;         // head_dim 512: the upper half of the segment's Q has landed
   uint64_t q_free;            // the segment's last Q K^T is complete
@@ -284,8 +289,7 @@ struct SmallState {
   SegmentInfo segment[kSegments];
   float row_ref[2][kRows];
   float row_sum[2][kRows];
-  long long scan[kThreads / 32];
-  long long total;
+  int scan[kThreads / 32];
   Walk start;
   uint32_t tmem_base;
   int abort;
@@ -394,6 +398,13 @@ __device__ __forceinline__ void tma_load_block(uint32_t dst, const CUtensorMap *
       : "memory");
 }
 
+__device__ __noinline__ bool wait_slowly(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+  for (uint32_t left = kWaitPolls; !mbar_try_wait(bar, parity); --left) {
+    if (left == 0 || ((left & 31u) == 0 && *abort_flag != 0)) return false;
+  }
+  return true;
+}
+
 template <class T>
 __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap map_k,
@@ -422,6 +433,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   const uint32_t bar_l_full = smem_u32(&small.l_full[0][0]);  // + 32 group + 8 warp quarter
   const uint32_t bar_s_free = smem_u32(&small.s_free[0]);  // + 8 b
   const uint32_t bar_q_hi_full = smem_u32(&small.q_hi_full);
+  const uint32_t bar_v_raw = smem_u32(&small.v_raw);
   const uint32_t bar_q_free = smem_u32(&small.q_free);
   const uint32_t bar_o_full = smem_u32(&small.o_full);
   const uint32_t bar_o_free = smem_u32(&small.o_free);
@@ -445,6 +457,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     mbar_init(bar_s_free, 4);
     mbar_init(bar_s_free + 8u, 4);
     mbar_init(bar_q_hi_full, 1);
+    mbar_init(bar_v_raw, 1);
     mbar_init(bar_q_free, 1);
     mbar_init(bar_o_full, 1);
     mbar_init(bar_o_free, kSoftmaxWarps);
@@ -477,56 +490,51 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     const int t1 = t0 + min(p.tile_tokens, run.count - token0) - 1;
     return key_tiles(p, run.first, t0, t1).count() + kItemCost;
   };
-  long long mine = 0;
+  int mine = 0;
   for (int i = 0; i < per_thread; ++i) {
     const int pair = tid * per_thread + i;
     if (pair < pairs) mine += pair_cost(pair);
   }
-  long long before = mine;  // inclusive scan over the warp
-#pragma unroll
+  int before = mine;  // inclusive scan over the warp
+#pragma unroll 1
   for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, before, o);
+    const int up = __shfl_up_sync(0xffffffffu, before, o);
     if (lane >= o) before += up;
   }
   if (lane == 31) small.scan[warp] = before;
   __syncthreads();
-  long long warps_before = 0, per_head = 0;
+  int warps_before = 0, per_head = 0;
+#pragma unroll 1
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) warps_before += small.scan[w];
     per_head += small.scan[w];
   }
   before += warps_before - mine;  // costs before this thread's first pair
-  // an even cut; 32-bit divisions where they do (nearly always)
-  const long long total = per_head * heads * T::kParts;
-  const long long most = min((long long)gridDim.x, (long long)kMinShare * gridDim.x > total
-                                                       ? (long long)(uint32_t(total) / kMinShare)
-                                                       : (long long)gridDim.x);
-  const int ctas = int(max(1ll, most));
-  const long long share = total < (1ll << 31) ? (long long)(uint32_t(total) / uint32_t(ctas)) : total / ctas;
-  const int extra = int(total - share * ctas);  // the first CTAs have one more
-  const int cta = int(blockIdx.x);
-  const long long c0 = cta < ctas ? share * cta + min(cta, extra) : 0;
-  const long long c1 = cta < ctas ? c0 + share + (cta < extra ? 1 : 0) : 0;
+  // an even cut (the host has seen to it that all of this fits 32 bits)
+  const uint32_t total = uint32_t(per_head) * uint32_t(heads * T::kParts);
+  const uint32_t ctas = max(1u, min(gridDim.x, total / kMinShare));
+  const uint32_t share = total / ctas;
+  const uint32_t extra = total - share * ctas;  // the first CTAs have one more
+  const uint32_t cta = blockIdx.x;
+  const int c0 = cta < ctas ? int(share * cta + min(cta, extra)) : 0;
+  const int c1 = cta < ctas ? c0 + int(share + (cta < extra ? 1 : 0)) : 0;
   if (tid == 0) {
     small.start.left = 0;
     small.start.hp = small.start.run = small.start.tile = small.start.offset = 0;
   }
   __syncthreads();
   if (c1 > c0) {
-    const int hp = total < (1ll << 31) ? int(uint32_t(c0) / uint32_t(per_head)) : int(c0 / per_head);
-    long long rem = c0 - (long long)hp * per_head;
+    const int hp = int(uint32_t(c0) / uint32_t(per_head));
+    int rem = c0 - hp * per_head;
     if (rem >= before && rem < before + mine) {
       rem -= before;
       int pair = tid * per_thread;
-      for (int cost = pair_cost(pair); rem >= cost; cost = pair_cost(pair)) {
-        rem -= cost;
-        ++pair;
-      }
+      for (int cost; rem >= (cost = pair_cost(pair)); ++pair) rem -= cost;
       small.start.left = c1 - c0;
       small.start.hp = hp;
       small.start.run = p.run_div.quotient(pair);
       small.start.tile = pair - small.start.run * p.tiles_per_run;
-      small.start.offset = int(rem);
+      small.start.offset = rem;
     }
   }
   tc_fence_before();
@@ -536,22 +544,20 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   volatile int *abort_flag = &small.abort;
   Walk walk = small.start;
 
-  // Bounded wait that also gives up when another role has; false = give up.
+  // Bounded wait that also gives up when another role has; false = give up (the role
+  // says so at the end). What is not ready at once is waited for out of line: there are
+  // dozens of waits, and the roles share one instruction cache.
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
-    if (mbar_try_wait(bar, parity)) return true;
-    const long long start = clock64();
-    for (uint32_t poll = 0;; ++poll) {
-      if (mbar_try_wait(bar, parity)) return true;
-      if ((poll & 31u) == 31u) {
-        if (*abort_flag != 0) return false;
-        if (clock64() - start > kTileWaitClocks) {
-          set_status(p.status, B200KV_STATUS_WAIT_TIMEOUT);
-          *abort_flag = 1;
-          return false;
-        }
-      }
-    }
+    return mbar_try_wait(bar, parity) || wait_slowly(bar, parity, &small.abort);
   };
+  // The same in line, for where a call would have to save a tile's scores.
+  auto wait_here = [&](uint32_t bar, uint32_t parity) -> bool {
+    for (uint32_t left = kWaitPolls; !mbar_try_wait(bar, parity); --left) {
+      if (left == 0) return false;
+    }
+    return true;
+  };
+  bool failed = false;
   // A ring's slots are filled and freed in order: a role keeps the slot of its next
   // fill and the parity of that slot's use. V of key tile n is fill n of its ring.
   struct Cursor {
@@ -583,6 +589,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     const uint32_t bar_full = is_v ? bar_v_full : bar_k_full;
     const uint32_t bar_done = is_v ? bar_v_done : bar_k_done;
     Cursor at;
+    uint32_t raw_phase = 0;  // of v_raw
     int n = 0, segments = 0;
     int4 meta = make_int4(-1, 0, 0, 0);
     ChunkRun mine;
@@ -669,7 +676,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         const int count = min(stop - k, s.end - j);
         j += count;
         const int origin = own ? s.run.first : 0;
-        const int limit = !own && p.k_rows != nullptr ? min(s.run.first, s.t1 + 1) : s.t1 + 1;
+        const int limit = own ? s.t1 + 1
+                              : min(p.k_rows != nullptr ? min(s.run.first, s.t1 + 1) : s.t1 + 1, p.table_end);
         // keys of the tile that some row sees, pages aside
         auto seen = [&](int base) -> unsigned long long {
           unsigned long long live = low_bits(limit - base);
@@ -688,11 +696,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           int logical = p.page_div.quotient(position);
           raw_offset = (position - logical * p.cfg.page_size) >> 3;
           const int slots = p.cfg.max_pages_per_seq;
-          if (p.cfg.window_size == 0) {
-            if (logical >= slots) return;
-          } else {
-            logical -= p.slot_div.quotient(logical) * slots;
-          }
+          if (p.cfg.window_size > 0) logical -= p.slot_div.quotient(logical) * slots;
           raw = __ldg(p.page_table + int64_t(s.run.batch) * slots + logical);
         };
         int group_of_box = -1;
@@ -754,7 +758,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
                                 (p.window > 0 && base <= s.t1 - p.window && base + kKeys > p.sinks);
               small.info[n % kInfos] = {live, base, edge ? 1 : 0};
             }
-            const uint32_t bar = bar_full + 8u * at.slot;
+            const bool clear = is_v && live != ~0ull;
+            const uint32_t bar = clear && p.box > 0 ? bar_v_raw : bar_full + 8u * at.slot;
             const uint32_t dst = ring + at.slot * kSlotBytes;
             if (p.box == 0) {
               int64_t row_at[2];  // element offset of rows lane, lane + 32
@@ -778,9 +783,11 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
                 }
               }
               asm volatile("cp.async.wait_all;" ::: "memory");
-              fence_proxy_async_shared();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(bar);
+              if (!clear) {
+                fence_proxy_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar);
+              }
             } else if (own) {
               if (lane == 0) mbar_arrive_expect_tx(bar, kSlotBytes);
               __syncwarp();
@@ -799,6 +806,31 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
                                   head, bar);
               }
             }
+            if (clear) {
+              if (p.box > 0) {
+                ok = __all_sync(0xffffffffu, wait(bar_v_raw, raw_phase));
+                if (!ok) {
+                  mbar_wait_bounded(bar_v_raw, raw_phase, kTileWaitClocks);
+                  break;
+                }
+                raw_phase ^= 1u;
+              }
+              uint8_t *row0 = smem_raw + T::kVAt + at.slot * kSlotBytes + (lane >> 3) * kBlockBytes +
+                              (lane & 7) * 16;
+#pragma unroll 1
+              for (int g = 0; g < 8; ++g) {  // groups of eight rows
+                const uint32_t alive = uint32_t(live >> (8 * g));
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                  if (((alive >> r) & 1u) == 0) {
+                    *reinterpret_cast<uint4 *>(row0 + g * kGroupBytes + r * 128) = make_uint4(0, 0, 0, 0);
+                  }
+                }
+              }
+              fence_proxy_async_shared();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar_v_full + 8u * at.slot);
+            }
             at.advance(ring_slots);
           }
           if (!ok) break;
@@ -806,6 +838,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       }
     }
     if (ok) tell_segment(0);
+    failed = !ok;
     if (!is_v && lane == 0) p.meta[blockIdx.x] = meta;
     if (!ok || *abort_flag != 0) {
       // nobody may be waiting for the last loads any more: see them land before the
@@ -851,7 +884,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         tc_fence_after();
         const uint32_t k = ((s_q_hi + T::kKAt + k_at.slot * kSlotBytes) >> 4) | kLoK;
         const uint32_t q_hi = (s_q_hi >> 4) | kLoK;
-#pragma unroll
+#pragma unroll 4
         for (int i = 0; i < 16; ++i) {
           const uint32_t at = uint32_t(i >> 2) * (kBlockBytes >> 4) + uint32_t(i & 3) * 2u;
           if (f == 0) {
@@ -956,6 +989,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       }
       if (ok) umma_commit_warp(bar_o_full, leader);
     }
+    failed = !ok;
   } else {
     // ------------------------------------------------------------ softmax
     const int group = warp >> 2;
@@ -1007,29 +1041,11 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       const int n1 = n0 + now_rows.tiles;
       float l_run = 0.0f;
       float ref = -INFINITY;  // what l_run's weights are scaled by
-      // V rows that no row of the tile sees become zeros
-      auto clear_v = [&](int n, unsigned long long live) -> bool {
-        if (!warp_wait(bar_v_full + 8u * v_slot(n), v_parity(n))) return false;
-        uint8_t *v = smem_raw + T::kVAt + v_slot(n) * kSlotBytes + (lane >> 3) * kBlockBytes +
-                     (lane & 7) * 16;
-        // the rows quarter, quarter + 4, ...: bits 0, 4, 8, ... of
-        unsigned long long dead = (~live >> quarter) & 0x1111111111111111ull;
-        while (dead != 0) {
-          const int r = __ffsll((long long)dead) - 1 + quarter;
-          dead &= dead - 1;
-          *reinterpret_cast<uint4 *>(v + (r >> 3) * kGroupBytes + (r & 7) * 128) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_shared();
-        return true;
-      };
       if (!active) {
         // no row of this warp is a query: it keeps the barriers' phases, which go by the
-        // tile's number, and clears its share of V
+        // tile's number
         for (int n = n0 + ((n0 ^ group) & 1); n < n1; n += 2) {
           ok = warp_wait(bar_s_full + 8u * uint32_t(group), uint32_t(n >> 1) & 1u);
-          if (!ok) break;
-          const unsigned long long live = small.info[n % kInfos].live;
-          if (live != ~0ull) ok = clear_v(n, live);
           if (!ok) break;
           if (T::kPShared && n >= 2) {  // not a phase ahead of the other warps' weights
             ok = warp_wait(bar_v_done + 8u * v_slot(n - 2), v_parity(n - 2));
@@ -1069,8 +1085,6 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
               if (((lo >> c) & 1u) == 0) sc[c] = -INFINITY;
               if (((hi >> c) & 1u) == 0) sc[c + 32] = -INFINITY;
             }
-            if (info.live != ~0ull) ok = clear_v(n, info.live);
-            if (!ok) break;
           }
           float mx[4] = {sc[0], sc[1], sc[2], sc[3]};
 #pragma unroll
@@ -1085,8 +1099,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           // the reference so far: the other group's tile before this one
           float last = -INFINITY;
           if (n > n0) {
-            ok = warp_wait(bar_m_full + 32u * uint32_t(group ^ 1) + 8u * uint32_t(quarter),
-                           uint32_t((n - 1) >> 1) & 1u);
+            ok = __all_sync(0xffffffffu, wait_here(bar_m_full + 32u * uint32_t(group ^ 1) +
+                                                       8u * uint32_t(quarter),
+                                                   uint32_t((n - 1) >> 1) & 1u));
             if (!ok) break;
             last = small.row_ref[group ^ 1][row];
           }
@@ -1102,22 +1117,23 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
             ref = now;
             const bool raised = last != -INFINITY && now != last;
             if (__any_sync(0xffffffffu, raised)) {
-              ok = warp_wait(bar_v_done + 8u * v_slot(n - 1), v_parity(n - 1));
+              ok = __all_sync(0xffffffffu, wait_here(bar_v_done + 8u * v_slot(n - 1), v_parity(n - 1)));
               if (!ok) break;
               tc_fence_after();
               const float factor = raised ? ex2_approx(last - now) : 1.0f;
 #pragma unroll 1
-              for (int c = 0; c < kPartDims; c += 32) {
-                float o[32];
-                tmem_ld32(tmem + lanes + uint32_t(c), o);
+              for (int c = 0; c < kPartDims; c += 16) {
+                float o[16];
+                uint32_t x[16];
+                tmem_ld<16>(tmem + lanes + uint32_t(c), o);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] *= factor;
-                tmem_st32(tmem + lanes + uint32_t(c), o);
+                for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(o[i] * factor);
+                tmem_st16(tmem + lanes + uint32_t(c), x);
               }
             }
           }
           if (T::kPShared && n >= 2) {  // the buffer's last weights have been used
-            ok = warp_wait(bar_v_done + 8u * v_slot(n - 2), v_parity(n - 2));
+            ok = __all_sync(0xffffffffu, wait_here(bar_v_done + 8u * v_slot(n - 2), v_parity(n - 2)));
             if (!ok) break;
           }
           // the weights, in packed pairs; rounded to bf16 for P V, summed unrounded
@@ -1279,6 +1295,11 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       more = next_segment(now_rows);
       ++segments;
     }
+    failed = !ok;
+  }
+  if (failed) {
+    set_status(p.status, B200KV_STATUS_WAIT_TIMEOUT);
+    *abort_flag = 1;
   }
   tc_fence_before();
   __syncthreads();
@@ -1365,6 +1386,11 @@ __global__ __launch_bounds__(kCombineWarps * 32) void chunk_combine_kernel(Chunk
   }
 }
 
+int table_end(const Gemma4KvCacheConfig &c) {
+  if (c.window_size > 0) return kMaxPosition;  // a ring has a place for every position
+  return int(std::min<int64_t>(kMaxPosition, int64_t(c.max_pages_per_seq) * c.page_size));
+}
+
 // Tokens per box: the largest power of two up to a key tile that divides the page
 // (a box then lies in one page); less than eight rows do not fill a swizzle atom.
 int box_tokens(int page_size) {
@@ -1449,6 +1475,7 @@ cudaError_t launch_chunk(const ChunkAttentionArgs &a, int ctas, cudaStream_t str
   p.tiles_per_run = div_up(std::min(a.runs.max_row_count, a.runs.rows), p.tile_tokens);
   p.window = a.window;
   p.sinks = a.sinks;
+  p.table_end = table_end(c);
   p.box = box_tokens(c.page_size);
   p.page_div = FastDiv::by(uint32_t(c.page_size));
   p.slot_div = FastDiv::by(uint32_t(c.max_pages_per_seq));
@@ -1507,11 +1534,13 @@ cudaError_t validate_chunk_attention(const ChunkAttentionArgs &a) {
       (a.sinks > 0 && a.window == 0) || !(a.softmax_scale > 0.0f)) {
     return cudaErrorInvalidValue;
   }
-  // (run, query tile) pairs that every CTA adds up
-  if (int64_t(a.runs.run_count) * div_up(a.runs.max_row_count, kRows / (a.q_heads / c.num_heads)) >
-      (1 << 24)) {
-    return cudaErrorInvalidValue;
-  }
+  // (run, query tile) pairs that every CTA adds up, and the most key tiles they can have
+  const int64_t tokens = kRows / (a.q_heads / c.num_heads);
+  const int64_t pairs = a.runs.run_count * div_up(int64_t(std::min(a.runs.max_row_count, a.runs.rows)), tokens);
+  const int64_t keys = (c.window_size > 0 ? c.window_size + tokens : table_end(c)) +
+                       (a.k_rows != nullptr ? a.runs.max_row_count : 0);
+  const double cost = double(keys / kKeys + 8) * double(pairs) * c.num_heads * (c.head_dim / kPartDims);
+  if (pairs > (1 << 24) || cost >= 2147483648.0) return cudaErrorInvalidValue;
   if (int64_t(a.workspace_bytes) < workspace_per_cta(a.q_heads / c.num_heads, a.runs.max_row_count)) {
     return cudaErrorInvalidValue;
   }
