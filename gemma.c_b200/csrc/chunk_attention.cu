@@ -150,6 +150,7 @@ struct ChunkParams {
   FastDiv page_div;      // by page_size
   FastDiv slot_div;      // by max_pages_per_seq
   FastDiv run_div;       // by tiles_per_run
+  FastDiv group_div;     // by group
   float scale_log2;
   int4 *meta;            // per CTA: see PartialMeta
   float *partials;       // [cta][2] x (acc [rows_cap][256], m [rows_cap], l [rows_cap])
@@ -190,8 +191,6 @@ struct Segment {
   ChunkRun run;
   KeyTiles keys;
   int hp;            // part * KV heads + KV head
-  int run_index;
-  int query_tile;
   int token0;        // first token of the tile within the run
   int rows;          // query rows
   int t0, t1;        // positions of the first and last row
@@ -233,8 +232,6 @@ struct Walk {
       s.keys = key_tiles(p, s.run.first, s.t0, s.t1);
       s.total = s.keys.count();
       s.hp = hp;
-      s.run_index = run;
-      s.query_tile = tile;
       const int cost = s.total + kItemCost;
       const int take = min(cost - offset, left);
       s.begin = max(0, offset - kItemCost);
@@ -618,8 +615,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         if (s.begin > 0) meta.w = s.end == s.total ? 1 : 2;
         if (s.begin == 0 && s.end < s.total) {
           meta.x = s.hp;
-          meta.y = s.run_index;
-          meta.z = s.query_tile;
+          meta.y = s.run.start + s.token0;
+          meta.z = s.rows;
         }
         // Q: 64-dim blocks, two to a slot, or all four where the box has at most 64 rows
         // (rows behind the segment's are other runs', or zeros behind the last, or what
@@ -1004,7 +1001,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     auto warp_wait = [&](uint32_t bar, uint32_t parity) -> bool {
       return __all_sync(0xffffffffu, wait(bar, parity));
     };
-    const int token = row / p.group;           // of the query tile
+    const int token = p.group_div.quotient(row);  // of the query tile
     const int head_of_group = row - token * p.group;
     // What is kept of a segment while its tiles go by.
     struct Rows {
@@ -1311,78 +1308,87 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
 }
 
 // Joins the partial rows of items that several CTAs share. Block (i, y): the item
-// whose first key tiles CTA i has (meta.x >= 0: KV head and part; meta.y, meta.z: run
-// and query tile); the pieces behind it are the first of CTA i + 1, i + 2, ... up to
-// the one that has the item's end (meta.w 1; 2: goes on). A warp per row:
+// whose first key tiles CTA i has (meta.x >= 0: KV head and part; meta.y: packed row of
+// its first token; meta.z: query rows); the pieces behind it are the first of CTA i + 1,
+// i + 2, ... up to the one that has the item's end (meta.w 1; 2: goes on). A warp per
+// row, 8 columns per lane:
 //   M = max m, out = sum 2^(m - M) acc / sum 2^(m - M) l, lse = (M + log2 sum) ln 2
+// Bound by the latency of its few dependent loads: the pieces' rows are asked for four
+// at a time, together with what weighs them.
 constexpr int kCombineWarps = 4;
 __global__ __launch_bounds__(kCombineWarps * 32) void chunk_combine_kernel(ChunkParams p, int head_dim) {
   pdl_wait_for_predecessor();
-  const int4 meta = p.meta[blockIdx.x];
-  if (meta.x < 0) return;
-  const int warp = int(threadIdx.x) >> 5;
   const int lane = int(threadIdx.x) & 31;
-  int pieces = 0;  // behind the first
-  for (int base = int(blockIdx.x) + 1;; base += 32) {
-    const int state = base + lane < int(gridDim.x) ? p.meta[base + lane].w : 1;
+  const int row = int(blockIdx.y) * kCombineWarps + (int(threadIdx.x) >> 5);
+  const int ctas = int(gridDim.x);
+  const int cta = int(blockIdx.x);
+  const int4 meta = p.meta[cta];
+  int state = cta + 1 + lane < ctas ? p.meta[cta + 1 + lane].w : 1;
+  if (meta.x < 0 || row >= meta.z) return;
+  int pieces = 1;  // the first and those behind it
+  for (int base = cta + 1;;) {
     const uint32_t end = __ballot_sync(0xffffffffu, state != 2);
     if (end != 0) {
       pieces += __ffs(int(end));
       break;
     }
     pieces += 32;
+    base += 32;
+    state = base + lane < ctas ? p.meta[base + lane].w : 1;
   }
-  pieces = min(pieces, int(gridDim.x) - 1 - int(blockIdx.x));
-  const ChunkRun run = chunk_run(p.runs, meta.y, p.cfg.batch_size);
-  const int token0 = meta.z * p.tile_tokens;
-  const int rows = min(p.tile_tokens, run.count - token0) * p.group;
-  const int head = meta.x % p.cfg.num_heads;
-  const int part = meta.x / p.cfg.num_heads;
+  pieces = min(pieces, ctas - cta);
   const int64_t slot_floats = int64_t(p.rows_cap) * (kPartDims + 2);
-  const float *first = p.partials + (int64_t(blockIdx.x) * 2 + 1) * slot_floats;
-  const float *rest = p.partials + (int64_t(blockIdx.x) + 1) * 2 * slot_floats;
-  const int row = int(blockIdx.y) * kCombineWarps + warp;
-  if (row < rows) {
-    auto piece = [&](int i) { return i == 0 ? first : rest + int64_t(i - 1) * 2 * slot_floats; };
-    float m = -INFINITY;
-    for (int i = lane; i <= pieces; i += 32) m = fmaxf(m, piece(i)[p.rows_cap * kPartDims + row]);
+  // piece 0: the second partial result of CTA i; piece k: the first of CTA i + k
+  const float *base = p.partials + int64_t(cta) * 2 * slot_floats;
+  auto piece = [&](int i) { return base + (i == 0 ? slot_floats : int64_t(i) * 2 * slot_floats); };
+  float m = -INFINITY, l = 0.0f;
+  float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i0 = 0; i0 < pieces; i0 += 4) {
+    float mi[4], li[4];
+    float4 a[4], b[4];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.0f;
-    float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int i = 0; i <= pieces; ++i) {
-      const float *from = piece(i);
-      const float mi = from[p.rows_cap * kPartDims + row];
-      const float li = from[p.rows_cap * (kPartDims + 1) + row];
-      const float4 a = *reinterpret_cast<const float4 *>(from + row * kPartDims + lane * 8);
-      const float4 b = *reinterpret_cast<const float4 *>(from + row * kPartDims + lane * 8 + 4);
-      // a piece without a visible key has accumulated zeros
-      const float f = mi == -INFINITY ? 0.0f : ex2_approx(mi - m);
-      l = fmaf(f, li, l);
-      acc[0] = fmaf(f, a.x, acc[0]);
-      acc[1] = fmaf(f, a.y, acc[1]);
-      acc[2] = fmaf(f, a.z, acc[2]);
-      acc[3] = fmaf(f, a.w, acc[3]);
-      acc[4] = fmaf(f, b.x, acc[4]);
-      acc[5] = fmaf(f, b.y, acc[5]);
-      acc[6] = fmaf(f, b.z, acc[6]);
-      acc[7] = fmaf(f, b.w, acc[7]);
+    for (int k = 0; k < 4; ++k) {
+      mi[k] = -INFINITY;
+      li[k] = 0.0f;
+      a[k] = b[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (i0 + k >= pieces) continue;
+      const float *from = piece(i0 + k);
+      mi[k] = __ldg(from + p.rows_cap * kPartDims + row);
+      li[k] = __ldg(from + p.rows_cap * (kPartDims + 1) + row);
+      a[k] = __ldg(reinterpret_cast<const float4 *>(from + row * kPartDims + lane * 8));
+      b[k] = __ldg(reinterpret_cast<const float4 *>(from + row * kPartDims + lane * 8) + 1);
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const int64_t at = (int64_t(run.start) + token0 + row / p.group) * p.q_heads + head * p.group +
-                       row % p.group;
-    uint32_t w[4];
+    const float now = fmaxf(fmaxf(fmaxf(mi[0], mi[1]), fmaxf(mi[2], mi[3])), m);
+    const float keep = m == -INFINITY ? 0.0f : ex2_approx(m - now);
+    l *= keep;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(acc[2 * j] * inv, acc[2 * j + 1] * inv);
-      w[j] = *reinterpret_cast<const uint32_t *>(&h);
+    for (int j = 0; j < 8; ++j) acc[j] *= keep;
+    m = now;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      // (a piece without a visible key has accumulated zeros)
+      const float f = mi[k] == -INFINITY ? 0.0f : ex2_approx(mi[k] - now);
+      l = fmaf(f, li[k], l);
+      acc[0] = fmaf(f, a[k].x, acc[0]);
+      acc[1] = fmaf(f, a[k].y, acc[1]);
+      acc[2] = fmaf(f, a[k].z, acc[2]);
+      acc[3] = fmaf(f, a[k].w, acc[3]);
+      acc[4] = fmaf(f, b[k].x, acc[4]);
+      acc[5] = fmaf(f, b[k].y, acc[5]);
+      acc[6] = fmaf(f, b[k].z, acc[6]);
+      acc[7] = fmaf(f, b[k].w, acc[7]);
     }
-    reinterpret_cast<uint4 *>(p.out + at * head_dim + part * kPartDims)[lane] =
-        make_uint4(w[0], w[1], w[2], w[3]);
-    if (p.lse != nullptr && part == 0 && lane == 0) {
-      p.lse[at] = l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
-    }
+  }
+  const int part = meta.x / p.cfg.num_heads;
+  const int head = meta.x - part * p.cfg.num_heads;
+  const int token = p.group_div.quotient(row);
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const int64_t at = (int64_t(meta.y) + token) * p.q_heads + head * p.group + (row - token * p.group);
+  reinterpret_cast<uint4 *>(p.out + at * head_dim + part * kPartDims)[lane] =
+      make_uint4(bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv),
+                 bf16_pair(acc[4] * inv, acc[5] * inv), bf16_pair(acc[6] * inv, acc[7] * inv));
+  if (p.lse != nullptr && part == 0 && lane == 0) {
+    p.lse[at] = l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
   }
 }
 
@@ -1479,6 +1485,7 @@ cudaError_t launch_chunk(const ChunkAttentionArgs &a, int ctas, cudaStream_t str
   p.box = box_tokens(c.page_size);
   p.page_div = FastDiv::by(uint32_t(c.page_size));
   p.slot_div = FastDiv::by(uint32_t(c.max_pages_per_seq));
+  p.group_div = FastDiv::by(uint32_t(p.group));
   p.run_div = FastDiv::by(uint32_t(p.tiles_per_run));
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   p.rows_cap = partial_rows(p.group, a.runs.max_row_count);
