@@ -878,6 +878,11 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
 #pragma unroll
       for (int f = 0; f < T::kKSlots; ++f) {
         if (!(waited && f == 0) && !warp_wait(bar_k_full + 8u * k_at.slot, k_at.phase)) return false;
+        // S[n & 1] held the weights of tile n - 2: asked for behind K, whose wait runs
+        // under that product
+        if (!T::kPShared && f == 0 && n >= 2 && !warp_wait(bar_v_done + 8u * v_last_slot, v_last_phase)) {
+          return false;
+        }
         tc_fence_after();
         const uint32_t k = ((s_q_hi + T::kKAt + k_at.slot * kSlotBytes) >> 4) | kLoK;
         const uint32_t q_hi = (s_q_hi >> 4) | kLoK;
@@ -908,7 +913,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
 #pragma unroll
       for (int i = 0; i < kKeys / 16; ++i) {
         if (i == 0 || (i == 2 && !T::kPShared)) {
-          if (!(waited && i == 0) && !warp_wait(p_bar(i / 2), p_parity())) return false;
+          if (!waited && !warp_wait(p_bar(i / 2), p_parity())) return false;
           tc_fence_after();
         }
         const uint32_t vi = v + uint32_t(i) * (2u * kGroupBytes >> 4);
@@ -967,15 +972,19 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           ready = __all_sync(0xffffffffu, ready);
         }
         if (j < tiles) {
-          // S[n & 1] held the scores (kPShared) or the weights of tile n - 2
-          if (n >= 2 && !ready) {
-            ok = T::kPShared ? warp_wait(bar_s_free + 8u * uint32_t(n & 1), s_free_parity())
-                             : warp_wait(bar_v_done + 8u * v_last_slot, v_last_phase);
+          // S[n & 1] held the scores of tile n - 2
+          if (T::kPShared && n >= 2 && !ready) {
+            ok = warp_wait(bar_s_free + 8u * uint32_t(n & 1), s_free_parity());
           }
           ok = ok && issue_qk(ready, j + 1 == tiles);
           if (!ok) break;
         }
         if (j >= T::kLag) {
+          if (!T::kPShared) {  // with P in two halves, each with its barrier
+            ready = mbar_try_wait(bar_v_full + 8u * v_at.slot, v_at.phase) &
+                    mbar_try_wait(p_bar(0), p_parity()) & mbar_try_wait(p_bar(1), p_parity());
+            ready = __all_sync(0xffffffffu, ready);
+          }
           // the segment's first P V writes O anew: the last segment's rows must be out
           if (added == first && segments > 0) {
             ok = warp_wait(bar_o_free, uint32_t(segments - 1) & 1u);
