@@ -170,12 +170,12 @@ __device__ __forceinline__ float rms_scale_of(float ss) {
 }
 
 // What a warp needs to know about pair `pr` of a token: kind 0 query heads, 1 K
-// heads, 2 V heads; its first head; whether it has a second row; where it is.
+// heads, 2 V heads; whether the pair has a second row; where its rows lie.
 struct PrepPair {
   int kind;
-  int h0;
   bool second;
   const __nv_bfloat16 *src;
+  __nv_bfloat16 *dst;
 };
 
 template <int D>
@@ -183,62 +183,15 @@ __device__ __forceinline__ PrepPair prep_pair_of(const PrefillPrepArgs &a, int64
                                                  int pq, int pk) {
   PrepPair p;
   p.kind = pr < pq ? 0 : (pr < pq + pk ? 1 : 2);
-  p.h0 = 2 * (p.kind == 0 ? pr : (p.kind == 1 ? pr - pq : pr - pq - pk));
-  p.second = p.h0 + 1 < (p.kind == 0 ? a.q_heads : a.kv_heads);
+  const int h0 = 2 * (p.kind == 0 ? pr : (p.kind == 1 ? pr - pq : pr - pq - pk));
+  p.second = h0 + 1 < (p.kind == 0 ? a.q_heads : a.kv_heads);
   p.src = p.kind == 0
-              ? a.q + (row * a.q_heads + p.h0) * D
-              : ((p.kind == 1 || a.v == nullptr ? a.k : a.v) + (row * a.kv_heads + p.h0) * D);
+              ? a.q + (row * a.q_heads + h0) * D
+              : ((p.kind == 1 || a.v == nullptr ? a.k : a.v) + (row * a.kv_heads + h0) * D);
+  p.dst = p.kind == 0 ? a.q_prepared + (row * a.q_heads + h0) * D
+                      : ((p.kind == 1 ? a.k_prepared : a.v_prepared) +
+                         (row * a.kv_heads + h0) * D);
   return p;
-}
-
-// Where a token's results go and its position (negative: nowhere). A prompt's
-// K and V rows lie in row order; a chunk's lie there or in the page of their
-// position (nullptr: not stored).
-struct PrepRow {
-  int position;
-  __nv_bfloat16 *k;
-  __nv_bfloat16 *v;
-};
-template <int D>
-__device__ __forceinline__ PrepRow prep_row_of(const PrefillPrepArgs &a, int64_t row) {
-  return {__ldg(a.token_position + row), a.k_prepared + row * a.kv_heads * D,
-          a.v_prepared + row * a.kv_heads * D};
-}
-// The run that names the row: every lane looks at its share of the runs (one
-// round of loads for up to 32 of them).
-template <int D>
-__device__ __forceinline__ PrepRow prep_row_of(const ChunkPrepArgs &a, int64_t row) {
-  const ChunkRuns &runs = a.runs;
-  const int lane = int(threadIdx.x) & 31;
-  ChunkRun run;
-  bool found = false;
-  for (int base = 0; base < runs.run_count && !found; base += 32) {
-    const ChunkRun mine = chunk_run(runs, base + lane, a.cfg.batch_size);
-    const uint32_t hit =
-        __ballot_sync(0xffffffffu, row >= mine.start && row < int64_t(mine.start) + mine.count);
-    if (hit != 0) {
-      const int from = __ffs(int(hit)) - 1;
-      run.start = __shfl_sync(0xffffffffu, mine.start, from);
-      run.count = __shfl_sync(0xffffffffu, mine.count, from);
-      run.first = __shfl_sync(0xffffffffu, mine.first, from);
-      run.batch = __shfl_sync(0xffffffffu, mine.batch, from);
-      found = true;
-    }
-  }
-  PrepRow r = {-1, nullptr, nullptr};
-  if (!found) return r;
-  r.position = run.first + int(row - run.start);
-  if (a.k_prepared != nullptr) {
-    r.k = a.k_prepared + row * a.kv_heads * D;
-    r.v = a.v_prepared + row * a.kv_heads * D;
-  } else {
-    const int64_t at = chunk_store_offset(a.cfg, a.page_table, a.layer, run, r.position);
-    if (at >= 0) {
-      r.k = a.cache_k + at;
-      r.v = a.cache_v + at;
-    }
-  }
-  return r;
 }
 
 // Up to 8 warps of two pairs each, four CTAs per SM: the kernel lives on loads in
@@ -247,10 +200,8 @@ __device__ __forceinline__ PrepRow prep_row_of(const ChunkPrepArgs &a, int64_t r
 // soon as the current one is in shared memory.
 constexpr int kPrepWarps = 8;
 
-// Args: PrefillPrepArgs (a prompt's rows) or ChunkPrepArgs (runs of rows, K and V
-// into the cache: they then cross HBM once each way instead of twice).
-template <int D, int ROT, bool kIeee, class Args>
-__global__ __launch_bounds__(kPrepWarps * 32, D == 256 ? 4 : 2) void prefill_prep_kernel(Args a) {
+template <int D, int ROT, bool kIeee>
+__global__ __launch_bounds__(kPrepWarps * 32, D == 256 ? 4 : 2) void prefill_prep_kernel(PrefillPrepArgs a) {
   constexpr int E = D / 32;          // elements per lane and row
   constexpr int kVecs = D / 8 / 32;  // 128-bit packs per lane and row
   constexpr int kPairs = ROT / 64;   // rotated (lo, hi) element pairs per lane
@@ -277,8 +228,7 @@ __global__ __launch_bounds__(kPrepWarps * 32, D == 256 ? 4 : 2) void prefill_pre
   };
   PrepPair cur = prep_pair_of<D>(a, row, warp, pq, pk);
   fetch(cur);
-  const PrepRow to = prep_row_of<D>(a, row);
-  const int position = to.position;
+  const int position = __ldg(a.token_position + row);
   if (position < 0) return;
 
   // RoPE factors of the token for this lane's rotated elements
@@ -369,27 +319,272 @@ __global__ __launch_bounds__(kPrepWarps * 32, D == 256 ? 4 : 2) void prefill_pre
     }
     __syncwarp();
     // 4. de-interleave and out
-    __nv_bfloat16 *dst = now.kind == 0 ? a.q_prepared + (row * a.q_heads + now.h0) * D
-                                       : (now.kind == 1 ? to.k : to.v);
-    if (now.kind != 0 && dst != nullptr) dst += now.h0 * D;
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
-      if constexpr (std::is_same_v<Args, ChunkPrepArgs>) {
-        if (dst == nullptr) break;
-      }
       const int pv = lane + 32 * v;
       const uint4 w0 = reinterpret_cast<const uint4 *>(mine)[pv];
       const uint4 w1 = reinterpret_cast<const uint4 *>(mine + L::kRegion)[pv];
-      reinterpret_cast<uint4 *>(dst)[pv] =
+      reinterpret_cast<uint4 *>(now.dst)[pv] =
           make_uint4(prmt(w0.x, w0.y, 0x5410u), prmt(w0.z, w0.w, 0x5410u),
                      prmt(w1.x, w1.y, 0x5410u), prmt(w1.z, w1.w, 0x5410u));
       if (now.second) {
-        reinterpret_cast<uint4 *>(dst + D)[pv] =
+        reinterpret_cast<uint4 *>(now.dst + D)[pv] =
             make_uint4(prmt(w0.x, w0.y, 0x7632u), prmt(w0.z, w0.w, 0x7632u),
                        prmt(w1.x, w1.y, 0x7632u), prmt(w1.z, w1.w, 0x7632u));
       }
     }
     __syncwarp();  // the next pair's packs overwrite the words
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The append of runs. The pairs, the words in shared memory and the bits are the
+// whole-prompt prep's; K and V go straight to the pages of their positions and so
+// cross HBM once each way. HBM would bound it (a token of 16 + 8 + 8 heads of 256:
+// 32 KB in and out), but at the prep's 420 warp instructions per pair the issue
+// slots do. So a warp takes the same pair of several consecutive rows: the pair's
+// place, its norm weights, the run and the page are looked up when they change, not
+// per row. Within a row
+//   * the two sums of squares share one butterfly: after the step of 16 the lower
+//     lanes hold the first row's sum, the upper ones the second's (the additions
+//     are those of two butterflies), and a lane takes the root of one of them;
+//   * a packed operation's halves are elements lane + 32 i and lane + 32 (i + 1)
+//     of one row, so that weights and RoPE factors are packed once.
+// The grid is one wave, a CTA per (even share of the rows, four pairs): small CTAs
+// start and end one by one. The next row's packs are asked for while a row is worked
+// on, its RoPE factors once those of the row before are used up.
+//
+// Measured, 6653 rows of nine runs, 16 + 8 + 8 heads of 256 (218 MB): 47.2 us, 4.6
+// TB/s of the 6.6 a copy reaches; the prep's form, one row per CTA of 8 warps, 59.6.
+// CTAs of 16 warps 53.8, two waves 47.5; three rows on their way in shared memory
+// (cp.async) instead of one in registers 51.5: it costs instructions, and those
+// bound it still. Nine rows: 7.9 us, a launch and four dependent loads.
+constexpr int kAppendWarps = 4;          // of a CTA, a pair each
+constexpr int kAppendCtasPerSm = 7;      // head_dim 256: 72 registers a thread
+constexpr int kAppendCtasPerSmWide = 4;  // head_dim 512: 128
+
+// What a warp keeps of the run and the page that its rows are in.
+struct AppendPlace {
+  int until = 0;       // rows below it need no new look-up
+  bool found = false;  // they belong to a run
+  ChunkRun run;
+  int page = -1;       // logical page of `at`
+  int64_t at = -1;     // its first position's elements (head 0), -1: none
+};
+
+// Position of the row (-1: no run names it). Where runs overlap the first one in
+// the list has the row, whatever the rows before it.
+__device__ __forceinline__ int append_position(const ChunkPrepArgs &a, AppendPlace &place, int row,
+                                               int lane) {
+  if (row >= place.until) {
+    const ChunkRuns &runs = a.runs;
+    place.found = false;
+    place.page = -1;
+    int until = runs.rows;
+    for (int base = 0; base < runs.run_count && !place.found; base += 32) {
+      const ChunkRun mine = chunk_run(runs, base + lane, a.cfg.batch_size);
+      const uint32_t hit =
+          __ballot_sync(0xffffffffu, row >= mine.start && row - mine.start < mine.count);
+      const int from = hit != 0 ? __ffs(int(hit)) - 1 : 32;
+      // what changes next: an earlier run's first row, or this run's end
+      int next = runs.rows;
+      if (lane < from && mine.count > 0 && mine.start > row) next = mine.start;
+      if (lane == from) next = mine.start + mine.count;
+      until = min(until, __reduce_min_sync(0xffffffffu, next));
+      if (hit != 0) {
+        place.run.start = __shfl_sync(0xffffffffu, mine.start, from);
+        place.run.count = __shfl_sync(0xffffffffu, mine.count, from);
+        place.run.first = __shfl_sync(0xffffffffu, mine.first, from);
+        place.run.batch = __shfl_sync(0xffffffffu, mine.batch, from);
+        place.found = true;
+      }
+    }
+    place.until = until;
+  }
+  return place.found ? place.run.first + (row - place.run.start) : -1;
+}
+
+// Where K and V of a position go (element offset of head 0; -1: nowhere).
+__device__ __forceinline__ int64_t append_store_offset(const ChunkPrepArgs &a, AppendPlace &place,
+                                                       int position) {
+  const Gemma4KvCacheConfig &c = a.cfg;
+  if (chunk_overwritten(c, place.run, position)) return -1;
+  const int row = c.num_heads * c.head_dim;
+  if (place.page < 0 || position - place.page * c.page_size >= c.page_size) {
+    place.page = position / c.page_size;
+    const int physical = chunk_page(c, a.page_table, place.run.batch, place.page);
+    place.at = physical < 0 ? -1 : cache_offset(c, a.layer, physical, 0, 0, 0);
+  }
+  return place.at < 0 ? -1 : place.at + int64_t(position - place.page * c.page_size) * row;
+}
+
+template <int D, int ROT, bool kIeee>
+__global__ __launch_bounds__(kAppendWarps * 32, D == 256 ? kAppendCtasPerSm : kAppendCtasPerSmWide) void chunk_append_kernel(
+    ChunkPrepArgs a) {
+  constexpr int E = D / 32;          // elements per lane and row
+  constexpr int kVecs = D / 8 / 32;  // 128-bit packs per lane and row
+  constexpr int kPairs = ROT / 64;   // rotated (lo, hi) element pairs per lane
+  using L = PairLayout<D>;
+  __shared__ __align__(16) uint32_t s_pairs[kAppendWarps][L::kWords];
+  const int warp = int(threadIdx.x) >> 5;
+  const int lane = int(threadIdx.x) & 31;
+  const int pq = (a.q_heads + 1) / 2;
+  const int pk = (a.kv_heads + 1) / 2;
+  const int pr = int(blockIdx.y) * kAppendWarps + warp;
+  if (pr >= pq + 2 * pk) return;
+  const int row0 = int(int64_t(a.runs.rows) * blockIdx.x / gridDim.x);
+  const int row1 = int(int64_t(a.runs.rows) * (blockIdx.x + 1) / gridDim.x);
+  uint32_t *mine = s_pairs[warp];
+  // this lane's words of the interleaved pair: element lane + 32 i
+  uint32_t *words = mine + ((lane & 7) >> 2) * L::kRegion + (lane >> 3) * 4 + (lane & 3);  // + 16 i
+
+  const int kind = pr < pq ? 0 : (pr < pq + pk ? 1 : 2);  // query, K, V heads
+  const int heads = kind == 0 ? a.q_heads : a.kv_heads;
+  const int h0 = 2 * (kind == 0 ? pr : (kind == 1 ? pr - pq : pr - pq - pk));
+  const bool second = h0 + 1 < heads;
+  const int64_t stride = int64_t(heads) * D;
+  const uint4 *src =
+      reinterpret_cast<const uint4 *>((kind == 0 ? a.q : (kind == 1 || a.v == nullptr ? a.k : a.v)) +
+                                      int64_t(row0) * stride + h0 * D) +
+      lane;
+  uint4 pa[kVecs], pb[kVecs];
+  auto fetch = [&]() {
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      pa[v] = __ldg(src + 32 * v);
+      pb[v] = second ? __ldg(src + D / 8 + 32 * v) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    src += stride / 8;
+  };
+  fetch();
+  // RoPE factors of a position for this lane's rotated elements
+  f32x2 rc[kPairs / 2], rs[kPairs / 2];
+  auto fetch_rope = [&](int position) {
+    if (kind == 2 || position < 0) return;
+    const float *cos_row = a.cos + int64_t(position) * (ROT / 2) + lane;
+    const float *sin_row = a.sin + int64_t(position) * (ROT / 2) + lane;
+#pragma unroll
+    for (int i = 0; i < kPairs / 2; ++i) {
+      rc[i] = pack2(__ldg(cos_row + 64 * i), __ldg(cos_row + 64 * i + 32));
+      rs[i] = pack2(__ldg(sin_row + 64 * i), __ldg(sin_row + 64 * i + 32));
+    }
+  };
+  AppendPlace place;
+  int position = append_position(a, place, row0, lane);
+  fetch_rope(position);
+  // the norm weights of this lane's elements; a V row has none (times 1)
+  f32x2 w[E / 2];
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) {
+    w[i] = pack2(1.0f, 1.0f);
+    if (kind != 2) {
+      const __nv_bfloat16 *weight = (kind == 0 ? a.q_norm_weight : a.k_norm_weight) + lane;
+      w[i] = pack2(__bfloat162float(__ldg(weight + 64 * i)),
+                   __bfloat162float(__ldg(weight + 64 * i + 32)));
+    }
+  }
+
+  for (int row = row0; row < row1; ++row) {
+    // 1. both rows, interleaved, into shared memory; the next row's are asked for
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      const int pv = lane + 32 * v;
+      reinterpret_cast<uint4 *>(mine)[pv] =
+          make_uint4(prmt(pa[v].x, pb[v].x, 0x5410u), prmt(pa[v].x, pb[v].x, 0x7632u),
+                     prmt(pa[v].y, pb[v].y, 0x5410u), prmt(pa[v].y, pb[v].y, 0x7632u));
+      reinterpret_cast<uint4 *>(mine + L::kRegion)[pv] =
+          make_uint4(prmt(pa[v].z, pb[v].z, 0x5410u), prmt(pa[v].z, pb[v].z, 0x7632u),
+                     prmt(pa[v].w, pb[v].w, 0x5410u), prmt(pa[v].w, pb[v].w, 0x7632u));
+    }
+    const int now = position;
+    __nv_bfloat16 *dst = nullptr;
+    if (now >= 0) {
+      if (kind == 0) {
+        dst = a.q_prepared + int64_t(row) * stride;
+      } else if (a.k_prepared != nullptr) {
+        dst = (kind == 1 ? a.k_prepared : a.v_prepared) + int64_t(row) * stride;
+      } else {
+        const int64_t at = append_store_offset(a, place, now);
+        if (at >= 0) dst = (kind == 1 ? a.cache_k : a.cache_v) + at;
+      }
+    }
+    if (row + 1 < row1) {
+      fetch();
+      position = append_position(a, place, row + 1, lane);
+    }
+    __syncwarp();
+    // 2. this lane's elements of both rows; sums of squares in the reference's order
+    f32x2 xa[E / 2], xb[E / 2];
+    float ss_a = 0.0f, ss_b = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const uint32_t w0 = words[32 * i], w1 = words[32 * i + 16];
+      const float a0 = __uint_as_float(w0 << 16), b0 = __uint_as_float(w0 & 0xffff0000u);
+      const float a1 = __uint_as_float(w1 << 16), b1 = __uint_as_float(w1 & 0xffff0000u);
+      ss_a = __fmaf_rn(a1, a1, __fmaf_rn(a0, a0, ss_a));
+      ss_b = __fmaf_rn(b1, b1, __fmaf_rn(b0, b0, ss_b));
+      xa[i] = pack2(a0, a1);
+      xb[i] = pack2(b0, b1);
+    }
+    const bool upper = lane >= 16;
+    float ss = upper ? ss_b : ss_a;
+    ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, upper ? ss_a : ss_b, 16));
+#pragma unroll
+    for (int offset = 8; offset > 0; offset /= 2) {
+      ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, offset));
+    }
+    const float scale = rms_scale_of<D, kIeee>(ss);
+    const float other = __shfl_xor_sync(0xffffffffu, scale, 16);
+    const float scale_a = upper ? other : scale;
+    const float scale_b = upper ? scale : other;
+    // 3. norm (+ weight, + rotation)
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      xa[i] = mul2_prep<kIeee>(mul2_prep<kIeee>(xa[i], pack2(scale_a, scale_a)), w[i]);
+      xb[i] = mul2_prep<kIeee>(mul2_prep<kIeee>(xb[i], pack2(scale_b, scale_b)), w[i]);
+    }
+    if (kind != 2) {
+#pragma unroll
+      for (int i = 0; i < kPairs / 2; ++i) {  // lo' = lo c - hi s, hi' = hi c + lo s
+        float s0, s1;
+        unpack2(rs[i], s0, s1);
+        const f32x2 minus = pack2(-s0, -s1);
+        const f32x2 lo_a = xa[i], hi_a = xa[i + kPairs / 2];
+        const f32x2 lo_b = xb[i], hi_b = xb[i + kPairs / 2];
+        xa[i] = fma2_rn(hi_a, minus, mul2_rn(lo_a, rc[i]));
+        xa[i + kPairs / 2] = fma2_rn(lo_a, rs[i], mul2_rn(hi_a, rc[i]));
+        xb[i] = fma2_rn(hi_b, minus, mul2_rn(lo_b, rc[i]));
+        xb[i + kPairs / 2] = fma2_rn(lo_b, rs[i], mul2_rn(hi_b, rc[i]));
+      }
+      if (row + 1 < row1) fetch_rope(position);
+    }
+    // rounded and packed per element of the pair; a lane's words take the results
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      float a0, a1, b0, b1;
+      unpack2(xa[i], a0, a1);
+      unpack2(xb[i], b0, b1);
+      words[32 * i] = cvt_bf16x2(a0, b0);
+      words[32 * i + 16] = cvt_bf16x2(a1, b1);
+    }
+    __syncwarp();
+    // 4. de-interleave and out
+    if (dst != nullptr) {
+      uint4 *out = reinterpret_cast<uint4 *>(dst + h0 * D) + lane;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const int pv = lane + 32 * v;
+        const uint4 w0 = reinterpret_cast<const uint4 *>(mine)[pv];
+        const uint4 w1 = reinterpret_cast<const uint4 *>(mine + L::kRegion)[pv];
+        out[32 * v] = make_uint4(prmt(w0.x, w0.y, 0x5410u), prmt(w0.z, w0.w, 0x5410u),
+                                 prmt(w1.x, w1.y, 0x5410u), prmt(w1.z, w1.w, 0x5410u));
+        if (second) {
+          out[D / 8 + 32 * v] = make_uint4(prmt(w0.x, w0.y, 0x7632u), prmt(w0.z, w0.w, 0x7632u),
+                                           prmt(w1.x, w1.y, 0x7632u), prmt(w1.z, w1.w, 0x7632u));
+        }
+      }
+    }
+    __syncwarp();  // the next row's packs overwrite the words
   }
 }
 
@@ -523,7 +718,7 @@ cudaError_t prefill_prep_bf16(const PrefillPrepArgs &a, cudaStream_t stream) {
   return dispatch_geometry(
       a.head_dim, a.rotary_dim, a.norm_mode, [&](auto d, auto rot, auto ieee) {
         prefill_prep_kernel<decltype(d)::value, decltype(rot)::value,
-                            decltype(ieee)::value, PrefillPrepArgs>
+                            decltype(ieee)::value>
             <<<unsigned(a.rows), warps * 32, 0, stream>>>(a);
         return cudaGetLastError();
       });
@@ -560,12 +755,19 @@ cudaError_t chunk_append_bf16(const ChunkPrepArgs &a, cudaStream_t stream) {
   if (valid != cudaSuccess) return valid;
   if (a.runs.run_count == 0 || a.runs.rows == 0) return cudaSuccess;
   const int pairs = (a.q_heads + 1) / 2 + 2 * ((a.kv_heads + 1) / 2);
-  const int warps = std::max(1, std::min(kPrepWarps, (pairs + 1) / 2));
+  const int warps = std::min(kAppendWarps, pairs);
+  const int groups = (pairs - 1) / kAppendWarps + 1;
+  int device = 0, sms = 0;
+  cudaError_t st = cudaGetDevice(&device);
+  if (st == cudaSuccess) st = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  if (st != cudaSuccess) return st;
+  // one wave of CTAs, each with an even share of the rows
+  const int wave = sms * (a.cfg.head_dim == 256 ? kAppendCtasPerSm : kAppendCtasPerSmWide);
+  const int ctas = std::min(a.runs.rows, std::max(1, wave / groups));
   return dispatch_geometry(
       a.cfg.head_dim, a.rotary_dim, a.norm_mode, [&](auto d, auto rot, auto ieee) {
-        prefill_prep_kernel<decltype(d)::value, decltype(rot)::value,
-                            decltype(ieee)::value, ChunkPrepArgs>
-            <<<unsigned(a.runs.rows), warps * 32, 0, stream>>>(a);
+        chunk_append_kernel<decltype(d)::value, decltype(rot)::value, decltype(ieee)::value>
+            <<<dim3(unsigned(ctas), unsigned(groups)), warps * 32, 0, stream>>>(a);
         return cudaGetLastError();
       });
 }

@@ -49,15 +49,19 @@ __device__ __forceinline__ int chunk_page(const Gemma4KvCacheConfig &c,
   return physical >= 0 && physical < c.num_pages ? physical : -1;
 }
 
+// A later row of the run takes the position's place of the ring.
+__device__ __forceinline__ bool chunk_overwritten(const Gemma4KvCacheConfig &c,
+                                                  const ChunkRun &run, int position) {
+  return c.window_size > 0 &&
+         position + int64_t(c.max_pages_per_seq) * c.page_size < int64_t(run.first) + run.count;
+}
+
 // Element offset (head 0) at which a run's row at `position` is stored, -1 where
 // it is not: no page, or a later row of the run takes the same place of the ring.
 __device__ __forceinline__ int64_t chunk_store_offset(const Gemma4KvCacheConfig &c,
                                                       const int32_t *page_table, int layer,
                                                       const ChunkRun &run, int position) {
-  if (c.window_size > 0 &&
-      position + int64_t(c.max_pages_per_seq) * c.page_size < int64_t(run.first) + run.count) {
-    return -1;
-  }
+  if (chunk_overwritten(c, run, position)) return -1;
   const int logical_page = position / c.page_size;
   const int physical = chunk_page(c, page_table, run.batch, logical_page);
   if (physical < 0) return -1;

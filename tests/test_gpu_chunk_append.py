@@ -69,6 +69,12 @@ APPENDS = {
     "ring": dict(counts=[200, 3, 64], firsts=[10, 1000, 0], ring=True, window=64, own_rows=False),
     "unmapped": dict(counts=[40], firsts=[0], unmap=[(0, 1)]),
     "many_runs": dict(counts=[1 + i % 3 for i in range(70)], firsts=[i * 3 for i in range(70)]),
+    # several rows to a CTA: runs that begin and end inside its share, gaps, pages of the ring it comes to again
+    "shares": dict(counts=[700, 1, 650, 90, 2, 33], firsts=[3, 500, 0, 41, 7, 15], gap=3),
+    "shares_ring": dict(counts=[700, 3, 640, 1], firsts=[10, 1000, 0, 63], ring=True, window=64, own_rows=False),
+    "shares_many": dict(counts=[1 + i % 40 for i in range(100)], firsts=[i * 7 for i in range(100)], page=5, gap=1),
+    "shares512": dict(counts=[300, 290, 5], firsts=[7, 64, 0], heads=1, group=16, dim=512, page=64, gap=2),
+    "shares_odd": dict(counts=[900, 301], firsts=[7, 64], heads=3, group=1),
 }
 
 
