@@ -87,9 +87,11 @@ constexpr int kInfos = 8;
 constexpr int kSegments = 8;
 constexpr long long kTileWaitClocks = 1ll << 26;
 constexpr uint32_t kWaitPolls = 1u << 20;     // tens of milliseconds at least; a tile takes microseconds
-// What starting an item costs next to a key tile (loading Q, reading O back), and
-// the least a CTA is given, both in key tiles: they shape the cut only.
-constexpr int kItemCost = 3;
+// What starting an item costs next to a key tile (loading Q, reading O back: some 10k
+// of a tile's 1.4k cycles), and the least a CTA is given, both in key tiles: they
+// shape the cut only. Item cost 3, 5, 8 on ragged runs over a ring: 117.2, 116.1,
+// 115.9 us; least share 2, 4, 8 for four tokens over a ring of 1024: 15.9, 16.1, 20.1.
+constexpr int kItemCost = 8;
 constexpr int kMinShare = 4;
 
 template <int kHeadDim_>
