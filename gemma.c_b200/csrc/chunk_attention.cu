@@ -42,7 +42,7 @@
 // Softmax: the maximum that a row's weights are scaled by is passed from tile to
 // tile (through shared memory, from one group to the other) and raised only when a
 // tile exceeds it by 2^8, so rescaling O is rare; scores, maxima, sums and O are
-// fp32, the weights are rounded to bf16 for P V (a relative 2^-9 each, which the
+// fp32, the weights are rounded to bf16 for P V (by at most 2^-8 of each, which the
 // average over keys does not add up), the sum takes them unrounded.
 //
 // Keys that no row of the tile sees (before the window, behind the last row, pages
@@ -283,6 +283,7 @@ struct SmallState {
   uint64_t q_free;            // the segment's last Q K^T is complete
   uint64_t o_full;            // its last P V is complete
   uint64_t o_free;            // its O has been read back
+  uint64_t drained;           // giving up: the MMAs issued so far are complete
   uint64_t seg_full[kSegments];
   TileInfo info[kInfos];
   SegmentInfo segment[kSegments];
@@ -418,7 +419,11 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   const int lane = tid & 31;
   const int heads = p.cfg.num_heads;
   if ((s_q_hi & 1023u) != 0) {  // the swizzle's atoms; the window starts on such a boundary
-    if (tid == 0) set_status(p.status, B200KV_STATUS_WAIT_TIMEOUT);
+    if (tid == 0) {
+      set_status(p.status, B200KV_STATUS_WAIT_TIMEOUT);
+      pdl_wait_for_predecessor();
+      p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    }
     return;
   }
 
@@ -436,6 +441,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   const uint32_t bar_q_free = smem_u32(&small.q_free);
   const uint32_t bar_o_full = smem_u32(&small.o_full);
   const uint32_t bar_o_free = smem_u32(&small.o_free);
+  const uint32_t bar_drained = smem_u32(&small.drained);
   const uint32_t bar_seg_full = smem_u32(&small.seg_full[0]);  // + 8 (segment % kSegments)
   if (tid == 0) {
     for (int i = 0; i < kMaxSlots; ++i) {
@@ -460,6 +466,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     mbar_init(bar_q_free, 1);
     mbar_init(bar_o_full, 1);
     mbar_init(bar_o_free, kSoftmaxWarps);
+    mbar_init(bar_drained, 1);
     for (int i = 0; i < kSegments; ++i) mbar_init(bar_seg_full + 8u * i, 1);
     small.abort = 0;
     mbar_fence_init();
@@ -688,9 +695,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         // box > 0: token group of box `lane` of the 32 from position `at` on, -1
         // without a page; asked for raw, checked when it is used
         int raw = -1, raw_offset = 0;
-        auto ask = [&](int at) {
+        auto ask = [&](uint32_t at) {  // (32 boxes on, this may be past 2^31)
           raw = -1;
-          const int position = at + (lane << box_shift);
+          const int position = int(min(at + (uint32_t(lane) << box_shift), uint32_t(limit)));
           if (position >= limit) return;
           int logical = p.page_div.quotient(position);
           raw_offset = (position - logical * p.cfg.page_size) >> 3;
@@ -700,7 +707,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         };
         int group_of_box = -1;
         int in_batch = batch_tiles;  // the current batch is used up
-        if (!own && p.box > 0) ask(k * kKeys);
+        if (!own && p.box > 0) ask(uint32_t(k * kKeys));
         for (int i = 0; i < count; ++i, ++n) {
           const int base = origin + (k + i) * kKeys;
           unsigned long long live = ~0ull;
@@ -712,7 +719,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
                                  ? layer_group + raw * page_groups + raw_offset
                                  : -1;
               in_batch = 0;
-              ask(base + 32 * p.box);
+              ask(uint32_t(base) + 32u * uint32_t(p.box));
             }
             group = __shfl_sync(0xffffffffu, group_of_box, (in_batch * tile_boxes + lane) & 31);
             ++in_batch;
@@ -998,6 +1005,10 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       if (ok) umma_commit_warp(bar_o_full, leader);
     }
     failed = !ok;
+    if (failed) {  // nothing reads shared memory or writes tensor memory when the CTA ends
+      umma_commit_warp(bar_drained, leader);
+      mbar_wait_bounded(bar_drained, 0, kTileWaitClocks);
+    }
   } else {
     // ------------------------------------------------------------ softmax
     const int group = warp >> 2;
@@ -1214,7 +1225,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       const bool whole = now_rows.piece < 0;
       const bool writes = active && row < now_rows.rows;
       const float l_row = active ? small.row_sum[0][row] + small.row_sum[1][row] : 0.0f;
-      const float inv = whole ? (l_row > 0.0f ? 1.0f / l_row : 0.0f) : 1.0f;
+      // (a sum of zero: no key; of NaN: the row is NaN)
+      const float inv = whole ? (l_row != 0.0f ? 1.0f / l_row : 0.0f) : 1.0f;
       float *piece = p.partials + (int64_t(blockIdx.x) * 2 + (whole ? 0 : now_rows.piece)) *
                                       (int64_t(p.rows_cap) * (kPartDims + 2));
       // This group's 128 columns of O, 32 lines of 128 bytes per warp at a time: 64
@@ -1296,7 +1308,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
           piece[p.rows_cap * kPartDims + row] = ref;
           piece[p.rows_cap * (kPartDims + 1) + row] = l_row;
         } else if (p.lse != nullptr && now_rows.part == 0) {
-          p.lse[now_rows.at] = l_row > 0.0f ? (ref + log2f(l_row)) * 0.6931471805599453f : -INFINITY;
+          p.lse[now_rows.at] = l_row != 0.0f ? (ref + log2f(l_row)) * 0.6931471805599453f : -INFINITY;
         }
       }
       n0 = n1;
@@ -1393,13 +1405,13 @@ __global__ __launch_bounds__(kCombineWarps * 32) void chunk_combine_kernel(Chunk
   const int part = meta.x / p.cfg.num_heads;
   const int head = meta.x - part * p.cfg.num_heads;
   const int token = p.group_div.quotient(row);
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   const int64_t at = (int64_t(meta.y) + token) * p.q_heads + head * p.group + (row - token * p.group);
   reinterpret_cast<uint4 *>(p.out + at * head_dim + part * kPartDims)[lane] =
       make_uint4(bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv),
                  bf16_pair(acc[4] * inv, acc[5] * inv), bf16_pair(acc[6] * inv, acc[7] * inv));
   if (p.lse != nullptr && part == 0 && lane == 0) {
-    p.lse[at] = l > 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+    p.lse[at] = l != 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
   }
 }
 
@@ -1557,7 +1569,8 @@ cudaError_t validate_chunk_attention(const ChunkAttentionArgs &a) {
   const int64_t pairs = a.runs.run_count * div_up(int64_t(std::min(a.runs.max_row_count, a.runs.rows)), tokens);
   const int64_t keys = (c.window_size > 0 ? c.window_size + tokens : table_end(c)) +
                        (a.k_rows != nullptr ? a.runs.max_row_count : 0);
-  const double cost = double(keys / kKeys + 8) * double(pairs) * c.num_heads * (c.head_dim / kPartDims);
+  // (each of the four stretches of keys may begin and end inside a tile)
+  const double cost = double(keys / kKeys + 8 + kItemCost) * double(pairs) * c.num_heads * (c.head_dim / kPartDims);
   if (pairs > (1 << 24) || cost >= 2147483648.0) return cudaErrorInvalidValue;
   if (int64_t(a.workspace_bytes) < workspace_per_cta(a.q_heads / c.num_heads, a.runs.max_row_count)) {
     return cudaErrorInvalidValue;

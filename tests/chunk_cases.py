@@ -57,7 +57,7 @@ def visible_positions(case: ChunkCase, i: int):
     _, num_pages, ps, slots, _, _, _, ring = case.cfg
     first, count, w = int(case.first[i]), int(case.count[i]), case.eff_window
     lo = max(0, first - w + 1) if w else 0
-    wanted = [p for p in range(first + count) if p >= lo or p < case.sinks]
+    wanted = [*range(min(case.sinks, lo, first + count)), *range(lo, first + count)]
     found = []
     for p in wanted:
         if case.k_rows is not None and p >= first:

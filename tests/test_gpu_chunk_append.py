@@ -143,6 +143,36 @@ def test_layer_step(kv, ring):
     check_attention(case, t)
 
 
+def test_a_captured_layer_step(kv):
+    """Append, attention and write captured once, replayed on rows and lengths of the moment."""
+    case = make_case(6, [90, 1, 17], [120, 300, 0], ring=True, window=64)
+    raw = raw_inputs(kv, case, 256, 4)
+    a, t = device_args(kv, case)
+    fill(a, raw)
+    a.rotary_dim = 256
+    before = [t[n].clone() for n in ("cache_k", "cache_v")]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kv.chunk_layer_step(a, stream=torch.cuda.current_stream())
+    case.count[:], case.first[:] = [33, 1, 16], [100, 290, 3]
+    case.cache_k, case.cache_v = (torch.from_numpy(np.random.default_rng(8 + i).standard_normal(
+        case.cache_k.shape, dtype=np.float32)).bfloat16() for i in range(2))
+    for n in ("cache_k", "cache_v"):
+        t[n].copy_(getattr(case, n))
+    t["row_count"].copy_(torch.from_numpy(case.count))
+    t["first_position"].copy_(torch.from_numpy(case.first))
+    raw["raw_q"].mul_(0.5)
+    q, k, v = prepared(kv, case, raw, 256, 0)
+    want_k, want_v = stored(case, t["cache_k"], k), stored(case, t["cache_v"], v)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not torch.equal(before[0], t["cache_k"])
+    bits = lambda x: x.view(torch.int16).reshape(-1)  # noqa: E731
+    assert torch.equal(bits(t["cache_k"]), bits(want_k)) and torch.equal(bits(t["cache_v"]), bits(want_v))
+    case.q, case.k_rows, case.v_rows = q.cpu(), k.cpu(), v.cpu()
+    check_attention(case, t)
+
+
 # --------------------------------------------------------------------------------------------- page copies
 def copy_case(kv, layers, pages, ps, heads, dim, fp8, seed):
     gen = torch.Generator(device="cuda")

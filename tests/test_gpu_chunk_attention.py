@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.chunk_cases import check_attention, device_args, make_case
+from tests.chunk_cases import attention_f64, check_attention, device_args, make_case
 from tests.gpu_util import need_gpu
 
 pytestmark = [pytest.mark.gpu, need_gpu]
@@ -126,6 +126,93 @@ def test_a_replayed_call_reads_the_lengths_of_the_moment(kv):
     graph.replay()
     torch.cuda.synchronize()
     check_attention(case, t)
+
+
+@pytest.mark.parametrize("page,own", [(16, True), (64, True), (64, False), (5, True)])
+def test_the_last_positions_there_are(kv, page, own):
+    """A ring at the end of the positions: nothing beyond them is looked up."""
+    end = 2**31 - 1024
+    window = 128 if page != 5 else 125
+    case = make_case(12, [40, 1], [end - 1 - 40, end - 1 - 1], ring=True, window=window, page=page, own_rows=own,
+                     ring_slots=None if own else 4)
+    a, t = device_args(kv, case)
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+
+
+def test_rows_of_no_run_are_not_used(kv):
+    """Rows between the runs hold NaN, and key tiles of 64 own rows reach into them and into the next run's."""
+    case = make_case(13, [70, 3, 65, 1], [100, 64, 0, 7], own_rows=True, gap=2)
+    free = torch.ones(case.rows, dtype=torch.bool)
+    for s, c in zip(case.start, case.count):
+        free[s:s + c] = False
+    for x in (case.q, case.k_rows, case.v_rows):
+        x[free] = float("nan")
+    a, t = device_args(kv, case)
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+
+
+@pytest.mark.parametrize("where", ["cache_k", "cache_v"])
+@pytest.mark.parametrize("first", [40, 4000])            # one CTA has the item; several share it
+def test_a_nan_that_a_row_sees_is_in_its_result(kv, where, first):
+    case = make_case(14, [3], [first])
+    page = int(case.table[0, 1])                         # position 20
+    getattr(case, where)[0, page * 16 + 4, 5] = float("nan")
+    a, t = device_args(kv, case)
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    out, lse = t["out"].cpu().view(3, 8, 2, 256), t["lse"].cpu().view(3, 8, 2)
+    assert bool(out[:, 5].isnan().all())
+    assert bool(lse[:, 5].isnan().all()) == (where == "cache_k")
+    want, want_lse, tol, tol_lse = (x.view(3, 8, 2, -1) for x in attention_f64(case)[0])
+    rest = [h for h in range(8) if h != 5]
+    assert bool(((out.double() - want).abs() <= tol)[:, rest].all())
+    assert bool(((lse.double()[..., None] - want_lse).abs() <= tol_lse)[:, rest].all())
+
+
+@pytest.mark.parametrize("ctas", [1, 2, 7])
+def test_a_small_workspace_means_fewer_ctas(kv, ctas):
+    case = make_case(15, [1, 130, 7], [900, 0, 255])
+    a, t = device_args(kv, case)
+    a.workspace_bytes = kv.chunk_workspace_bytes(16, 8, 256, 3, 130, sm_count=ctas)
+    t["workspace"][a.workspace_bytes:].fill_(77)
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+    assert bool((t["workspace"][a.workspace_bytes:] == 77).all())
+
+
+def test_calls_on_two_streams_at_once(kv):
+    """Each with its own workspace, on streams of their own; the bits are those of the call alone."""
+    case = make_case(16, [1, 130, 7, 300], [3000, 100, 255, 77])
+    calls = [device_args(kv, case) for _ in range(3)]
+    kv.chunk_attention(calls[0][0])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        for (a, _t), s in zip(calls[1:], streams):
+            kv.chunk_attention(a, stream=s)
+    torch.cuda.synchronize()
+    for _a, t in calls[1:]:
+        assert torch.equal(t["out"], calls[0][1]["out"]) and torch.equal(t["lse"], calls[0][1]["lse"])
+    check_attention(case, calls[0][1])
+
+
+def test_calls_one_behind_the_other_share_a_workspace(kv):
+    """On one stream: the second call's partial results come after the first one's have been joined."""
+    one, two = make_case(17, [3, 1], [6000, 4097]), make_case(18, [1, 130, 7], [2000, 0, 255])
+    (a, ta), (b, tb) = device_args(kv, one), device_args(kv, two)
+    work = torch.empty(max(a.workspace_bytes, b.workspace_bytes), dtype=torch.uint8, device="cuda")
+    a.workspace = b.workspace = work.data_ptr()
+    for _ in range(5):
+        kv.chunk_attention(a)
+        kv.chunk_attention(b)
+    torch.cuda.synchronize()
+    check_attention(one, ta)
+    check_attention(two, tb)
 
 
 def test_cache_offsets_beyond_32_bits(kv):
