@@ -1600,6 +1600,8 @@ cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &a, cudaStream_t strea
   if (st != cudaSuccess) return st;
   st = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
   if (st != cudaSuccess) return st;
+  const int few = chunk_few_cluster(a, sms, table_end(a.cfg));
+  if (few > 0) return chunk_attention_few_bf16(a, few, table_end(a.cfg), stream);
   // one CTA per SM, or as many as the workspace has room for
   const int64_t room = int64_t(a.workspace_bytes) /
                        workspace_per_cta(a.q_heads / a.cfg.num_heads, a.runs.max_row_count);
