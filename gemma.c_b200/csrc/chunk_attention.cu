@@ -112,21 +112,6 @@ struct ChunkTraits {
   static constexpr int kTileBytes = kVAt + kVRing * kSlotBytes;
 };
 
-// Division of 0 .. 2^31 - 1 by a fixed number: the quotient's high part by a 32-bit
-// multiplication (Granlund and Montgomery's round-up method).
-struct FastDiv {
-  uint32_t d, m, shift;
-  __device__ __forceinline__ int quotient(int n) const {
-    return int((__umulhi(uint32_t(n), m) + uint32_t(n)) >> shift);
-  }
-  static FastDiv by(uint32_t d) {
-    FastDiv f = {d, 0, 0};
-    while ((1ull << f.shift) < d) ++f.shift;
-    f.m = uint32_t(((1ull << 32) * ((1ull << f.shift) - d)) / d + 1);
-    return f;
-  }
-};
-
 struct ChunkParams {
   __nv_bfloat16 *out;
   float *lse;
@@ -1600,8 +1585,9 @@ cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &a, cudaStream_t strea
   if (st != cudaSuccess) return st;
   st = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
   if (st != cudaSuccess) return st;
-  const int few = chunk_few_cluster(a, sms, table_end(a.cfg));
-  if (few > 0) return chunk_attention_few_bf16(a, few, table_end(a.cfg), stream);
+  bool taken = false;
+  st = chunk_attention_few_bf16(a, device, table_end(a.cfg), stream, &taken);
+  if (st != cudaSuccess || taken) return st;
   // one CTA per SM, or as many as the workspace has room for
   const int64_t room = int64_t(a.workspace_bytes) /
                        workspace_per_cta(a.q_heads / a.cfg.num_heads, a.runs.max_row_count);

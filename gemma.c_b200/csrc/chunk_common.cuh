@@ -10,6 +10,21 @@ namespace b200kv {
 // Positions below this leave room for a key tile's arithmetic in 32 bits.
 constexpr int32_t kMaxPosition = 2147483647 - 1024;
 
+// Division of 0 .. 2^31 - 1 by a fixed number: the quotient's high part by a 32-bit
+// multiplication (Granlund and Montgomery's round-up method).
+struct FastDiv {
+  uint32_t d, m, shift;
+  __device__ __forceinline__ int quotient(int n) const {
+    return int((__umulhi(uint32_t(n), m) + uint32_t(n)) >> shift);
+  }
+  static FastDiv by(uint32_t d) {
+    FastDiv f = {d, 0, 0};
+    while ((1ull << f.shift) < d) ++f.shift;
+    f.m = uint32_t(((1ull << 32) * ((1ull << f.shift) - d)) / d + 1);
+    return f;
+  }
+};
+
 // One run as the device sees it; count 0 where the call skips it.
 struct ChunkRun {
   int32_t batch = 0;

@@ -331,12 +331,10 @@ struct ChunkAttentionArgs {
 };
 cudaError_t validate_chunk_attention(const ChunkAttentionArgs &args);
 cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &args, cudaStream_t stream);
-// The form for few rows and few sequences (chunk_attention_few.cu): CTAs per (run, KV
-// head) for these sizes, 0: not for them. table_end: first position past a linear
-// cache's table.
-int chunk_few_cluster(const ChunkAttentionArgs &args, int sm_count, int table_end);
-cudaError_t chunk_attention_few_bf16(const ChunkAttentionArgs &args, int cluster, int table_end,
-                                     cudaStream_t stream);
+// The form for few rows and few sequences (chunk_attention_few.cu); *taken: it was for
+// these sizes. table_end: first position past a linear cache's table.
+cudaError_t chunk_attention_few_bf16(const ChunkAttentionArgs &args, int device, int table_end,
+                                     cudaStream_t stream, bool *taken);
 size_t chunk_workspace_bytes(int q_heads, int kv_heads, int head_dim, int run_count,
                              int max_row_count, int sm_count);
 
