@@ -54,6 +54,7 @@
 #include <algorithm>
 
 #include "chunk_common.cuh"
+#include "chunk_maps.cuh"
 #include "kernels.cuh"
 #include "umma_common.cuh"
 
@@ -310,25 +311,6 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&r)[64]) {
   }
 }
 
-// One box of a page: `box` tokens x 256 dims, token groups of eight from `token_group`.
-__device__ __forceinline__ void tma_load_page_box(uint32_t dst, const CUtensorMap *map, int block,
-                                                  int token_group, int head, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(0), "r"(block), "r"(token_group),
-      "r"(head), "r"(bar)
-      : "memory");
-}
-// Eight packed rows x 256 dims; rows past the tensor arrive as zeros.
-__device__ __forceinline__ void tma_load_rows_box(uint32_t dst, const CUtensorMap *map, int block,
-                                                  int row, int head, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(block), "r"(head), "r"(bar)
-      : "memory");
-}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -1405,44 +1387,6 @@ int table_end(const Gemma4KvCacheConfig &c) {
   return int(std::min<int64_t>(kMaxPosition, int64_t(c.max_pages_per_seq) * c.page_size));
 }
 
-// Tokens per box: the largest power of two up to a key tile that divides the page
-// (a box then lies in one page); less than eight rows do not fill a swizzle atom.
-int box_tokens(int page_size) {
-  int box = kKeys;
-  while (page_size % box != 0) box /= 2;
-  return box >= 8 ? box : 0;
-}
-
-bool make_cache_map(CUtensorMap *map, const __nv_bfloat16 *base, const Gemma4KvCacheConfig &c, int box) {
-  EncodeTiledFn encode = encode_tiled_fn();
-  if (encode == nullptr) return false;
-  const cuuint64_t row = cuuint64_t(c.num_heads) * c.head_dim * 2;
-  // [head][group of 8 tokens][block of 64 dims][token of the group][64 dims]: the
-  // pages of all layers are one row of tokens, of which a box takes whole groups
-  const cuuint64_t dims[5] = {64, 8, cuuint64_t(c.head_dim / 64),
-                              cuuint64_t(c.num_layers) * c.num_pages * (c.page_size / 8),
-                              cuuint64_t(c.num_heads)};
-  const cuuint64_t strides[4] = {row, 128, row * 8, cuuint64_t(c.head_dim) * 2};
-  const cuuint32_t boxes[5] = {64, 8, kPartDims / 64, cuuint32_t(box / 8), 1};
-  const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<__nv_bfloat16 *>(base), dims,
-                strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-bool make_rows_map(CUtensorMap *map, const __nv_bfloat16 *base, int rows, int heads, int head_dim) {
-  EncodeTiledFn encode = encode_tiled_fn();
-  if (encode == nullptr) return false;
-  const cuuint64_t row = cuuint64_t(heads) * head_dim * 2;
-  const cuuint64_t dims[4] = {64, cuuint64_t(rows), cuuint64_t(head_dim / 64), cuuint64_t(heads)};
-  const cuuint64_t strides[3] = {row, 128, cuuint64_t(head_dim) * 2};
-  const cuuint32_t box[4] = {64, 8, kPartDims / 64, 1};
-  const cuuint32_t steps[4] = {1, 1, 1, 1};
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<__nv_bfloat16 *>(base), dims,
-                strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 bool make_q_map(CUtensorMap *map, const __nv_bfloat16 *q, int rows, int q_heads, int head_dim,
                 int group, int box_tokens) {
   EncodeTiledFn encode = encode_tiled_fn();
@@ -1490,7 +1434,7 @@ cudaError_t launch_chunk(const ChunkAttentionArgs &a, int ctas, cudaStream_t str
   p.window = a.window;
   p.sinks = a.sinks;
   p.table_end = table_end(c);
-  p.box = box_tokens(c.page_size);
+  p.box = box_tokens(c.page_size, kKeys);
   p.page_div = FastDiv::by(uint32_t(c.page_size));
   p.slot_div = FastDiv::by(uint32_t(c.max_pages_per_seq));
   p.group_div = FastDiv::by(uint32_t(p.group));

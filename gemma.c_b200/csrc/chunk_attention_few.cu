@@ -6,20 +6,23 @@
 // rows of the warp-level products (mma.sync m16n8k16): tcgen05 would spend its 128
 // rows, its tensor memory and its barriers on them. A cluster of CTAs takes one (run,
 // KV head) and each of its CTAs an even share of the keys in units of 16, a tile of 64
-// (head_dim 512: 32) at a time. K and V rows come by a bulk copy each, a tile ahead,
-// whatever the page size; rows that nobody sees are zeros. Per tile, eight warps:
+// (head_dim 512: 32) at a time, brought by TMA a tile ahead: each of the eight warps asks
+// for one unit of K or V (head_dim 512: half of one), in a box or two that lie in a page,
+// so pages are of whole groups of eight tokens. (A copy per row costs its warp 86 clocks
+// each, 16 of them more than the tile's arithmetic.) Per tile:
 //   S = Q K^T     16 keys and 128 dims each, joined through shared memory
 //   softmax       16 threads to a row: running maximum and sum in fp32, the weights
 //                 rounded to bf16 for P V (by at most 2^-8 of each), summed unrounded
 //   O = a O + P V an eighth of the output dims each, fp32 in registers
 // At the end every CTA sends each other one its share of the output dims, with maxima
-// and sums, over distributed shared memory; after one cluster barrier a CTA joins and
-// writes its share. One launch, no partial results in memory. The code is kept small:
+// and sums, by bulk copies between their shared memories; a CTA joins and writes its
+// share when those have come. One launch, no partial results in memory. The code is kept small:
 // a call runs most of it once, and fetching it is part of what that takes.
 #include <algorithm>
 #include <atomic>
 
 #include "chunk_common.cuh"
+#include "chunk_maps.cuh"
 #include "kernels.cuh"
 
 namespace b200kv {
@@ -38,8 +41,8 @@ struct FewTraits {
   static constexpr int kKeys = D == 256 ? 64 : 32;        // of a tile
   static constexpr int kUnits = kKeys / kFewUnit;
   static constexpr int kDimParts = kFewWarps / kUnits;    // warps that share 16 keys, 128 dims each
-  static constexpr int kPitch = D * 2 + 16;               // bytes of a row: no bank twice
-  static constexpr int kTileBytes = kKeys * kPitch;       // of K or V
+  static constexpr int kUnitBytes = kFewUnit * D * 2;     // D / 256 boxes of 16 keys x 256 dims
+  static constexpr int kTileBytes = kUnits * kUnitBytes;  // of K or V
   static constexpr int kPartPitch = kKeys + 8;            // floats of a row of scores
   static constexpr int kOut = D / kFewWarps;              // dims of a warp's part of P V
   static constexpr int kGroups = D / 16;                  // of 16 output dims
@@ -48,20 +51,23 @@ struct FewTraits {
 template <int D>
 struct FewShared {
   using T = FewTraits<D>;
-  uint8_t tile[kFewStages][2][T::kTileBytes];             // K and V
+  uint8_t tile[kFewStages][2][T::kTileBytes];             // K and V; at the end O, in groups
   float part[T::kDimParts][kFewRows][T::kPartPitch];      // scores
   uint8_t weights[kFewRows][T::kKeys * 2 + 16];           // bf16
   float alpha[kFewRows];                                  // what O is rescaled by
-  unsigned long long alive[kFewStages];  // keys of the tile that some row sees, 8 to a byte
-  uint64_t full[kFewStages];             // the tile has landed
+  uint16_t alive[kFewStages][4];  // keys of the tile's units that some row sees
+  uint64_t full[kFewStages];      // the tile has landed
+  uint64_t joined;                // what the cluster's CTAs send has landed
+  alignas(16) float2 mine[kFewRows];                 // maximum and sum that this CTA has of the rows
+  float factor[kFewRows][kFewMaxCluster];  // what a CTA's O counts for in the row
   // What the cluster's CTAs send here: maximum and sum of [rank][row], and [rank][n][row]
   // 16 dims of this CTA's n-th group.
-  float2 row[kFewMaxCluster][kFewRows];
-  float sent[(T::kGroups + kFewMaxCluster) * kFewRows * 16];
+  alignas(16) float2 row[kFewMaxCluster][kFewRows];
+  alignas(16) float sent[(T::kGroups + kFewMaxCluster) * kFewRows * 16];
 };
 
 struct FewDivs {
-  FastDiv page;   // by page_size
+  FastDiv page;   // by page_size (tokens)
   FastDiv slots;  // by max_pages_per_seq
   FastDiv group;  // by the query heads of a KV head
   FastDiv ctas;   // by the cluster's size
@@ -136,16 +142,28 @@ __device__ __forceinline__ uint32_t peer_address(uint32_t at, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void store_peer(uint32_t at, float x, float y) {
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(x), "f"(y) : "memory");
+// Shared memory to that of another CTA, counted on a barrier there.
+__device__ __forceinline__ void copy_to_peer(uint32_t to, uint32_t from, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
+      "r"(from), "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ bool few_wait(uint32_t bar, uint32_t parity) {
+  for (uint32_t left = kFewPolls; !mbar_try_wait(bar, parity); --left) {
+    if (left == 0) return false;
+  }
+  return true;
 }
 
 // grid (CTAs of a cluster, KV heads, runs)
 template <int D>
 __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
-    const __grid_constant__ ChunkAttentionArgs a, int table_end, FewDivs div) {
+    const __grid_constant__ ChunkAttentionArgs a, const __grid_constant__ CUtensorMap map_k,
+    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k_rows,
+    const __grid_constant__ CUtensorMap map_v_rows, int table_end, int box, FewDivs div) {
   using T = FewTraits<D>;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   FewShared<D> &s = *reinterpret_cast<FewShared<D> *>(smem_raw);
   const int tid = int(threadIdx.x);
   const int warp = tid >> 5;
@@ -157,9 +175,14 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
   const int rank = int(blockIdx.x);
   const int head = int(blockIdx.y);
   const uint32_t bar_full = smem_u32(&s.full[0]);
+  const uint32_t bar_joined = smem_u32(&s.joined);
+  // groups of 16 output dims that this CTA joins: number n of the dims is CTA n % ctas's
+  const int slots = div.ctas.quotient(T::kGroups + ctas - 1 - rank);
   if (tid == 0) {
     for (int i = 0; i < kFewStages; ++i) mbar_init(bar_full + 8u * i, kFewWarps);
+    mbar_init(bar_joined, 1);
     mbar_fence_init();
+    mbar_arrive_expect_tx(bar_joined, uint32_t(ctas * (slots * 1024 + int(sizeof(s.mine)))));
   }
   __syncthreads();
   pdl_wait_for_predecessor();
@@ -176,55 +199,59 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
   const int units = even + (rank < rest ? 1 : 0);
   const int tiles = div_up(units, T::kUnits);
 
-  // ---- K and V. A warp brings eight rows of a tile, of both (head_dim 512: of one of
-  // them); lane l looks up row l % 8 of tile l / 8 of a batch of four.
-  constexpr int64_t kOwn = int64_t(1) << 62;
-  const int row8 = (warp % (T::kKeys / 8)) * 8;
-  int64_t here = -1;  // element offset (kOwn: of the run's rows), -1: nobody sees it
+  // ---- K and V: this warp's unit of a tile. Lanes 2 i and 2 i + 1 look up the first and
+  // the last eight keys of the unit of tile i, 16 tiles at a time.
+  const bool is_v = (warp & 1) != 0;
+  const int my_unit = (warp >> 1) % T::kUnits;
+  const int block0 = (warp >> 1) / T::kUnits * (kBoxDims / 64);  // head_dim 512: dims from 256 on
+  const int page_groups = c.page_size / 8;
+  int token_group = -1;  // cache: group of eight tokens; -1: none
   auto issue = [&](int j) {
     if (j >= tiles) return;
-    if ((j & 3) == 0) {
-      here = -1;
-      const int of_tile = row8 + (lane & 7);
-      const int unit = (j + (lane >> 3)) * T::kUnits + of_tile / kFewUnit;
+    const int unit = j * T::kUnits + my_unit;
+    if ((j & 15) == 0) {
+      token_group = -1;
+      const int ask = unit + (lane >> 1) * T::kUnits;
       bool own;
-      const int at = keys.base(unit0 + unit, own) + of_tile % kFewUnit;
-      if (unit < units && own) {
-        if (at - run.first < run.count) {
-          here = kOwn + ((int64_t(run.start) + (at - run.first)) * heads + head) * D;
-        }
-      } else if (unit < units && at < keys.cache_end && (at >= keys.lo || at < a.sinks)) {
+      const int at = keys.base(unit0 + ask, own) + 8 * (lane & 1);
+      if (ask < units && !own && at < keys.cache_end) {
         const int logical = div.page.quotient(at);
         const int slot = c.window_size > 0 ? logical - div.slots.quotient(logical) * c.max_pages_per_seq : logical;
         const int page = __ldg(a.page_table + int64_t(run.batch) * c.max_pages_per_seq + slot);
         if (page >= 0 && page < c.num_pages) {
-          here = cache_offset(c, a.layer, page, at - logical * c.page_size, head, 0);
+          token_group = (a.layer * c.num_pages + page) * page_groups + ((at - logical * c.page_size) >> 3);
         }
       }
     }
+    // the keys of the unit that some row sees
+    bool own;
+    const int base = keys.base(unit0 + unit, own);
+    uint32_t alive = unit >= units ? 0u
+                     : own         ? low16(run.first + run.count - base)
+                                   : low16(keys.cache_end - base) & (~low16(keys.lo - base) | low16(a.sinks - base));
+    const int group0 = __shfl_sync(0xffffffffu, token_group, 2 * (j & 15));
+    const int group1 = __shfl_sync(0xffffffffu, token_group, 2 * (j & 15) + 1);
+    if (!own) alive &= (group0 >= 0 ? 0xffu : 0u) | (group1 >= 0 ? 0xff00u : 0u);
     const int stage = j % kFewStages;
     const uint32_t bar = bar_full + 8u * uint32_t(stage);
-    const int64_t at = __shfl_sync(0xffffffffu, here, (j & 3) * 8 + (lane & 7));
-    const uint32_t alive = __ballot_sync(0xffffffffu, at >= 0) & 0xffu;
-    constexpr int kTensors = D == 256 ? 2 : 1;  // that a warp brings
-    const int tensor = D == 256 ? lane >> 3 : warp >> 2;
+    const uint32_t to = smem_u32(&s.tile[stage][is_v][my_unit * T::kUnitBytes]) + uint32_t(block0 * 2048);
+    const bool both = !own && box == 16;  // one box for both groups of eight
+    const bool half0 = (alive & 0xffu) != 0 || (both && alive != 0), half1 = (alive >> 8) != 0 && !both;
     if (lane == 0) {
-      if (warp < T::kKeys / 8) reinterpret_cast<uint8_t *>(&s.alive[stage])[warp] = uint8_t(alive);
-      mbar_arrive_expect_tx(bar, uint32_t(__popc(alive)) * uint32_t(kTensors * D * 2));
-    }
-    __syncwarp();
-    uint8_t *to = &s.tile[stage][tensor & 1][(row8 + (lane & 7)) * T::kPitch];
-    if (lane < 8 * kTensors) {
-      if (at >= 0) {
-        const bool own = (at & kOwn) != 0;
-        const __nv_bfloat16 *from = tensor == 0 ? (own ? a.k_rows : a.cache_k) : (own ? a.v_rows : a.cache_v);
-        bulk_load(smem_u32(to), from + (at & ~kOwn), D * 2, bar);
-      } else {
+      if (!is_v && block0 == 0) s.alive[stage][my_unit] = uint16_t(alive);
+      mbar_arrive_expect_tx(bar, uint32_t((half0 ? (both ? 2 : 1) : 0) + (half1 ? 1 : 0)) * 4096u);
+      const CUtensorMap *map = own ? (is_v ? &map_v_rows : &map_k_rows) : (is_v ? &map_v : &map_k);
 #pragma unroll 1
-        for (int i = 0; i < D * 2; i += 16) *reinterpret_cast<uint4 *>(to + i) = make_uint4(0u, 0u, 0u, 0u);
-        fence_proxy_async_shared();  // (a later tile's copy comes after these)
+      for (int h = 0; h < 2; ++h) {
+        if (!(h == 0 ? half0 : half1)) continue;
+        if (own) {
+          tma_load_rows_box(to + uint32_t(4096 * h), map, block0, run.start + base - run.first + 8 * h, head, bar);
+        } else {
+          tma_load_page_box(to + uint32_t(4096 * h), map, block0, h == 0 ? group0 : group1, head, bar);
+        }
       }
     }
+    __syncwarp();
   };
   issue(0);
 
@@ -259,27 +286,20 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
 #pragma unroll 1
   for (int j = 0; j < tiles; ++j) {
     const int stage = j % kFewStages;
-    const uint32_t parity = uint32_t(j / kFewStages) & 1u;
-    for (uint32_t left = kFewPolls; ok && !mbar_try_wait(bar_full + 8u * uint32_t(stage), parity); --left) {
-      ok = left > 0;
-    }
-    ok = __syncthreads_and(ok);
-    if (!ok) {  // a copy did not come; give it time to land before the CTA ends
-      mbar_wait_bounded(bar_full + 8u * uint32_t(stage), parity, 1ll << 26);
-      set_status(a.status, B200KV_STATUS_WAIT_TIMEOUT);
-      break;
-    }
-    issue(j + 1);
+    issue(j + 1);  // (its place was read before the barrier among the scores of tile j - 1)
+    ok = few_wait(bar_full + 8u * uint32_t(stage), uint32_t(j / kFewStages) & 1u);
     const uint32_t k_at = tile_at + uint32_t(2 * stage * T::kTileBytes);
     const uint32_t v_at = k_at + uint32_t(T::kTileBytes);
     {  // a part of the scores
       float sc[2][2][4] = {};
-      const uint32_t from = k_at + uint32_t((key16 + (lane & 7) + (lane >> 4) * 8) * T::kPitch + dim_part * 256 +
-                                            ((lane >> 3) & 1) * 16);
+      // (unit, group of eight keys, block of 64 dims, key, its 16-byte chunks swizzled)
+      const uint32_t from = k_at + uint32_t(key16 / 16 * T::kUnitBytes + (dim_part >> 1) * 8192 + (lane >> 4) * 4096 +
+                                            (dim_part & 1) * 2048 + (lane & 7) * 128);
+      const uint32_t chunk = uint32_t(((lane >> 3) & 1) ^ (lane & 7)) << 4;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         uint32_t b[4];
-        ldmatrix_x4(b, from + 32u * uint32_t(k));
+        ldmatrix_x4(b, from + uint32_t(k >> 2) * 1024u + (chunk ^ (uint32_t(k & 3) << 5)));
         mma_bf16(sc[k & 1][0], q[k], b[0], b[1]);
         mma_bf16(sc[k & 1][1], q[k], b[2], b[3]);
       }
@@ -297,19 +317,40 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
       bool own;
       const int first = kMine * place;
       const int at = keys.base(unit0 + j * T::kUnits + first / kFewUnit, own) + first % kFewUnit;
-      sees = uint32_t(s.alive[stage] >> first) & low16(t + 1 - at);
+      sees = uint32_t(s.alive[stage][first / kFewUnit] >> (first % kFewUnit)) & low16(t + 1 - at);
       if (a.window > 0) sees &= ~low16(t - a.window + 1 - at) | low16(a.sinks - at);
     }
     uint32_t v[T::kUnits][T::kOut / 16][4];
+    const int v_block = warp * T::kOut / 64;  // of 64 dims
 #pragma unroll
     for (int u = 0; u < T::kUnits; ++u) {
+      const uint32_t from = v_at + uint32_t(u * T::kUnitBytes + (v_block >> 2) * 8192 + (in8 >> 3) * 4096 +
+                                            (v_block & 3) * 1024 + (in8 & 7) * 128);
+      const uint32_t chunk = uint32_t((((warp * T::kOut) & 63) / 8 + (lane >> 4)) ^ (in8 & 7)) << 4;
 #pragma unroll
-      for (int n = 0; n < T::kOut / 16; ++n) {
-        ldmatrix_x4_trans(v[u][n], v_at + uint32_t((16 * u + in8) * T::kPitch + warp * T::kOut * 2 + 32 * n +
-                                                   (lane >> 4) * 16));
+      for (int n = 0; n < T::kOut / 16; ++n) ldmatrix_x4_trans(v[u][n], from + (chunk ^ uint32_t(32 * n)));
+      // keys that nobody sees may hold anything (0 * NaN): this lane has keys 2 (lane % 4),
+      // + 1, + 8 and + 9
+      const uint32_t alive = s.alive[stage][u];
+      if (alive != 0xffffu) {
+        const uint32_t mine = alive >> t2;
+        const uint32_t keep0 = ((mine & 1u) != 0 ? 0xffffu : 0u) | ((mine & 2u) != 0 ? 0xffff0000u : 0u);
+        const uint32_t keep1 = ((mine & 0x100u) != 0 ? 0xffffu : 0u) | ((mine & 0x200u) != 0 ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int n = 0; n < T::kOut / 16; ++n) {
+          v[u][n][0] &= keep0;
+          v[u][n][1] &= keep1;
+          v[u][n][2] &= keep0;
+          v[u][n][3] &= keep1;
+        }
       }
     }
-    __syncthreads();
+    ok = __syncthreads_and(ok);
+    if (!ok) {  // a tile did not come: give its copies time to land before the CTA ends
+      mbar_wait_bounded(bar_full + 8u * uint32_t(stage), uint32_t(j / kFewStages) & 1u, 1ll << 26);
+      set_status(a.status, B200KV_STATUS_WAIT_TIMEOUT);
+      break;
+    }
     {
       float x[kMine];
 #pragma unroll
@@ -373,51 +414,71 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
       }
     }
   }
-  // ---- to the CTAs that join the dims: group n of 16 is CTA n % ctas's
+  // ---- to the CTAs that join the dims: a group is 16 rows x 16 dims
 #pragma unroll
   for (int d = 8; d > 0; d /= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
+  if (place == 0) s.mine[row] = make_float2(m, l);
+  float *groups = reinterpret_cast<float *>(&s.tile[0][0][0]);
+#pragma unroll
+  for (int n = 0; n < T::kOut / 8; ++n) {
+    float *to = groups + (warp * (T::kOut / 16) + n / 2) * 256 + g * 16 + 8 * (n & 1) + t2;
+    *reinterpret_cast<float2 *>(to) = make_float2(o[n][0], o[n][1]);
+    *reinterpret_cast<float2 *>(to + 128) = make_float2(o[n][2], o[n][3]);
+  }
+  fence_proxy_async_shared();
+  __syncthreads();
   cluster_wait();
-  if (place < ctas) store_peer(peer_address(smem_u32(&s.row[rank][row]), uint32_t(place)), m, l);
-  const int slots = div.ctas.quotient(T::kGroups + ctas - 1);  // groups of a CTA
-#pragma unroll
-  for (int n = 0; n < T::kOut / 16; ++n) {
-    const int of_dims = warp * (T::kOut / 16) + n;
+  // (a copy costs its warp its time: a few to each)
+  if (lane < T::kOut / 16) {
+    const int of_dims = warp * (T::kOut / 16) + lane;
     const int slot = div.ctas.quotient(of_dims);
-    const uint32_t at = peer_address(smem_u32(&s.sent[((rank * slots + slot) * kFewRows + g) * 16 + t2]),
-                                     uint32_t(of_dims - slot * ctas));
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      store_peer(at + 32u * uint32_t(h), o[2 * n + h][0], o[2 * n + h][1]);
-      store_peer(at + 32u * uint32_t(h) + 512u, o[2 * n + h][2], o[2 * n + h][3]);
+    const int owner = of_dims - slot * ctas;
+    const int theirs = div.ctas.quotient(T::kGroups + ctas - 1 - owner);
+    copy_to_peer(peer_address(smem_u32(&s.sent[(rank * theirs + slot) * 256]), uint32_t(owner)),
+                 smem_u32(groups + of_dims * 256), 1024u, peer_address(bar_joined, uint32_t(owner)));
+  } else if (lane >= 8 && lane < 10) {
+    const int peer = 2 * warp + lane - 8;
+    if (peer < ctas) {
+      copy_to_peer(peer_address(smem_u32(&s.row[rank][0]), uint32_t(peer)), smem_u32(&s.mine[0]),
+                   uint32_t(sizeof(s.mine)), peer_address(bar_joined, uint32_t(peer)));
     }
   }
-  cluster_arrive();
-  cluster_wait();
+  __syncwarp();
+  ok = __all_sync(0xffffffffu, few_wait(bar_joined, 0));
+  cluster_arrive();  // (what this CTA has sent may be read until all have theirs)
   // ---- joined: out = sum 2^(m_k - M) O_k / sum 2^(m_k - M) l_k
-  if (row >= rows) return;
-  const int token = div.group.quotient(row);
-  const int64_t out = (int64_t(run.start) + token) * a.q_heads + head * group + (row - token * group);
-  float top = -INFINITY;
-#pragma unroll 4
-  for (int k = 0; k < ctas; ++k) top = fmaxf(top, s.row[k][row].x);
+  if (ok && row < rows) {
+    float2 ml = make_float2(-INFINITY, 0.0f);  // of CTA `place`
+    if (place < ctas) ml = s.row[place][row];
+    const uint32_t lanes = 0xffffu << (lane & 16);
+    float top = ml.x;
+#pragma unroll
+    for (int d = 8; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(lanes, top, d));
+    // (a CTA without a visible key has zeros; one that saw only NaN has a NaN sum)
+    const float f = ml.y == 0.0f ? 0.0f : ex2_approx(ml.x == -INFINITY ? 0.0f : ml.x - top);
+    float sum = f * ml.y;
+#pragma unroll
+    for (int d = 8; d > 0; d /= 2) sum += __shfl_xor_sync(lanes, sum, d);
+    s.factor[row][place] = f * (sum != 0.0f ? 1.0f / sum : 0.0f);
+    __syncwarp(lanes);
+    const int token = div.group.quotient(row);
+    const int64_t out = (int64_t(run.start) + token) * a.q_heads + head * group + (row - token * group);
 #pragma unroll 1
-  for (int slot = 0; slot < slots; ++slot) {
-    const int of_dims = slot * ctas + rank;
-    if (of_dims >= T::kGroups) break;
-    float sum = 0.0f, acc = 0.0f;
+    for (int slot = 0; slot < slots; ++slot) {
+      float acc = 0.0f;
 #pragma unroll 4
-    for (int k = 0; k < ctas; ++k) {
-      const float2 ml = s.row[k][row];
-      // (a CTA without a visible key has zeros; one that saw only NaN has a NaN sum)
-      const float f = ml.y == 0.0f ? 0.0f : ex2_approx(ml.x == -INFINITY ? 0.0f : ml.x - top);
-      sum = fmaf(f, ml.y, sum);
-      acc = fmaf(f, s.sent[((k * slots + slot) * kFewRows + row) * 16 + place], acc);
+      for (int k = 0; k < ctas; ++k) {
+        acc = fmaf(s.factor[row][k], s.sent[((k * slots + slot) * kFewRows + row) * 16 + place], acc);
+      }
+      a.out[out * D + (slot * ctas + rank) * 16 + place] = __float2bfloat16_rn(acc);
     }
-    a.out[out * D + of_dims * 16 + place] = __float2bfloat16_rn(acc * (sum != 0.0f ? 1.0f / sum : 0.0f));
-    if (a.lse != nullptr && of_dims == 0 && place == 0) {
+    if (a.lse != nullptr && rank == 0 && place == 0) {
       a.lse[out] = sum != 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
     }
   }
+  if (!ok) set_status(a.status, B200KV_STATUS_WAIT_TIMEOUT);
+  __syncwarp();
+  cluster_wait();
 }
 
 struct FewLaunch {
@@ -469,6 +530,8 @@ cudaError_t clusters_at_once(int device, int cluster, int *count) {
 
 template <int D>
 cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cudaStream_t stream, bool *taken) {
+  const int box = box_tokens(a.cfg.page_size, kFewUnit);
+  if (box == 0) return cudaSuccess;
   const int64_t items = int64_t(a.runs.run_count) * a.cfg.num_heads;
   const int64_t most = a.window > 0 ? int64_t(a.window) + a.sinks : table_end;  // keys of a row
   int cluster = kFewMaxCluster;
@@ -481,10 +544,18 @@ cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cuda
   }
   if (most > 512 * int64_t(cluster)) return cudaSuccess;
   *taken = true;
+  CUtensorMap map_k = {}, map_v = {}, map_k_rows = {}, map_v_rows = {};
+  if (!make_cache_map(&map_k, a.cache_k, a.cfg, box) || !make_cache_map(&map_v, a.cache_v, a.cfg, box) ||
+      (a.k_rows != nullptr &&
+       (!make_rows_map(&map_k_rows, a.k_rows, a.runs.rows, a.cfg.num_heads, D) ||
+        !make_rows_map(&map_v_rows, a.v_rows, a.runs.rows, a.cfg.num_heads, D)))) {
+    return cudaErrorInvalidValue;
+  }
   const FewLaunch launch(cluster, a.cfg.num_heads, a.runs.run_count, int(sizeof(FewShared<D>)), stream);
   const FewDivs div = {FastDiv::by(uint32_t(a.cfg.page_size)), FastDiv::by(uint32_t(a.cfg.max_pages_per_seq)),
                        FastDiv::by(uint32_t(a.q_heads / a.cfg.num_heads)), FastDiv::by(uint32_t(cluster))};
-  return cudaLaunchKernelEx(&launch.config, chunk_attention_few_kernel<D>, a, table_end, div);
+  return cudaLaunchKernelEx(&launch.config, chunk_attention_few_kernel<D>, a, map_k, map_v, map_k_rows, map_v_rows,
+                            table_end, box, div);
 }
 
 }  // namespace
