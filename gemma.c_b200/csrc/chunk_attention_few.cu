@@ -14,9 +14,9 @@
 //   softmax       16 threads to a row: running maximum and sum in fp32, the weights
 //                 rounded to bf16 for P V (by at most 2^-8 of each), summed unrounded
 //   O = a O + P V an eighth of the output dims each, fp32 in registers
-// At the end every CTA sends each other one its share of the output dims, with maxima
-// and sums, by bulk copies between their shared memories; a CTA joins and writes its
-// share when those have come. One launch, no partial results in memory. The code is kept small:
+// At the end every CTA stores in each other one's shared memory what that joins: its
+// share of the output dims, with maxima and sums. A CTA joins and writes its share when
+// those have come, and waits for nobody to end. One launch, no partial results in memory. The code is kept small:
 // a call runs most of it once, and fetching it is part of what that takes.
 #include <algorithm>
 #include <atomic>
@@ -51,14 +51,13 @@ struct FewTraits {
 template <int D>
 struct FewShared {
   using T = FewTraits<D>;
-  uint8_t tile[kFewStages][2][T::kTileBytes];             // K and V; at the end O, in groups
+  uint8_t tile[kFewStages][2][T::kTileBytes];             // K and V
   float part[T::kDimParts][kFewRows][T::kPartPitch];      // scores
   uint8_t weights[kFewRows][T::kKeys * 2 + 16];           // bf16
   float alpha[kFewRows];                                  // what O is rescaled by
   uint16_t alive[kFewStages][4];  // keys of the tile's units that some row sees
   uint64_t full[kFewStages];      // the tile has landed
-  uint64_t joined;                // what the cluster's CTAs send has landed
-  alignas(16) float2 mine[kFewRows];                 // maximum and sum that this CTA has of the rows
+  uint64_t joined;                // what the cluster's warps send has landed
   float factor[kFewRows][kFewMaxCluster];  // what a CTA's O counts for in the row
   // What the cluster's CTAs send here: maximum and sum of [rank][row], and [rank][n][row]
   // 16 dims of this CTA's n-th group.
@@ -131,7 +130,7 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void cluster_arrive() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -142,12 +141,24 @@ __device__ __forceinline__ uint32_t peer_address(uint32_t at, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
   return r;
 }
-// Shared memory to that of another CTA, counted on a barrier there.
-__device__ __forceinline__ void copy_to_peer(uint32_t to, uint32_t from, uint32_t bytes, uint32_t bar) {
+__device__ __forceinline__ void store_peer(uint32_t at, float x, float y) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(x), "f"(y) : "memory");
+}
+__device__ __forceinline__ void arrive_at_peer(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool try_wait_for_peers(uint32_t bar) {
+  uint32_t done;
   asm volatile(
-      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to),
-      "r"(from), "r"(bytes), "r"(bar)
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar)
       : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 __device__ __forceinline__ bool few_wait(uint32_t bar, uint32_t parity) {
   for (uint32_t left = kFewPolls; !mbar_try_wait(bar, parity); --left) {
@@ -180,16 +191,24 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
   const int slots = div.ctas.quotient(T::kGroups + ctas - 1 - rank);
   if (tid == 0) {
     for (int i = 0; i < kFewStages; ++i) mbar_init(bar_full + 8u * i, kFewWarps);
-    mbar_init(bar_joined, 1);
+    mbar_init(bar_joined, uint32_t(ctas * kFewWarps));
     mbar_fence_init();
-    mbar_arrive_expect_tx(bar_joined, uint32_t(ctas * (slots * 1024 + int(sizeof(s.mine)))));
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
+    if (a.k_rows != nullptr) {
+      prefetch_map(&map_k_rows);
+      prefetch_map(&map_v_rows);
+    }
   }
   __syncthreads();
+  cluster_arrive();  // (its CTAs must have started before they are written to)
   pdl_wait_for_predecessor();
   pdl_release_successor();
   const ChunkRun run = chunk_run(a.runs, int(blockIdx.z), c.batch_size);
-  if (run.count == 0) return;  // the whole cluster
-  cluster_arrive();            // (its CTAs must have started before they are written to)
+  if (run.count == 0) {  // the whole cluster
+    cluster_wait();
+    return;
+  }
   const int rows = run.count * group;
   const FewKeys keys = few_keys(a, run, table_end);
   const int total = keys.count();
@@ -206,23 +225,25 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
   const int block0 = (warp >> 1) / T::kUnits * (kBoxDims / 64);  // head_dim 512: dims from 256 on
   const int page_groups = c.page_size / 8;
   int token_group = -1;  // cache: group of eight tokens; -1: none
+  auto look_up = [&](int j) {
+    token_group = -1;
+    const int ask = j * T::kUnits + my_unit + (lane >> 1) * T::kUnits;
+    bool own;
+    const int at = keys.base(unit0 + ask, own) + 8 * (lane & 1);
+    if (ask < units && !own && at < keys.cache_end) {
+      const int logical = div.page.quotient(at);
+      const int slot = c.window_size > 0 ? logical - div.slots.quotient(logical) * c.max_pages_per_seq : logical;
+      const int page = __ldg(a.page_table + int64_t(run.batch) * c.max_pages_per_seq + slot);
+      if (page >= 0 && page < c.num_pages) {
+        token_group = (a.layer * c.num_pages + page) * page_groups + ((at - logical * c.page_size) >> 3);
+      }
+    }
+  };
+  look_up(0);
   auto issue = [&](int j) {
     if (j >= tiles) return;
     const int unit = j * T::kUnits + my_unit;
-    if ((j & 15) == 0) {
-      token_group = -1;
-      const int ask = unit + (lane >> 1) * T::kUnits;
-      bool own;
-      const int at = keys.base(unit0 + ask, own) + 8 * (lane & 1);
-      if (ask < units && !own && at < keys.cache_end) {
-        const int logical = div.page.quotient(at);
-        const int slot = c.window_size > 0 ? logical - div.slots.quotient(logical) * c.max_pages_per_seq : logical;
-        const int page = __ldg(a.page_table + int64_t(run.batch) * c.max_pages_per_seq + slot);
-        if (page >= 0 && page < c.num_pages) {
-          token_group = (a.layer * c.num_pages + page) * page_groups + ((at - logical * c.page_size) >> 3);
-        }
-      }
-    }
+    if (j > 0 && (j & 15) == 0) look_up(j);
     // the keys of the unit that some row sees
     bool own;
     const int base = keys.base(unit0 + unit, own);
@@ -253,8 +274,6 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
     }
     __syncwarp();
   };
-  issue(0);
-
   // ---- Q: the A operand for this warp's 128 dims (rows behind the last: zeros)
   const int key16 = (warp % T::kUnits) * 16, dim_part = warp / T::kUnits;
   const int g = lane >> 2, t2 = (lane & 3) * 2;
@@ -271,6 +290,8 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
       q[k][h + 2] = row < rows ? __ldg(reinterpret_cast<const uint32_t *>(from + 16 * k + 8)) : 0u;
     }
   }
+
+  issue(0);
 
   // ---- this thread's row and keys of the softmax
   constexpr int kMine = T::kKeys / 16;
@@ -417,35 +438,27 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
   // ---- to the CTAs that join the dims: a group is 16 rows x 16 dims
 #pragma unroll
   for (int d = 8; d > 0; d /= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
-  if (place == 0) s.mine[row] = make_float2(m, l);
-  float *groups = reinterpret_cast<float *>(&s.tile[0][0][0]);
-#pragma unroll
-  for (int n = 0; n < T::kOut / 8; ++n) {
-    float *to = groups + (warp * (T::kOut / 16) + n / 2) * 256 + g * 16 + 8 * (n & 1) + t2;
-    *reinterpret_cast<float2 *>(to) = make_float2(o[n][0], o[n][1]);
-    *reinterpret_cast<float2 *>(to + 128) = make_float2(o[n][2], o[n][3]);
-  }
-  fence_proxy_async_shared();
-  __syncthreads();
   cluster_wait();
-  // (a copy costs its warp its time: a few to each)
-  if (lane < T::kOut / 16) {
-    const int of_dims = warp * (T::kOut / 16) + lane;
+  if (place < ctas) store_peer(peer_address(smem_u32(&s.row[rank][row]), uint32_t(place)), m, l);
+#pragma unroll
+  for (int n = 0; n < T::kOut / 16; ++n) {
+    const int of_dims = warp * (T::kOut / 16) + n;
     const int slot = div.ctas.quotient(of_dims);
     const int owner = of_dims - slot * ctas;
     const int theirs = div.ctas.quotient(T::kGroups + ctas - 1 - owner);
-    copy_to_peer(peer_address(smem_u32(&s.sent[(rank * theirs + slot) * 256]), uint32_t(owner)),
-                 smem_u32(groups + of_dims * 256), 1024u, peer_address(bar_joined, uint32_t(owner)));
-  } else if (lane >= 8 && lane < 10) {
-    const int peer = 2 * warp + lane - 8;
-    if (peer < ctas) {
-      copy_to_peer(peer_address(smem_u32(&s.row[rank][0]), uint32_t(peer)), smem_u32(&s.mine[0]),
-                   uint32_t(sizeof(s.mine)), peer_address(bar_joined, uint32_t(peer)));
+    const uint32_t at = peer_address(smem_u32(&s.sent[(rank * theirs + slot) * 256 + g * 16 + t2]), uint32_t(owner));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      store_peer(at + 32u * uint32_t(h), o[2 * n + h][0], o[2 * n + h][1]);
+      store_peer(at + 32u * uint32_t(h) + 512u, o[2 * n + h][2], o[2 * n + h][3]);
     }
   }
   __syncwarp();
-  ok = __all_sync(0xffffffffu, few_wait(bar_joined, 0));
-  cluster_arrive();  // (what this CTA has sent may be read until all have theirs)
+  if (lane < ctas) arrive_at_peer(peer_address(bar_joined, uint32_t(lane)));
+  // (longer than any wait of a CTA that is to arrive)
+  ok = true;
+  for (uint32_t left = 32 * kFewPolls; ok && !try_wait_for_peers(bar_joined); --left) ok = left > 0;
+  ok = __all_sync(0xffffffffu, ok);
   // ---- joined: out = sum 2^(m_k - M) O_k / sum 2^(m_k - M) l_k
   if (ok && row < rows) {
     float2 ml = make_float2(-INFINITY, 0.0f);  // of CTA `place`
@@ -477,8 +490,6 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
     }
   }
   if (!ok) set_status(a.status, B200KV_STATUS_WAIT_TIMEOUT);
-  __syncwarp();
-  cluster_wait();
 }
 
 struct FewLaunch {

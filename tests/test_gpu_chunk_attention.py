@@ -48,6 +48,28 @@ CASES = {
     "sinks_own_rows": dict(counts=[150, 33], firsts=[700, 20], window=100, sinks=30, free_middle=True, own_rows=True),
     "hole": dict(counts=[40], firsts=[200], unmap=[(0, 3), (0, 14)]),
     "no_key_at_all": dict(counts=[2, 5], firsts=[14, 100], unmap=[(0, 0)]),
+    # few rows of few sequences (a kernel of their own)
+    "few_ring": dict(counts=[4], firsts=[1500], ring=True, window=1024),
+    "few_ring_runs": dict(counts=[4, 8], firsts=[300, 64], ring=True, window=256),
+    "few_ring_uneven": dict(counts=[8, 1, 3], firsts=[1000, 0, 250], ring=True, window=250, page=8, gap=1),
+    "few_slack": dict(counts=[5], firsts=[777], ring=True, window=200, page=8, ring_slots=30, own_rows=False),
+    "few_linear": dict(counts=[7], firsts=[1333]),
+    "few_page24": dict(counts=[3, 2], firsts=[131, 700], page=24),
+    "few_page64": dict(counts=[8], firsts=[1190], page=64),
+    "few_page200": dict(counts=[6], firsts=[1190], page=200),
+    "few_sinks": dict(counts=[1], firsts=[3000], window=500, sinks=4, free_middle=True),
+    "few_sinks_own": dict(counts=[8], firsts=[700], window=100, sinks=37, free_middle=True, own_rows=True),
+    "few_window_inside_run": dict(counts=[8], firsts=[40], window=3),
+    "few_hole": dict(counts=[5], firsts=[300], unmap=[(0, 2), (0, 3), (0, 18)]),
+    "few_no_key": dict(counts=[3], firsts=[12], unmap=[(0, 0)]),
+    "few_group16": dict(counts=[1], firsts=[900], heads=2, group=16),
+    "few_group3": dict(counts=[5], firsts=[200], heads=2, group=3),
+    "few_group1": dict(counts=[16], firsts=[350], heads=3, group=1),
+    "few_512": dict(counts=[1, 1], firsts=[2000, 5], heads=1, group=16, dim=512, page=64),
+    "few_512_tokens": dict(counts=[5], firsts=[900], heads=4, group=2, dim=512, page=8),
+    "few_512_ring": dict(counts=[7, 8], firsts=[1000, 40], heads=1, group=2, dim=512, ring=True, window=512),
+    "few_layer": dict(counts=[3], firsts=[200], layers=3, layer=2),
+    "few_peaked": dict(counts=[8], firsts=[900], q_scale=30.0),
     "peaked": dict(counts=[64, 3], firsts=[500, 800], q_scale=30.0),
 }
 
@@ -75,6 +97,16 @@ def test_runs_that_make_no_sense_are_skipped(kv):
     case.first[2] = -1
     case.count[3] = 0
     case.start[4] = case.rows - 3
+    a, t = device_args(kv, case)
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+
+
+def test_few_rows_of_runs_that_make_no_sense_are_skipped(kv):
+    case = make_case(6, [5, 6, 7], [50, 60, 70], gap=1)
+    case.seq[1] = 3          # not a sequence
+    case.count[2] = 0
     a, t = device_args(kv, case)
     kv.chunk_attention(a)
     torch.cuda.synchronize()
@@ -156,7 +188,7 @@ def test_rows_of_no_run_are_not_used(kv):
 
 
 @pytest.mark.parametrize("where", ["cache_k", "cache_v"])
-@pytest.mark.parametrize("first", [40, 4000])            # one CTA has the item; several share it
+@pytest.mark.parametrize("first", [40, 4000, 40000])      # few keys to a cluster's CTA, many; one launch more
 def test_a_nan_that_a_row_sees_is_in_its_result(kv, where, first):
     case = make_case(14, [3], [first])
     page = int(case.table[0, 1])                         # position 20
