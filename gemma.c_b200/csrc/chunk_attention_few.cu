@@ -16,8 +16,16 @@
 //   O = a O + P V an eighth of the output dims each, fp32 in registers
 // At the end every CTA stores in each other one's shared memory what that joins: its
 // share of the output dims, with maxima and sums. A CTA joins and writes its share when
-// those have come, and waits for nobody to end. One launch, no partial results in memory. The code is kept small:
-// a call runs most of it once, and fetching it is part of what that takes.
+// those have come, and waits for nobody to end. One launch, no partial results in memory.
+//
+// Latency bounds it. Measured, four tokens of 16 + 8 heads of 256 over a ring of 1024 (4
+// MB of K and V, 1.3 us of HBM): 7.5 us of the GPU in a row of calls, 15.2 by the other
+// kernel and its join; one token over 100 keys 6.0. Of the way (80 CTAs, 2 tiles each) in
+// clocks: the runs 800, what follows from them 1100, page and first tile 1800, a tile
+// 1500 (of which the first is fetching code), sending and joining 2000. Earlier forms: a
+// copy of 16 bytes per lane instead of boxes 10.1 us (64 CTAs), a bulk copy per row 8.1,
+// all of the rows' copies from one warp 14.2, a softmax in every warp for itself 10.7
+// (twice the code). The code is kept small: a call runs most of it once.
 #include <algorithm>
 #include <atomic>
 
@@ -547,13 +555,19 @@ cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cuda
   const int64_t most = a.window > 0 ? int64_t(a.window) + a.sinks : table_end;  // keys of a row
   int cluster = kFewMaxCluster;
   for (;; --cluster) {  // the largest that all run at once
-    if (cluster < 4) return cudaSuccess;
+    if (cluster < 2) return cudaSuccess;
     int at_once = 0;
     const cudaError_t st = clusters_at_once<D>(device, cluster, &at_once);
     if (st != cudaSuccess) return st;
     if (items <= at_once) break;
   }
-  if (most > 512 * int64_t(cluster)) return cudaSuccess;
+  // What the host knows of the lengths is the most that a row can see. Beyond 640 keys of
+  // 256 dims to a CTA the even cut over all SMs is worth its second launch. Eight heads of
+  // 256, GPU time here / there: one sequence of 500, 4000, 8000 keys 6.4 / 14.1, 13.4 /
+  // 17.0, 20.7 / 19.9 us; two of 4000 18.3 / 18.8, four of 2000 14.5 / 18.9, eight of 500
+  // 9.6 / 21.8; one of 16 heads of 512 on one KV head over 2000, 8000 10.5 / 16.4, 23.9 /
+  // 20.6. Where the lengths differ the longest counts here: four of 100 .. 4000 24.0 / 19.1.
+  if (most * D > 640 * 256 * int64_t(cluster)) return cudaSuccess;
   *taken = true;
   CUtensorMap map_k = {}, map_v = {}, map_k_rows = {}, map_v_rows = {};
   if (!make_cache_map(&map_k, a.cache_k, a.cfg, box) || !make_cache_map(&map_v, a.cache_v, a.cfg, box) ||

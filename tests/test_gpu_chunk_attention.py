@@ -68,6 +68,8 @@ CASES = {
     "few_512": dict(counts=[1, 1], firsts=[2000, 5], heads=1, group=16, dim=512, page=64),
     "few_512_tokens": dict(counts=[5], firsts=[900], heads=4, group=2, dim=512, page=8),
     "few_512_ring": dict(counts=[7, 8], firsts=[1000, 40], heads=1, group=2, dim=512, ring=True, window=512),
+    "few_many": dict(counts=[1 + 3 * i % 8 for i in range(8)], firsts=[(i * 331) % 1200 for i in range(8)], gap=1),
+    "few_many_512": dict(counts=[1] * 12, firsts=[(i * 331) % 1500 for i in range(12)], heads=2, group=8, dim=512, page=16),
     "few_layer": dict(counts=[3], firsts=[200], layers=3, layer=2),
     "few_peaked": dict(counts=[8], firsts=[900], q_scale=30.0),
     "peaked": dict(counts=[64, 3], firsts=[500, 800], q_scale=30.0),
