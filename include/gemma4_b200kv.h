@@ -668,10 +668,15 @@ int b200kv_chunk_append_bf16(const B200KvChunkArgs *args, b200kv_stream stream);
  * the same and sink_tokens 0. For a linear cache window_size (0: none) and
  * sink_tokens (0: none; needs a window) choose it; pages between the sinks and
  * the first row's window may be given back (-1 in the page table). A row that
- * sees no key gets zeros and an lse of -inf. Values at positions that no row of
- * the call sees are not used, whatever they hold. head_dim 256 or 512, any
- * number G of query heads per KV head up to 64; run_count *
- * ceil(max_row_count / floor(128 / G)) <= 2^24.
+ * sees no key gets zeros and an lse of -inf. Keys past a linear cache's table do
+ * not exist. Values at positions that no row of the call sees are not used,
+ * whatever they hold; a NaN or an infinity in V at a position that a later row of
+ * the same run sees may reach earlier rows of it too (as 0 * NaN). head_dim 256 or
+ * 512, any number G of query heads per KV head up to 64. With P = run_count *
+ * ceil(min(max_row_count, rows) / floor(128 / G)) query tiles: P <= 2^24 and
+ * P * kv_heads * (head_dim / 256) * (keys / 64 + 16) < 2^31, keys being the most
+ * that a row can see (the window, or the table's positions) and, with k_rows,
+ * max_row_count; larger calls are refused.
  * `workspace` holds the partial results of rows whose keys several CTAs share;
  * it need not be cleared and nothing is kept in it between calls; calls that may
  * overlap on the GPU (two streams, two captured graphs) need one each. */
