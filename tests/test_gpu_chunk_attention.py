@@ -162,6 +162,31 @@ def test_a_replayed_call_reads_the_lengths_of_the_moment(kv):
     check_attention(case, t)
 
 
+@pytest.mark.parametrize("over", [dict(ring=True, window=256), dict(heads=1, group=8, dim=512), dict()])
+def test_few_rows_captured_and_replayed(kv, over):
+    """The small call's kernel in a graph, between eager calls on the same and on another stream; lengths change."""
+    case = make_case(19, [2, 1], [700, 90], **over)
+    case.count[:], case.first[:] = [1, 1], [650, 60]
+    (a, t), (b, tb) = device_args(kv, case), device_args(kv, case)
+    a.max_row_count = b.max_row_count = 2
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            kv.chunk_attention(b, stream=torch.cuda.current_stream())
+    case.count[:], case.first[:] = [2, 1], [700, 90]
+    for x in (t, tb):
+        x["row_count"].copy_(torch.from_numpy(case.count))
+        x["first_position"].copy_(torch.from_numpy(case.first))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        graph.replay()
+        kv.chunk_attention(a, stream=side)
+        kv.chunk_attention(a, stream=side)
+    torch.cuda.synchronize()
+    assert torch.equal(t["out"], tb["out"]) and torch.equal(t["lse"], tb["lse"])
+    check_attention(case, t)
+
+
 @pytest.mark.parametrize("page,own", [(16, True), (64, True), (64, False), (5, True)])
 def test_the_last_positions_there_are(kv, page, own):
     """A ring at the end of the positions: nothing beyond them is looked up."""
