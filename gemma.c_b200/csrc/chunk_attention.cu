@@ -69,7 +69,10 @@
 // out of line and rolled MMA and epilogue loops (6000 to 4500 instructions) made the tile
 // a quarter faster; four more warps for the epilogue, an epilogue put off until the next
 // item's first tile (more registers and code), and for head_dim 512 both groups on every
-// tile (448k clocks instead of 430k) did not pay.
+// tile (448k clocks instead of 430k) did not pay. Nor did, for head_dim 512, two CTAs with
+// half of the dims each that send one another their part of the scores: 1024 clocks of
+// MMAs a tile instead of 1792 and a third less from L2, but 32 KB of scores a tile and
+// CTA between shared memories took 4400 (390 us instead of 250).
 #include <algorithm>
 
 #include "chunk_common.cuh"
