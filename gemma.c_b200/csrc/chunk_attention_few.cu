@@ -521,30 +521,22 @@ struct FewLaunch {
 // Clusters of this size that the device runs at once: they lie within a group of SMs,
 // and the groups differ (148 SMs: 7 of 16 or 11, 11 of 10, 15 of 8, 33 of 4).
 template <int D>
-cudaError_t clusters_at_once(int device, int cluster, int *count) {
+int clusters_at_once(int device, int cluster) {
   constexpr int kDevices = 64;
   static std::atomic<int> known[kDevices][kFewMaxCluster + 1];  // 0: not asked yet
   if (device < kDevices) {
     const int n = known[device][cluster].load(std::memory_order_relaxed);
-    if (n > 0) {
-      *count = n - 1;
-      return cudaSuccess;
-    }
+    if (n > 0) return n - 1;
   }
-  constexpr int kSmem = int(sizeof(FewShared<D>));
-  static_assert(kSmem <= 227 * 1024, "the tiles must fit one SM");
-  const auto kernel = chunk_attention_few_kernel<D>;
-  cudaError_t st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  if (st == cudaSuccess) st = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (st != cudaSuccess) return st;
-  FewLaunch launch(cluster, 1, 1, kSmem, nullptr);
+  FewLaunch launch(cluster, 1, 1, int(sizeof(FewShared<D>)), nullptr);
   launch.config.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(count, kernel, &launch.config) != cudaSuccess) {
+  int count = 0;
+  if (cudaOccupancyMaxActiveClusters(&count, chunk_attention_few_kernel<D>, &launch.config) != cudaSuccess) {
     cudaGetLastError();
-    *count = 0;  // not a size for this device
+    count = 0;  // not a size for this device
   }
-  if (device < kDevices) known[device][cluster].store(*count + 1, std::memory_order_relaxed);
-  return cudaSuccess;
+  if (device < kDevices) known[device][cluster].store(count + 1, std::memory_order_relaxed);
+  return count;
 }
 
 template <int D>
@@ -553,14 +545,15 @@ cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cuda
   if (box == 0) return cudaSuccess;
   const int64_t items = int64_t(a.runs.run_count) * a.cfg.num_heads;
   const int64_t most = a.window > 0 ? int64_t(a.window) + a.sinks : table_end;  // keys of a row
-  int cluster = kFewMaxCluster;
-  for (;; --cluster) {  // the largest that all run at once
-    if (cluster < 2) return cudaSuccess;
-    int at_once = 0;
-    const cudaError_t st = clusters_at_once<D>(device, cluster, &at_once);
-    if (st != cudaSuccess) return st;
-    if (items <= at_once) break;
-  }
+  constexpr int kSmem = int(sizeof(FewShared<D>));
+  static_assert(kSmem <= 227 * 1024, "the tiles must fit one SM");
+  const auto kernel = chunk_attention_few_kernel<D>;
+  cudaError_t st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (st == cudaSuccess) st = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (st != cudaSuccess) return st;
+  int cluster = kFewMaxCluster;  // the largest of which all run at once
+  while (cluster >= 2 && items > clusters_at_once<D>(device, cluster)) --cluster;
+  if (cluster < 2) return cudaSuccess;
   // What the host knows of the lengths is the most that a row can see. Beyond 640 keys of
   // 256 dims to a CTA the even cut over all SMs is worth its second launch. Eight heads of
   // 256, GPU time here / there: one sequence of 500, 4000, 8000 keys 6.4 / 14.1, 13.4 /
@@ -576,10 +569,10 @@ cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cuda
         !make_rows_map(&map_v_rows, a.v_rows, a.runs.rows, a.cfg.num_heads, D)))) {
     return cudaErrorInvalidValue;
   }
-  const FewLaunch launch(cluster, a.cfg.num_heads, a.runs.run_count, int(sizeof(FewShared<D>)), stream);
+  const FewLaunch launch(cluster, a.cfg.num_heads, a.runs.run_count, kSmem, stream);
   const FewDivs div = {FastDiv::by(uint32_t(a.cfg.page_size)), FastDiv::by(uint32_t(a.cfg.max_pages_per_seq)),
                        FastDiv::by(uint32_t(a.q_heads / a.cfg.num_heads)), FastDiv::by(uint32_t(cluster))};
-  return cudaLaunchKernelEx(&launch.config, chunk_attention_few_kernel<D>, a, map_k, map_v, map_k_rows, map_v_rows,
+  return cudaLaunchKernelEx(&launch.config, kernel, a, map_k, map_v, map_k_rows, map_v_rows,
                             table_end, box, div);
 }
 
