@@ -1,10 +1,10 @@
-// Attention of runs with few query rows (a token, the drafted tokens of a
-// speculative step) over few sequences: the same definition as chunk_attention.cu,
-// for calls so small that the way through a call is what it costs.
+// Attention of small calls (a token, the drafted tokens of a speculative step, a short
+// chunk over a short cache): the same definition as chunk_attention.cu, for calls whose
+// way is what they cost.
 //
-// All rows of a run (tokens x the G query heads of a KV head, at most 16) are the 16
-// rows of the warp-level products (mma.sync m16n8k16): tcgen05 would spend its 128
-// rows, its tensor memory and its barriers on them. A cluster of CTAs takes one (run,
+// A query tile is 16 rows, tokens x the G query heads of a KV head: the rows of the
+// warp-level products (mma.sync m16n8k16). tcgen05 would spend 128 rows, its tensor
+// memory and its barriers on them. A cluster of CTAs takes one (query tile,
 // KV head) and each of its CTAs an even share of the keys in units of 16, a tile of 64
 // (head_dim 512: 32) at a time, brought by TMA a tile ahead: each of the eight warps asks
 // for one unit of K or V (head_dim 512: half of one), in a box or two that lie in a page,
@@ -78,38 +78,45 @@ struct FewDivs {
   FastDiv slots;  // by max_pages_per_seq
   FastDiv group;  // by the query heads of a KV head
   FastDiv ctas;   // by the cluster's size
+  FastDiv tiles;  // by the query tiles of the longest run
 };
 
-// The units of 16 keys of a run, in this order: of the cache [0, ca) (sinks) and [cb0,
-// cb1), of the run's own rows [0, oa). Their positions ascend.
+// The units of 16 keys of a query tile, in this order: of the cache [0, ca) (sinks) and
+// [cb0, cb1), of the run's own rows [0, oa) (sinks) and [ob0, ob1). Positions ascend.
 struct FewKeys {
-  int ca, cb0, cb1, oa;
+  int ca, cb0, cb1, oa, ob0, ob1;
   int lo, cache_end, first;
-  __device__ __forceinline__ int count() const { return ca + (cb1 - cb0) + oa; }
+  __device__ __forceinline__ int count() const { return ca + (cb1 - cb0) + oa + (ob1 - ob0); }
   // position of the first key of unit j
   __device__ __forceinline__ int base(int j, bool &own) const {
     own = false;
     if (j < ca) return j * kFewUnit;
     j -= ca;
     if (j < cb1 - cb0) return (cb0 + j) * kFewUnit;
+    j -= cb1 - cb0;
     own = true;
-    return first + (j - (cb1 - cb0)) * kFewUnit;
+    return first + (j < oa ? j : ob0 + j - oa) * kFewUnit;
   }
 };
 
-__device__ __forceinline__ FewKeys few_keys(const ChunkAttentionArgs &a, const ChunkRun &run, int table_end) {
+// Of the rows at positions t0 .. t1.
+__device__ __forceinline__ FewKeys few_keys(const ChunkAttentionArgs &a, int first, int t0, int t1, int table_end) {
   FewKeys k = {};
-  const int end = run.first + run.count;
-  k.first = run.first;
-  k.lo = a.window > 0 ? max(0, run.first - a.window + 1) : 0;
-  k.cache_end = min(a.k_rows != nullptr ? run.first : end, table_end);
-  k.ca = div_up(min(min(a.sinks, k.lo), k.cache_end), kFewUnit);
+  k.first = first;
+  k.lo = a.window > 0 ? max(0, t0 - a.window + 1) : 0;
+  k.cache_end = min(a.k_rows != nullptr ? first : t1 + 1, table_end);
+  const int sink_end = min(a.sinks, k.lo);
+  k.ca = div_up(min(sink_end, k.cache_end), kFewUnit);
   if (k.cache_end > k.lo) {
     k.cb0 = k.lo / kFewUnit;
     k.cb1 = div_up(k.cache_end, kFewUnit);
     k.ca = min(k.ca, k.cb0);
   }
-  if (a.k_rows != nullptr) k.oa = div_up(run.count, kFewUnit);  // (all in the first row's window)
+  if (a.k_rows != nullptr) {
+    k.ob0 = max(k.lo - first, 0) / kFewUnit;
+    k.ob1 = (t1 - first) / kFewUnit + 1;
+    k.oa = sink_end > first ? min(div_up(sink_end - first, kFewUnit), k.ob0) : 0;
+  }
   return k;
 }
 
@@ -175,7 +182,7 @@ __device__ __forceinline__ bool few_wait(uint32_t bar, uint32_t parity) {
   return true;
 }
 
-// grid (CTAs of a cluster, KV heads, runs)
+// grid (CTAs of a cluster, KV heads, query tiles of the runs)
 template <int D>
 __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
     const __grid_constant__ ChunkAttentionArgs a, const __grid_constant__ CUtensorMap map_k,
@@ -212,13 +219,18 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
   cluster_arrive();  // (its CTAs must have started before they are written to)
   pdl_wait_for_predecessor();
   pdl_release_successor();
-  const ChunkRun run = chunk_run(a.runs, int(blockIdx.z), c.batch_size);
-  if (run.count == 0) {  // the whole cluster
+  const int of_run = div.tiles.quotient(int(blockIdx.z));
+  const ChunkRun run = chunk_run(a.runs, of_run, c.batch_size);
+  const int token0 = (int(blockIdx.z) - of_run * int(div.tiles.d)) * div.group.quotient(kFewRows);
+  if (token0 >= run.count) {  // the whole cluster
     cluster_wait();
     return;
   }
-  const int rows = run.count * group;
-  const FewKeys keys = few_keys(a, run, table_end);
+  const int tokens = min(div.group.quotient(kFewRows), run.count - token0);
+  const int rows = tokens * group;
+  const int t0 = run.first + token0, t1 = t0 + tokens - 1;
+  const int64_t row0 = int64_t(run.start) + token0;  // packed row of the first token
+  const FewKeys keys = few_keys(a, run.first, t0, t1, table_end);
   const int total = keys.count();
   const int even = div.ctas.quotient(total);
   const int rest = total - even * ctas;  // the first CTAs have one more
@@ -256,8 +268,8 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
     bool own;
     const int base = keys.base(unit0 + unit, own);
     uint32_t alive = unit >= units ? 0u
-                     : own         ? low16(run.first + run.count - base)
-                                   : low16(keys.cache_end - base) & (~low16(keys.lo - base) | low16(a.sinks - base));
+                                   : low16((own ? t1 + 1 : keys.cache_end) - base) &
+                                         (~low16(keys.lo - base) | low16(a.sinks - base));
     const int group0 = __shfl_sync(0xffffffffu, token_group, 2 * (j & 15));
     const int group1 = __shfl_sync(0xffffffffu, token_group, 2 * (j & 15) + 1);
     if (!own) alive &= (group0 >= 0 ? 0xffu : 0u) | (group1 >= 0 ? 0xff00u : 0u);
@@ -291,7 +303,7 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
     const int row = g + 8 * h;
     const int token = div.group.quotient(row);
     const __nv_bfloat16 *from =
-        a.q + ((int64_t(run.start) + token) * a.q_heads + head * group + (row - token * group)) * D + dim_part * 128 + t2;
+        a.q + ((row0 + token) * a.q_heads + head * group + (row - token * group)) * D + dim_part * 128 + t2;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       q[k][h] = row < rows ? __ldg(reinterpret_cast<const uint32_t *>(from + 16 * k)) : 0u;
@@ -304,7 +316,7 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
   // ---- this thread's row and keys of the softmax
   constexpr int kMine = T::kKeys / 16;
   const int row = tid >> 4, place = tid & 15;
-  const int t = run.first + div.group.quotient(row);
+  const int t = t0 + div.group.quotient(row);
   const float scale = a.softmax_scale * 1.4426950408889634f;
   const int in8 = (lane & 7) + ((lane >> 3) & 1) * 8;  // row that the lane names to ldmatrix
   const uint32_t tile_at = smem_u32(&s.tile[0][0][0]);
@@ -483,7 +495,7 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
     s.factor[row][place] = f * (sum != 0.0f ? 1.0f / sum : 0.0f);
     __syncwarp(lanes);
     const int token = div.group.quotient(row);
-    const int64_t out = (int64_t(run.start) + token) * a.q_heads + head * group + (row - token * group);
+    const int64_t out = (row0 + token) * a.q_heads + head * group + (row - token * group);
 #pragma unroll 1
     for (int slot = 0; slot < slots; ++slot) {
       float acc = 0.0f;
@@ -503,8 +515,8 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
 struct FewLaunch {
   cudaLaunchConfig_t config = {};
   cudaLaunchAttribute attr[2];
-  FewLaunch(int cluster, int heads, int runs, int smem, cudaStream_t stream) {
-    config.gridDim = dim3(unsigned(cluster), unsigned(heads), unsigned(runs));
+  FewLaunch(int cluster, int heads, int tiles, int smem, cudaStream_t stream) {
+    config.gridDim = dim3(unsigned(cluster), unsigned(heads), unsigned(tiles));
     config.blockDim = dim3(kFewWarps * 32);
     config.dynamicSmemBytes = size_t(smem);
     config.stream = stream;
@@ -543,7 +555,9 @@ template <int D>
 cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cudaStream_t stream, bool *taken) {
   const int box = box_tokens(a.cfg.page_size, kFewUnit);
   if (box == 0) return cudaSuccess;
-  const int64_t items = int64_t(a.runs.run_count) * a.cfg.num_heads;
+  const int group = a.q_heads / a.cfg.num_heads;
+  const int tiles = div_up(std::min(a.runs.max_row_count, a.runs.rows), kFewRows / group);  // of a run
+  const int64_t items = int64_t(a.runs.run_count) * a.cfg.num_heads * tiles;
   const int64_t most = a.window > 0 ? int64_t(a.window) + a.sinks : table_end;  // keys of a row
   constexpr int kSmem = int(sizeof(FewShared<D>));
   static_assert(kSmem <= 227 * 1024, "the tiles must fit one SM");
@@ -552,14 +566,17 @@ cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cuda
   if (st == cudaSuccess) st = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (st != cudaSuccess) return st;
   int cluster = kFewMaxCluster;  // the largest of which all run at once
-  while (cluster >= 2 && items > clusters_at_once<D>(device, cluster)) --cluster;
-  if (cluster < 2) return cudaSuccess;
-  // What the host knows of the lengths is the most that a row can see. Beyond 640 keys of
-  // 256 dims to a CTA the even cut over all SMs is worth its second launch. Eight heads of
-  // 256, GPU time here / there: one sequence of 500, 4000, 8000 keys 6.4 / 14.1, 13.4 /
-  // 17.0, 20.7 / 19.9 us; two of 4000 18.3 / 18.8, four of 2000 14.5 / 18.9, eight of 500
-  // 9.6 / 21.8; one of 16 heads of 512 on one KV head over 2000, 8000 10.5 / 16.4, 23.9 /
-  // 20.6. Where the lengths differ the longest counts here: four of 100 .. 4000 24.0 / 19.1.
+  while (cluster >= 1 && items > clusters_at_once<D>(device, cluster)) --cluster;
+  if (cluster < 1) return cudaSuccess;
+  // A tile of 64 keys is 1.2 us here behind some 5.6 of start and end; the other kernel and
+  // its join take 12 to 17 and hardly more for more keys, so up to 640 keys of 256 dims to a
+  // CTA belong here. What the host knows of the lengths is the most that a row can see. GPU
+  // time here / there, eight heads of 256: four tokens of one sequence over 500, 4000, 8000
+  // keys 6.4 / 14.1, 13.4 / 17.0, 20.7 / 19.9 us; of four over 2000 14.5 / 18.9, of eight
+  // over 500 9.6 / 21.8; 40 tokens over 500, 2000 8.6 / 16.9, 18.2 / 18.3; 100 over 50, 500
+  // 8.4 / 16.0, 16.8 / 18.5; 16 tokens of 16 heads of 512 on one KV head over 500, 2000 10.0
+  // / 18.9, 18.8 / 20.3. Where the lengths differ the longest counts here: four tokens of
+  // four sequences over 100 .. 4000 keys 24.0 / 19.1.
   if (most * D > 640 * 256 * int64_t(cluster)) return cudaSuccess;
   *taken = true;
   CUtensorMap map_k = {}, map_v = {}, map_k_rows = {}, map_v_rows = {};
@@ -569,9 +586,10 @@ cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cuda
         !make_rows_map(&map_v_rows, a.v_rows, a.runs.rows, a.cfg.num_heads, D)))) {
     return cudaErrorInvalidValue;
   }
-  const FewLaunch launch(cluster, a.cfg.num_heads, a.runs.run_count, kSmem, stream);
+  const FewLaunch launch(cluster, a.cfg.num_heads, a.runs.run_count * tiles, kSmem, stream);
   const FewDivs div = {FastDiv::by(uint32_t(a.cfg.page_size)), FastDiv::by(uint32_t(a.cfg.max_pages_per_seq)),
-                       FastDiv::by(uint32_t(a.q_heads / a.cfg.num_heads)), FastDiv::by(uint32_t(cluster))};
+                       FastDiv::by(uint32_t(group)), FastDiv::by(uint32_t(cluster)),
+                       FastDiv::by(uint32_t(tiles))};
   return cudaLaunchKernelEx(&launch.config, kernel, a, map_k, map_v, map_k_rows, map_v_rows,
                             table_end, box, div);
 }
@@ -581,8 +599,7 @@ cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cuda
 cudaError_t chunk_attention_few_bf16(const ChunkAttentionArgs &a, int device, int table_end,
                                      cudaStream_t stream, bool *taken) {
   *taken = false;
-  const int group = a.q_heads / a.cfg.num_heads;
-  if (int64_t(std::min(a.runs.max_row_count, a.runs.rows)) * group > kFewRows) return cudaSuccess;
+  if (a.q_heads / a.cfg.num_heads > kFewRows) return cudaSuccess;
   return a.cfg.head_dim == 256 ? try_few<256>(a, device, table_end, stream, taken)
                                : try_few<512>(a, device, table_end, stream, taken);
 }

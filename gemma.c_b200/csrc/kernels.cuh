@@ -331,7 +331,7 @@ struct ChunkAttentionArgs {
 };
 cudaError_t validate_chunk_attention(const ChunkAttentionArgs &args);
 cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &args, cudaStream_t stream);
-// The form for few rows and few sequences (chunk_attention_few.cu); *taken: it was for
+// The form for small calls (chunk_attention_few.cu); *taken: it was for
 // these sizes. table_end: first position past a linear cache's table.
 cudaError_t chunk_attention_few_bf16(const ChunkAttentionArgs &args, int device, int table_end,
                                      cudaStream_t stream, bool *taken);

@@ -48,7 +48,24 @@ CASES = {
     "sinks_own_rows": dict(counts=[150, 33], firsts=[700, 20], window=100, sinks=30, free_middle=True, own_rows=True),
     "hole": dict(counts=[40], firsts=[200], unmap=[(0, 3), (0, 14)]),
     "no_key_at_all": dict(counts=[2, 5], firsts=[14, 100], unmap=[(0, 0)]),
-    # few rows of few sequences (a kernel of their own)
+    # the same geometries in calls that are not small
+    "large_heads1": dict(counts=[1200, 5], firsts=[700, 2000], heads=1),
+    "large_heads4": dict(counts=[310, 2], firsts=[300, 10], heads=4),
+    "large_group1": dict(counts=[310, 3], firsts=[130, 64], heads=4, group=1),
+    "large_group3": dict(counts=[300, 3], firsts=[130, 64], heads=2, group=3),
+    "large_512_two_heads": dict(counts=[650], firsts=[90], heads=2, group=2, dim=512),
+    "large_512_single": dict(counts=[1, 2], firsts=[6000, 5200], heads=1, group=16, dim=512, page=64),
+    "large_512_own": dict(counts=[100, 60], firsts=[6000, 20], heads=1, group=16, dim=512, page=64, own_rows=True),
+    "large_page8": dict(counts=[170, 2], firsts=[131, 100], page=8),
+    "large_page24": dict(counts=[170, 2], firsts=[131, 100], page=24),
+    "large_page64": dict(counts=[170, 2], firsts=[131, 1000], page=64),
+    "large_sinks_single": dict(counts=[1] * 20, firsts=[(i * 97) % 1200 for i in range(20)], window=64, sinks=4,
+                               free_middle=True),
+    "large_ring_single": dict(counts=[1] * 20, firsts=[(i * 97) % 1200 for i in range(20)], ring=True, window=128),
+    "large_hole": dict(counts=[300], firsts=[200], unmap=[(0, 3), (0, 14)]),
+    "large_no_key": dict(counts=[300, 5], firsts=[14, 100], unmap=[(0, 0)]),
+    "large_peaked": dict(counts=[200, 3], firsts=[500, 800], q_scale=30.0),
+    # small calls (a kernel of their own)
     "few_ring": dict(counts=[4], firsts=[1500], ring=True, window=1024),
     "few_ring_runs": dict(counts=[4, 8], firsts=[300, 64], ring=True, window=256),
     "few_ring_uneven": dict(counts=[8, 1, 3], firsts=[1000, 0, 250], ring=True, window=250, page=8, gap=1),
@@ -71,6 +88,19 @@ CASES = {
     "few_many": dict(counts=[1 + 3 * i % 8 for i in range(8)], firsts=[(i * 331) % 1200 for i in range(8)], gap=1),
     "few_many_512": dict(counts=[1] * 12, firsts=[(i * 331) % 1500 for i in range(12)], heads=2, group=8, dim=512, page=16),
     "few_layer": dict(counts=[3], firsts=[200], layers=3, layer=2),
+    # more than one query tile of 16 rows
+    "few_tiles": dict(counts=[40], firsts=[300]),
+    "few_tiles_ring": dict(counts=[61], firsts=[500], ring=True, window=128),
+    "few_tiles_short_window": dict(counts=[70], firsts=[90], ring=True, window=16),
+    "few_tiles_slack": dict(counts=[33, 5], firsts=[400, 10], ring=True, window=64, ring_slots=8, own_rows=False),
+    "few_tiles_own_sinks": dict(counts=[90], firsts=[10], window=20, sinks=37, own_rows=True, heads=2),
+    "few_tiles_sinks": dict(counts=[50], firsts=[333], window=40, sinks=20, free_middle=True, page=8),
+    "few_tiles_uneven": dict(counts=[30, 1, 17], firsts=[0, 200, 64], heads=2, group=3, gap=2),
+    "few_tiles_group16": dict(counts=[9, 3], firsts=[100, 30], heads=2, group=16),
+    "few_tiles_group1": dict(counts=[100], firsts=[200], heads=3, group=1),
+    "few_tiles_512": dict(counts=[20, 3], firsts=[300, 0], heads=1, group=16, dim=512, page=64),
+    "few_tiles_512_own": dict(counts=[24], firsts=[200], heads=2, group=2, dim=512, own_rows=True),
+    "few_tiles_hole": dict(counts=[40], firsts=[120], unmap=[(0, 3), (0, 9)], heads=4),
     "few_peaked": dict(counts=[8], firsts=[900], q_scale=30.0),
     "peaked": dict(counts=[64, 3], firsts=[500, 800], q_scale=30.0),
 }
@@ -187,13 +217,14 @@ def test_few_rows_captured_and_replayed(kv, over):
     check_attention(case, t)
 
 
+@pytest.mark.parametrize("count", [40, 170])
 @pytest.mark.parametrize("page,own", [(16, True), (64, True), (64, False), (5, True)])
-def test_the_last_positions_there_are(kv, page, own):
+def test_the_last_positions_there_are(kv, page, own, count):
     """A ring at the end of the positions: nothing beyond them is looked up."""
     end = 2**31 - 1024
     window = 128 if page != 5 else 125
-    case = make_case(12, [40, 1], [end - 1 - 40, end - 1 - 1], ring=True, window=window, page=page, own_rows=own,
-                     ring_slots=None if own else 4)
+    case = make_case(12, [count, 1], [end - 1 - count, end - 1 - 1], ring=True, window=window, page=page,
+                     own_rows=own, ring_slots=None if own else 5)
     a, t = device_args(kv, case)
     kv.chunk_attention(a)
     torch.cuda.synchronize()
@@ -274,9 +305,10 @@ def test_calls_one_behind_the_other_share_a_workspace(kv):
     check_attention(two, tb)
 
 
-def test_cache_offsets_beyond_32_bits(kv):
+@pytest.mark.parametrize("count", [20, 170])
+def test_cache_offsets_beyond_32_bits(kv, count):
     """A cache of more than 2^32 bytes a tensor: the run's pages are its last ones."""
-    case = make_case(10, [20, 1], [200, 70], page=64)
+    case = make_case(10, [count, 1], [200, 70], page=64)
     a, t = device_args(kv, case)
     page_elems = 64 * 8 * 256
     pages = (1 << 32) // (page_elems * 2) + case.cfg[1] + 7
