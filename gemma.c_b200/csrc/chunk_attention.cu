@@ -747,9 +747,12 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
               page[r] = -1;
               const int at = lane + 32 * r;
               if (((live >> at) & 1ull) != 0) {
-                const int logical = p.page_div.quotient(base + at);
+                int logical = p.page_div.quotient(base + at);
                 offset[r] = base + at - logical * p.cfg.page_size;
-                page[r] = chunk_page(p.cfg, p.page_table, s.run.batch, logical);
+                const int slots = p.cfg.max_pages_per_seq;
+                if (p.cfg.window_size > 0) logical -= p.slot_div.quotient(logical) * slots;
+                page[r] = __ldg(p.page_table + int64_t(s.run.batch) * slots + logical);
+                if (page[r] >= p.cfg.num_pages) page[r] = -1;
               }
             }
             const uint32_t lo = __ballot_sync(0xffffffffu, page[0] >= 0);
@@ -782,14 +785,17 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
                                 : cache_offset(p.cfg, p.layer, page[r], offset[r], head, 0);
               }
               const __nv_bfloat16 *from = own ? rows : cache;
-              const uint32_t column = dst + uint32_t(lane >> 3) * kBlockBytes;
+              // eight lanes to 128 bytes of a row, four rows at a time, block by block
 #pragma unroll 4
-              for (int r = 0; r < kKeys; ++r) {
-                const int64_t at = __shfl_sync(0xffffffffu, row_at[r >> 5], r & 31);
+              for (int r4 = 0; r4 < kKeys; r4 += 4) {
+                const int r = r4 + (lane >> 3);
+                const int64_t at = __shfl_sync(0xffffffffu, row_at[r4 >> 5], r & 31);
                 if (at >= 0) {
-                  cp_async16(column + uint32_t(r >> 3) * kGroupBytes + uint32_t(r & 7) * 128u +
-                                 ((uint32_t(lane & 7) ^ uint32_t(r & 7)) << 4),
-                             from + at + block0 * 64 + lane * 8);
+                  const __nv_bfloat16 *src = from + at + block0 * 64 + (lane & 7) * 8;
+                  const uint32_t to = dst + uint32_t(r >> 3) * kGroupBytes + uint32_t(r & 7) * 128u +
+                                      ((uint32_t(lane & 7) ^ uint32_t(r & 7)) << 4);
+#pragma unroll
+                  for (int b = 0; b < kPartDims / 64; ++b) cp_async16(to + uint32_t(b) * kBlockBytes, src + b * 64);
                 }
               }
               asm volatile("cp.async.wait_all;" ::: "memory");
