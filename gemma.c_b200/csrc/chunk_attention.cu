@@ -62,8 +62,10 @@
 // rows: HBM. Measured (16 + 8 heads of 256 unless said): 4096 tokens behind 12288 0.82 to
 // 0.99 ms by the GPU's power (1160 TFLOP/s at best); 32 runs of 1 .. 8 tokens over 512 ..
 // 12000 keys 261 us, 6.5 TB/s; runs of 239 .. 1211 tokens over rings of 1024 116 us; 64
-// tokens with a window of 2048 and 4 sinks 178 us, 6.0 TB/s; three runs of 406 .. 695
-// tokens of 16 heads of 512 on one KV head 244 us, 780 TFLOP/s.
+// tokens with a window of 2048 and 4 sinks 171 us, 6.3 TB/s; three runs of 406 .. 695
+// tokens of 16 heads of 512 on one KV head 250 us, 760 TFLOP/s. Pages of five tokens (a
+// copy of 16 bytes per lane by one warp, a tile of 64 keys some 5000 clocks): 453, 204,
+// 212 (725 .. 896 tokens, window 2048), 530.
 //
 // The roles share one instruction cache and much of what was tried is about that: waits
 // out of line and rolled MMA and epilogue loops (6000 to 4500 instructions) made the tile
@@ -605,6 +607,21 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       }
       ++segments;
     };
+    // box == 0: the slot whose copies are on their way. It is said to be full when the next
+    // slot's have been asked for, or at the segment's end.
+    uint32_t copied = 0;
+    auto copies_landed = [&](bool all) {
+      if (copied == 0) return;
+      if (all) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      } else {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      }
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(copied);
+      copied = 0;
+    };
     while (ok && walk.next(p, s, mine, first_run)) {
       const int head = s.hp % heads;
       const int part = s.hp / heads;
@@ -798,12 +815,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
                   for (int b = 0; b < kPartDims / 64; ++b) cp_async16(to + uint32_t(b) * kBlockBytes, src + b * 64);
                 }
               }
-              asm volatile("cp.async.wait_all;" ::: "memory");
-              if (!clear) {
-                fence_proxy_async_shared();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar);
-              }
+              asm volatile("cp.async.commit_group;" ::: "memory");
             } else if (own) {
               if (lane == 0) mbar_arrive_expect_tx(bar, kSlotBytes);
               __syncwarp();
@@ -843,15 +855,22 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
                   }
                 }
               }
-              fence_proxy_async_shared();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(bar_v_full + 8u * at.slot);
+              if (p.box > 0) {
+                fence_proxy_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_v_full + 8u * at.slot);
+              }
+            }
+            if (p.box == 0) {
+              copies_landed(false);
+              copied = bar_full + 8u * at.slot;
             }
             at.advance(ring_slots);
           }
           if (!ok) break;
         }
       }
+      copies_landed(true);
     }
     if (ok) tell_segment(0);
     failed = !ok;
