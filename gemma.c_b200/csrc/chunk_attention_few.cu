@@ -7,9 +7,9 @@
 // memory and its barriers on them. A cluster of CTAs takes one (query tile,
 // KV head) and each of its CTAs an even share of the keys in units of 16, a tile of 64
 // (head_dim 512: 32) at a time, brought by TMA a tile ahead: each of the eight warps asks
-// for one unit of K or V (head_dim 512: half of one), in a box or two that lie in a page,
-// so pages are of whole groups of eight tokens. (A copy per row costs its warp 86 clocks
-// each, 16 of them more than the tile's arithmetic.) Per tile:
+// for one unit of K or V (head_dim 512: half of one), in a box or two that lie in a page;
+// where pages are no whole groups of eight tokens by copies of 16 bytes. (A bulk copy per
+// row costs its warp 86 clocks each, 16 of them more than the tile's arithmetic.) Per tile:
 //   S = Q K^T     16 keys and 128 dims each, joined through shared memory
 //   softmax       16 threads to a row: running maximum and sum in fp32, the weights
 //                 rounded to bf16 for P V (by at most 2^-8 of each), summed unrounded
@@ -20,7 +20,7 @@
 //
 // Latency bounds it. Measured, four tokens of 16 + 8 heads of 256 over a ring of 1024 (4
 // MB of K and V, 1.3 us of HBM): 7.5 us of the GPU in a row of calls, 15.2 by the other
-// kernel and its join; one token over 100 keys 6.0. Of the way (80 CTAs, 2 tiles each) in
+// kernel and its join; one token over 100 keys 6.0; over pages of five 7.9 instead of 21.7. Of the way (80 CTAs, 2 tiles each) in
 // clocks: the runs 800, what follows from them 1100, page and first tile 1800, a tile
 // 1500 (of which the first is fetching code), sending and joining 2000. Earlier forms: a
 // copy of 16 bytes per lane instead of boxes 10.1 us (64 CTAs), a bulk copy per row 8.1,
@@ -175,6 +175,13 @@ __device__ __forceinline__ bool try_wait_for_peers(uint32_t bar) {
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
+__device__ __forceinline__ void copy_async16(uint32_t to, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// This lane's copies so far count as one arrival when they have landed.
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ bool few_wait(uint32_t bar, uint32_t parity) {
   for (uint32_t left = kFewPolls; !mbar_try_wait(bar, parity); --left) {
     if (left == 0) return false;
@@ -205,14 +212,17 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
   // groups of 16 output dims that this CTA joins: number n of the dims is CTA n % ctas's
   const int slots = div.ctas.quotient(T::kGroups + ctas - 1 - rank);
   if (tid == 0) {
-    for (int i = 0; i < kFewStages; ++i) mbar_init(bar_full + 8u * i, kFewWarps);
+    // a warp's word, and without boxes each lane's copies
+    for (int i = 0; i < kFewStages; ++i) mbar_init(bar_full + 8u * i, box > 0 ? kFewWarps : 33 * kFewWarps);
     mbar_init(bar_joined, uint32_t(ctas * kFewWarps));
     mbar_fence_init();
-    prefetch_map(&map_k);
-    prefetch_map(&map_v);
-    if (a.k_rows != nullptr) {
-      prefetch_map(&map_k_rows);
-      prefetch_map(&map_v_rows);
+    if (box > 0) {
+      prefetch_map(&map_k);
+      prefetch_map(&map_v);
+      if (a.k_rows != nullptr) {
+        prefetch_map(&map_k_rows);
+        prefetch_map(&map_v_rows);
+      }
     }
   }
   __syncthreads();
@@ -247,6 +257,7 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
   int token_group = -1;  // cache: group of eight tokens; -1: none
   auto look_up = [&](int j) {
     token_group = -1;
+    if (box == 0) return;
     const int ask = j * T::kUnits + my_unit + (lane >> 1) * T::kUnits;
     bool own;
     const int at = keys.base(unit0 + ask, own) + 8 * (lane & 1);
@@ -270,12 +281,49 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
     uint32_t alive = unit >= units ? 0u
                                    : low16((own ? t1 + 1 : keys.cache_end) - base) &
                                          (~low16(keys.lo - base) | low16(a.sinks - base));
-    const int group0 = __shfl_sync(0xffffffffu, token_group, 2 * (j & 15));
-    const int group1 = __shfl_sync(0xffffffffu, token_group, 2 * (j & 15) + 1);
-    if (!own) alive &= (group0 >= 0 ? 0xffu : 0u) | (group1 >= 0 ? 0xff00u : 0u);
     const int stage = j % kFewStages;
     const uint32_t bar = bar_full + 8u * uint32_t(stage);
     const uint32_t to = smem_u32(&s.tile[stage][is_v][my_unit * T::kUnitBytes]) + uint32_t(block0 * 2048);
+    if (box == 0) {  // pages of no whole groups of eight: row by row
+      int64_t offset = -1;  // of row `lane` of the unit
+      if (((alive >> lane) & 1u) != 0) {
+        const int at = base + lane;
+        if (own) {
+          offset = ((int64_t(run.start) + (at - run.first)) * heads + head) * D;
+        } else {
+          const int logical = div.page.quotient(at);
+          const int slot = c.window_size > 0 ? logical - div.slots.quotient(logical) * c.max_pages_per_seq : logical;
+          const int page = __ldg(a.page_table + int64_t(run.batch) * c.max_pages_per_seq + slot);
+          if (page >= 0 && page < c.num_pages) {
+            offset = cache_offset(c, a.layer, page, at - logical * c.page_size, head, 0);
+          }
+        }
+      }
+      alive = __ballot_sync(0xffffffffu, offset >= 0);
+      const __nv_bfloat16 *rows_of = own ? (is_v ? a.v_rows : a.k_rows) : (is_v ? a.cache_v : a.cache_k);
+      // eight lanes to 128 bytes of a row
+#pragma unroll
+      for (int r4 = 0; r4 < kFewUnit; r4 += 4) {
+        const int r = r4 + (lane >> 3);
+        const int64_t at = __shfl_sync(0xffffffffu, offset, r);
+        if (at >= 0) {
+          const __nv_bfloat16 *from = rows_of + at + block0 * 64 + (lane & 7) * 8;
+          const uint32_t dst = to + uint32_t((r >> 3) * 4096 + (r & 7) * 128 + (((lane & 7) ^ (r & 7)) << 4));
+#pragma unroll
+          for (int b = 0; b < kBoxDims / 64; ++b) copy_async16(dst + uint32_t(1024 * b), from + 64 * b);
+        }
+      }
+      copies_arrive(bar);
+      if (lane == 0) {
+        if (!is_v && block0 == 0) s.alive[stage][my_unit] = uint16_t(alive);
+        mbar_arrive(bar);
+      }
+      __syncwarp();
+      return;
+    }
+    const int group0 = __shfl_sync(0xffffffffu, token_group, 2 * (j & 15));
+    const int group1 = __shfl_sync(0xffffffffu, token_group, 2 * (j & 15) + 1);
+    if (!own) alive &= (group0 >= 0 ? 0xffu : 0u) | (group1 >= 0 ? 0xff00u : 0u);
     const bool both = !own && box == 16;  // one box for both groups of eight
     const bool half0 = (alive & 0xffu) != 0 || (both && alive != 0), half1 = (alive >> 8) != 0 && !both;
     if (lane == 0) {
@@ -554,7 +602,6 @@ int clusters_at_once(int device, int cluster) {
 template <int D>
 cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cudaStream_t stream, bool *taken) {
   const int box = box_tokens(a.cfg.page_size, kFewUnit);
-  if (box == 0) return cudaSuccess;
   const int group = a.q_heads / a.cfg.num_heads;
   const int tiles = div_up(std::min(a.runs.max_row_count, a.runs.rows), kFewRows / group);  // of a run
   const int64_t items = int64_t(a.runs.run_count) * a.cfg.num_heads * tiles;
@@ -580,10 +627,11 @@ cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cuda
   if (most * D > 640 * 256 * int64_t(cluster)) return cudaSuccess;
   *taken = true;
   CUtensorMap map_k = {}, map_v = {}, map_k_rows = {}, map_v_rows = {};
-  if (!make_cache_map(&map_k, a.cache_k, a.cfg, box) || !make_cache_map(&map_v, a.cache_v, a.cfg, box) ||
-      (a.k_rows != nullptr &&
-       (!make_rows_map(&map_k_rows, a.k_rows, a.runs.rows, a.cfg.num_heads, D) ||
-        !make_rows_map(&map_v_rows, a.v_rows, a.runs.rows, a.cfg.num_heads, D)))) {
+  if (box > 0 &&
+      (!make_cache_map(&map_k, a.cache_k, a.cfg, box) || !make_cache_map(&map_v, a.cache_v, a.cfg, box) ||
+       (a.k_rows != nullptr &&
+        (!make_rows_map(&map_k_rows, a.k_rows, a.runs.rows, a.cfg.num_heads, D) ||
+         !make_rows_map(&map_v_rows, a.v_rows, a.runs.rows, a.cfg.num_heads, D))))) {
     return cudaErrorInvalidValue;
   }
   const FewLaunch launch(cluster, a.cfg.num_heads, a.runs.run_count * tiles, kSmem, stream);

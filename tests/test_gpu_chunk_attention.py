@@ -100,6 +100,17 @@ CASES = {
     "few_tiles_group1": dict(counts=[100], firsts=[200], heads=3, group=1),
     "few_tiles_512": dict(counts=[20, 3], firsts=[300, 0], heads=1, group=16, dim=512, page=64),
     "few_tiles_512_own": dict(counts=[24], firsts=[200], heads=2, group=2, dim=512, own_rows=True),
+    "few_page5": dict(counts=[4], firsts=[777], page=5),
+    "few_page5_ring": dict(counts=[8, 3], firsts=[333, 64], ring=True, window=61, page=5),
+    "few_page3_tiles": dict(counts=[37, 2], firsts=[100, 9], page=3, heads=4, gap=1),
+    "few_page5_hole": dict(counts=[40], firsts=[120], unmap=[(0, 3), (0, 19)], heads=4, page=5),
+    "few_page5_512": dict(counts=[9, 1], firsts=[200, 3], heads=1, group=16, dim=512, page=5),
+    "few_page7_512_own": dict(counts=[24], firsts=[200], heads=2, group=2, dim=512, own_rows=True, page=7),
+    "few_page5_sinks": dict(counts=[50], firsts=[333], window=40, sinks=18, free_middle=True, page=5),
+    "large_page5": dict(counts=[170, 2], firsts=[131, 100], page=5),
+    "large_page5_own": dict(counts=[170, 2], firsts=[131, 100], page=5, own_rows=True),
+    "large_page5_512": dict(counts=[60, 100], firsts=[131, 100], heads=1, group=16, dim=512, page=5),
+    "large_page1": dict(counts=[170, 2], firsts=[60, 100], page=1),
     "few_tiles_hole": dict(counts=[40], firsts=[120], unmap=[(0, 3), (0, 9)], heads=4),
     "few_peaked": dict(counts=[8], firsts=[900], q_scale=30.0),
     "peaked": dict(counts=[64, 3], firsts=[500, 800], q_scale=30.0),
