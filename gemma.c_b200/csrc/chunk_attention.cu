@@ -1591,9 +1591,13 @@ cudaError_t validate_chunk_attention(const ChunkAttentionArgs &a) {
   return (align & 15u) == 0 ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &a, cudaStream_t stream) {
-  const cudaError_t valid = validate_chunk_attention(a);
+cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &given, cudaStream_t stream) {
+  const cudaError_t valid = validate_chunk_attention(given);
   if (valid != cudaSuccess) return valid;
+  // A window of all the positions hides nothing; cut to those, the distance of its start
+  // from a key tile behind the row (t - window + 1 - base) fits 32 bits in both kernels.
+  ChunkAttentionArgs a = given;
+  a.window = std::min(a.window, kMaxPosition);
   if (a.runs.run_count == 0 || a.runs.rows == 0) return cudaSuccess;
   int device = 0, sms = 0;
   cudaError_t st = cudaGetDevice(&device);
