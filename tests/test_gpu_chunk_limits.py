@@ -50,3 +50,57 @@ def test_a_ring_with_a_window_of_all_positions(kv, own):
     kv.chunk_attention(a)
     torch.cuda.synchronize()
     check_attention(case, t)
+
+
+# --------------------------------------------------------------------------------------------- the write
+def check_write(kv, case, run_count=None, **over):
+    """The runs' rows are where they belong, every other row of the cache as it was."""
+    from tests.test_gpu_chunk_append import stored
+
+    a, t = device_args(kv, case)
+    if run_count is not None:                    # runs without rows behind the case's own
+        for n in ("seq_batch", "first_position", "row_count", "row_start"):
+            t[n] = torch.cat([t[n], torch.zeros(run_count - t[n].numel(), dtype=torch.int32, device="cuda")])
+            setattr(a, n, t[n].data_ptr())
+        a.run_count = run_count
+    for name, value in over.items():
+        setattr(a, name, value)
+    bits = lambda x: x.view(torch.int16).reshape(-1)  # noqa: E731
+    want = [bits(stored(case, t[c], t[r])) for c, r in (("cache_k", "k_rows"), ("cache_v", "v_rows"))]
+    kv.chunk_write(a)
+    torch.cuda.synchronize()
+    assert torch.equal(bits(t["cache_k"]), want[0]) and torch.equal(bits(t["cache_v"]), want[1])
+
+
+WRITES = {
+    "ragged": dict(counts=[1, 33, 70, 2], firsts=[100, 0, 15, 300], own_rows=True, gap=2),
+    "ring": dict(counts=[200, 3, 64, 1], firsts=[10, 1000, 0, 70], ring=True, window=64, gap=1),
+    "ring_page5": dict(counts=[140, 7], firsts=[33, 9], ring=True, window=61, page=5),
+    "odd_heads": dict(counts=[9, 40], firsts=[7, 64], heads=3, group=1, own_rows=True),
+    "dim512": dict(counts=[9, 40], firsts=[7, 64], heads=1, group=16, dim=512, page=64, own_rows=True),
+    "layer": dict(counts=[21, 3], firsts=[7, 30], layers=3, layer=1, own_rows=True),
+    "unmapped": dict(counts=[40], firsts=[0], unmap=[(0, 1)], own_rows=True),
+    # several rows to a CTA
+    "long": dict(counts=[1500, 1, 650, 90, 2, 33], firsts=[3, 500, 0, 41, 7, 15], heads=2, gap=3, own_rows=True),
+    "long_ring": dict(counts=[1700, 3, 640, 1], firsts=[10, 1000, 0, 63], heads=2, ring=True, window=64),
+    "many_runs": dict(counts=[1 + i % 40 for i in range(100)], firsts=[i * 7 for i in range(100)], heads=2, page=5, gap=1,
+                      own_rows=True),
+}
+
+
+@pytest.mark.parametrize("name", list(WRITES))
+def test_write_of_runs(kv, name):
+    check_write(kv, make_case(23, **WRITES[name]))
+
+
+@pytest.mark.parametrize("name", ["ragged", "ring"])
+@pytest.mark.parametrize("bound", [100 * 70, 2**31 - 1])
+def test_a_generous_bound_of_the_run_length(kv, name, bound):
+    """The grid is cut to the rows there are and to a fixed size: max_row_count x run_count is 2^41 here."""
+    check_write(kv, make_case(24, **WRITES[name]), run_count=1024, max_row_count=bound)
+
+
+@pytest.mark.parametrize("name", ["long", "long_ring", "many_runs"])
+def test_a_cta_writes_every_so_manyth_row(kv, name):
+    """1024 runs leave a run 32 CTAs."""
+    check_write(kv, make_case(25, **WRITES[name]), run_count=1024)
