@@ -1615,4 +1615,17 @@ cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &given, cudaStream_t s
                                : launch_chunk<ChunkTraits<512>>(a, ctas, stream);
 }
 
+cudaError_t chunk_attention_give_up_selftest(const ChunkAttentionArgs &a, int32_t tile,
+                                             cudaStream_t stream) {
+  const cudaError_t valid = validate_chunk_attention(a);
+  if (valid != cudaSuccess) return valid;
+  if (a.status == nullptr || tile < 0 || a.runs.run_count == 0 || a.runs.rows == 0) return cudaErrorInvalidValue;
+  int device = 0;
+  cudaError_t st = cudaGetDevice(&device);
+  if (st != cudaSuccess) return st;
+  bool taken = false;
+  st = chunk_attention_few_bf16(a, device, table_end(a.cfg), stream, &taken, tile);
+  return st != cudaSuccess || taken ? st : cudaErrorInvalidValue;
+}
+
 }  // namespace b200kv

@@ -189,12 +189,13 @@ __device__ __forceinline__ bool few_wait(uint32_t bar, uint32_t parity) {
   return true;
 }
 
-// grid (CTAs of a cluster, KV heads, query tiles of the runs)
+// grid (CTAs of a cluster, KV heads, query tiles of the runs). give_up_at: the wait for
+// this key tile counts as run out (-1 but in the self-test).
 template <int D>
 __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
     const __grid_constant__ ChunkAttentionArgs a, const __grid_constant__ CUtensorMap map_k,
     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k_rows,
-    const __grid_constant__ CUtensorMap map_v_rows, int table_end, int box, FewDivs div) {
+    const __grid_constant__ CUtensorMap map_v_rows, int table_end, int box, FewDivs div, int give_up_at) {
   using T = FewTraits<D>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   FewShared<D> &s = *reinterpret_cast<FewShared<D> *>(smem_raw);
@@ -376,7 +377,7 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
   for (int j = 0; j < tiles; ++j) {
     const int stage = j % kFewStages;
     issue(j + 1);  // (its place was read before the barrier among the scores of tile j - 1)
-    ok = few_wait(bar_full + 8u * uint32_t(stage), uint32_t(j / kFewStages) & 1u);
+    ok = j != give_up_at && few_wait(bar_full + 8u * uint32_t(stage), uint32_t(j / kFewStages) & 1u);
     const uint32_t k_at = tile_at + uint32_t(2 * stage * T::kTileBytes);
     const uint32_t v_at = k_at + uint32_t(T::kTileBytes);
     {  // a part of the scores
@@ -435,9 +436,15 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
       }
     }
     ok = __syncthreads_and(ok);
-    if (!ok) {  // a tile did not come: give its copies time to land before the CTA ends
-      mbar_wait_bounded(bar_full + 8u * uint32_t(stage), uint32_t(j / kFewStages) & 1u, 1ll << 26);
+    if (!ok) {
+      // A tile did not come: its copies and those of the next one, asked for above, get the
+      // time to land before the CTA gives its shared memory back. A NaN in the sums makes
+      // the rows and their log-sum-exp NaN, whichever CTA joins them.
+      for (int i = j; i < min(j + 2, tiles); ++i) {
+        mbar_wait_bounded(bar_full + 8u * uint32_t(i % kFewStages), uint32_t(i / kFewStages) & 1u, 1ll << 26);
+      }
       set_status(a.status, B200KV_STATUS_WAIT_TIMEOUT);
+      l = __int_as_float(0x7fffffff);
       break;
     }
     {
@@ -528,7 +535,7 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
   for (uint32_t left = 32 * kFewPolls; ok && !try_wait_for_peers(bar_joined); --left) ok = left > 0;
   ok = __all_sync(0xffffffffu, ok);
   // ---- joined: out = sum 2^(m_k - M) O_k / sum 2^(m_k - M) l_k
-  if (ok && row < rows) {
+  if (row < rows) {
     float2 ml = make_float2(-INFINITY, 0.0f);  // of CTA `place`
     if (place < ctas) ml = s.row[place][row];
     const uint32_t lanes = 0xffffu << (lane & 16);
@@ -540,6 +547,7 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
     float sum = f * ml.y;
 #pragma unroll
     for (int d = 8; d > 0; d /= 2) sum += __shfl_xor_sync(lanes, sum, d);
+    if (!ok) sum = __int_as_float(0x7fffffff);  // some CTA has not sent its share
     s.factor[row][place] = f * (sum != 0.0f ? 1.0f / sum : 0.0f);
     __syncwarp(lanes);
     const int token = div.group.quotient(row);
@@ -600,7 +608,8 @@ int clusters_at_once(int device, int cluster) {
 }
 
 template <int D>
-cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cudaStream_t stream, bool *taken) {
+cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cudaStream_t stream, bool *taken,
+                    int give_up_at) {
   const int box = box_tokens(a.cfg.page_size, kFewUnit);
   const int group = a.q_heads / a.cfg.num_heads;
   const int tiles = div_up(std::min(a.runs.max_row_count, a.runs.rows), kFewRows / group);  // of a run
@@ -639,17 +648,17 @@ cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cuda
                        FastDiv::by(uint32_t(group)), FastDiv::by(uint32_t(cluster)),
                        FastDiv::by(uint32_t(tiles))};
   return cudaLaunchKernelEx(&launch.config, kernel, a, map_k, map_v, map_k_rows, map_v_rows,
-                            table_end, box, div);
+                            table_end, box, div, give_up_at);
 }
 
 }  // namespace
 
 cudaError_t chunk_attention_few_bf16(const ChunkAttentionArgs &a, int device, int table_end,
-                                     cudaStream_t stream, bool *taken) {
+                                     cudaStream_t stream, bool *taken, int give_up_at) {
   *taken = false;
   if (a.q_heads / a.cfg.num_heads > kFewRows) return cudaSuccess;
-  return a.cfg.head_dim == 256 ? try_few<256>(a, device, table_end, stream, taken)
-                               : try_few<512>(a, device, table_end, stream, taken);
+  return a.cfg.head_dim == 256 ? try_few<256>(a, device, table_end, stream, taken, give_up_at)
+                               : try_few<512>(a, device, table_end, stream, taken, give_up_at);
 }
 
 }  // namespace b200kv

@@ -1342,6 +1342,12 @@ int b200kv_chunk_attention_bf16(const B200KvChunkArgs *s, b200kv_stream stream) 
   return b200kv::chunk_attention_bf16(chunk_attention_args(s), static_cast<cudaStream_t>(stream));
 }
 
+int b200kv_chunk_attention_give_up_selftest(const B200KvChunkArgs *s, int32_t tile, b200kv_stream stream) {
+  if (s == nullptr) return cudaErrorInvalidValue;
+  return b200kv::chunk_attention_give_up_selftest(chunk_attention_args(s), tile,
+                                                  static_cast<cudaStream_t>(stream));
+}
+
 size_t b200kv_chunk_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                                     int32_t run_count, int32_t max_row_count,
                                     int32_t sm_count) {

@@ -332,9 +332,12 @@ struct ChunkAttentionArgs {
 cudaError_t validate_chunk_attention(const ChunkAttentionArgs &args);
 cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &args, cudaStream_t stream);
 // The form for small calls (chunk_attention_few.cu); *taken: it was for
-// these sizes. table_end: first position past a linear cache's table.
+// these sizes. table_end: first position past a linear cache's table. give_up_at: the
+// key tile of every CTA whose wait counts as run out (-1: none).
 cudaError_t chunk_attention_few_bf16(const ChunkAttentionArgs &args, int device, int table_end,
-                                     cudaStream_t stream, bool *taken);
+                                     cudaStream_t stream, bool *taken, int give_up_at = -1);
+cudaError_t chunk_attention_give_up_selftest(const ChunkAttentionArgs &args, int32_t tile,
+                                             cudaStream_t stream);
 size_t chunk_workspace_bytes(int q_heads, int kv_heads, int head_dim, int run_count,
                              int max_row_count, int sm_count);
 

@@ -687,6 +687,14 @@ size_t b200kv_chunk_workspace_bytes(int32_t q_heads, int32_t kv_heads,
                                     int32_t head_dim, int32_t run_count,
                                     int32_t max_row_count, int32_t sm_count);
 
+/* Self-test of the attention's give-up path, for calls of few rows over few keys (which
+ * a kernel of their own computes; others are refused): the wait of every CTA for its key
+ * tile `tile` (from 0; a tile is 64 keys, of head_dim 512 32) counts as run out although the
+ * tile comes. CTAs that have such a tile write B200KV_STATUS_WAIT_TIMEOUT to status[0], which
+ * must be given, and the rows they share come out as NaN with a NaN lse; nothing faults. */
+int b200kv_chunk_attention_give_up_selftest(const B200KvChunkArgs *args, int32_t tile,
+                                            b200kv_stream stream);
+
 /* Stores k_rows / v_rows of the runs in the cache (see above). */
 int b200kv_chunk_write_bf16(const B200KvChunkArgs *args, b200kv_stream stream);
 

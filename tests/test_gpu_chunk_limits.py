@@ -104,3 +104,46 @@ def test_a_generous_bound_of_the_run_length(kv, name, bound):
 def test_a_cta_writes_every_so_manyth_row(kv, name):
     """1024 runs leave a run 32 CTAs."""
     check_write(kv, make_case(25, **WRITES[name]), run_count=1024)
+
+
+# --------------------------------------------------------------------------------------------- waits that run out
+GIVE_UPS = {
+    "first_tile": (0, dict(counts=[4], firsts=[1500], ring=True, window=1024)),
+    "next_tile_on_its_way": (0, dict(counts=[3], firsts=[3000])),
+    "second_tile": (1, dict(counts=[3], firsts=[3000])),
+    "page5": (0, dict(counts=[4], firsts=[3000], page=5)),
+    "dim512": (1, dict(counts=[1, 1], firsts=[1900, 2000], heads=1, group=16, dim=512, page=64)),
+}
+
+
+@pytest.mark.parametrize("name", list(GIVE_UPS))
+def test_rows_of_a_call_that_gives_up_are_nan(kv, name):
+    """Not an average over the keys that came in time. The context stays usable: the same call afterwards is right."""
+    tile, over = GIVE_UPS[name]
+    case = make_case(26, **over)
+    a, t = device_args(kv, case)
+    kv.chunk_attention_give_up_selftest(a, tile)
+    torch.cuda.synchronize()
+    assert t["status"][0].item() == kv.STATUS_WAIT_TIMEOUT
+    assert bool(t["out"].isnan().all()) and bool(t["lse"].isnan().all())
+    t["status"].zero_()
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+
+
+def test_give_up_selftest_of_a_tile_that_no_cta_has(kv):
+    case = make_case(27, [4], [500])
+    a, t = device_args(kv, case)
+    kv.chunk_attention_give_up_selftest(a, 1000)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+
+
+def test_give_up_selftest_refuses(kv):
+    a, t = device_args(kv, make_case(28, [4], [500]))
+    assert kv.chunk_attention_give_up_selftest(a, -1, check=False) == 1
+    a.status = None
+    assert kv.chunk_attention_give_up_selftest(a, 0, check=False) == 1
+    large, _ = device_args(kv, make_case(28, [1, 2], [6000, 5200], heads=1, group=16, dim=512, page=64))
+    assert kv.chunk_attention_give_up_selftest(large, 0, check=False) == 1
