@@ -112,7 +112,10 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *r) {
       : "memory");
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 32; ++i) r[i] = __uint_as_float(u[i]);
+  for (int i = 0; i < 32; ++i) {
+    asm volatile("" : "+r"(u[i]));  // not used before the wait
+    r[i] = __uint_as_float(u[i]);
+  }
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float *r) {
   asm volatile(
@@ -167,7 +170,10 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, float *r) {
         : "memory");
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 16; ++i) r[i] = __uint_as_float(u[i]);
+    for (int i = 0; i < 16; ++i) {
+      asm volatile("" : "+r"(u[i]));  // not used before the wait
+      r[i] = __uint_as_float(u[i]);
+    }
   }
 }
 // kCount packed bf16 pairs into this thread's lane (kCount = 16 or 8)

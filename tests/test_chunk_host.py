@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -226,3 +227,18 @@ def test_compact_needs_an_empty_list_and_room(kv):
     q.fork(0, 1, 6)
     q.ensure(1, 6, 1)
     assert kv.pages_compact(q.table, q.refs, q.cfg, q.copies)[0] == -1          # a copy is still to be made
+
+
+# --------------------------------------------------------------------------------------------- sources
+def test_registers_of_tensor_memory_loads_are_tied_to_the_wait(kv):
+    """A load from tensor memory is asynchronous: its registers hold nothing before the wait, and nothing but a mention
+    of them behind it keeps the compiler from moving what is computed with them ahead of it."""
+    sources = sorted((Path(kv.__file__).parent / "csrc").glob("*.cu*"))
+    waits = 0
+    for path in sources:
+        lines = path.read_text().splitlines()
+        for at in (i for i, line in enumerate(lines) if "tcgen05.wait::ld" in line):
+            waits += 1
+            tied = any('asm volatile("" : "+r"(' in line for line in lines[at + 1:at + 4])
+            assert tied, f"{path.name}:{at + 1}"
+    assert waits >= 3
