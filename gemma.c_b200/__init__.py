@@ -228,6 +228,7 @@ _SIGNATURES = {
                                                   c_int32, c_int32, _P, _P, _P, _P, _P, _P]),
     "b200kv_chunk_append_bf16": (c_int, [POINTER(ChunkArgs), _P]),
     "b200kv_chunk_attention_bf16": (c_int, [POINTER(ChunkArgs), _P]),
+    "b200kv_chunk_attention_launches": (c_int32, [POINTER(ChunkArgs)]),
     "b200kv_chunk_attention_give_up_selftest": (c_int, [POINTER(ChunkArgs), c_int32, _P]),
     "b200kv_chunk_workspace_bytes": (c_size_t, [c_int32] * 6),
     "b200kv_chunk_write_bf16": (c_int, [POINTER(ChunkArgs), _P]),
@@ -629,6 +630,11 @@ def chunk_attention(args: ChunkArgs, stream=None, check: bool = True) -> int:
     """Attention of the runs' rows over their sequences' cached keys (and their own rows)."""
     code = load_library().b200kv_chunk_attention_bf16(ctypes.byref(args), _stream(stream))
     return _check(code, "b200kv_chunk_attention_bf16", check)
+
+
+def chunk_attention_launches(args: ChunkArgs) -> int:
+    """1: a small call, one kernel; 2: attention and join; 0: refused, or nothing to do."""
+    return int(load_library().b200kv_chunk_attention_launches(ctypes.byref(args)))
 
 
 def chunk_attention_give_up_selftest(args: ChunkArgs, tile: int, stream=None, check: bool = True) -> int:

@@ -1567,8 +1567,7 @@ cudaError_t validate_chunk_attention(const ChunkAttentionArgs &a) {
   // (run, query tile) pairs that every CTA adds up, and the most key tiles they can have
   const int64_t tokens = kRows / (a.q_heads / c.num_heads);
   const int64_t pairs = a.runs.run_count * div_up(int64_t(std::min(a.runs.max_row_count, a.runs.rows)), tokens);
-  const int64_t keys = (c.window_size > 0 ? c.window_size + tokens : table_end(c)) +
-                       (a.k_rows != nullptr ? a.runs.max_row_count : 0);
+  const int64_t keys = most_keys(a, table_end(c), tokens);
   // (each of the four stretches of keys may begin and end inside a tile)
   const double cost = double(keys / kKeys + 8 + kItemCost) * double(pairs) * c.num_heads * (c.head_dim / kPartDims);
   if (pairs > (1 << 24) || cost >= 2147483648.0) return cudaErrorInvalidValue;
@@ -1613,6 +1612,15 @@ cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &given, cudaStream_t s
   const int ctas = int(std::min<int64_t>(sms, room));
   return a.cfg.head_dim == 256 ? launch_chunk<ChunkTraits<256>>(a, ctas, stream)
                                : launch_chunk<ChunkTraits<512>>(a, ctas, stream);
+}
+
+int chunk_attention_launches(const ChunkAttentionArgs &a) {
+  int device = 0;
+  if (validate_chunk_attention(a) != cudaSuccess || a.runs.run_count == 0 || a.runs.rows == 0 ||
+      cudaGetDevice(&device) != cudaSuccess) {
+    return 0;
+  }
+  return chunk_attention_few_takes(a, device, table_end(a.cfg)) ? 1 : 2;  // the other one's join
 }
 
 cudaError_t chunk_attention_give_up_selftest(const ChunkAttentionArgs &a, int32_t tile,

@@ -607,34 +607,47 @@ int clusters_at_once(int device, int cluster) {
   return count;
 }
 
+// Query tiles of the longest run.
+int64_t few_tiles(const ChunkAttentionArgs &a) {
+  return div_up(int64_t(std::min(a.runs.max_row_count, a.runs.rows)), kFewRows / (a.q_heads / a.cfg.num_heads));
+}
+
+// The clusters' size for the call; *cluster 0: it is not a small one.
 template <int D>
-cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cudaStream_t stream, bool *taken,
-                    int give_up_at) {
-  const int box = box_tokens(a.cfg.page_size, kFewUnit);
-  const int group = a.q_heads / a.cfg.num_heads;
-  const int tiles = div_up(std::min(a.runs.max_row_count, a.runs.rows), kFewRows / group);  // of a run
-  const int64_t items = int64_t(a.runs.run_count) * a.cfg.num_heads * tiles;
-  const int64_t most = a.window > 0 ? int64_t(a.window) + a.sinks : table_end;  // keys of a row
+cudaError_t few_cluster(const ChunkAttentionArgs &a, int device, int table_end, int *cluster) {
+  *cluster = 0;
+  const int64_t items = a.runs.run_count * a.cfg.num_heads * few_tiles(a);
   constexpr int kSmem = int(sizeof(FewShared<D>));
   static_assert(kSmem <= 227 * 1024, "the tiles must fit one SM");
   const auto kernel = chunk_attention_few_kernel<D>;
   cudaError_t st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (st == cudaSuccess) st = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (st != cudaSuccess) return st;
-  int cluster = kFewMaxCluster;  // the largest of which all run at once
-  while (cluster >= 1 && items > clusters_at_once<D>(device, cluster)) --cluster;
-  if (cluster < 1) return cudaSuccess;
+  int size = kFewMaxCluster;  // the largest of which all run at once
+  while (size >= 1 && items > clusters_at_once<D>(device, size)) --size;
+  if (size < 1) return cudaSuccess;
   // A tile of 64 keys is 1.2 us here behind some 5.6 of start and end; the other kernel and
   // its join take 12 to 17 and hardly more for more keys, so up to 640 keys of 256 dims to a
-  // CTA belong here. What the host knows of the lengths is the most that a row can see. GPU
+  // CTA belong here. Of the lengths the host knows the most that a row can see. GPU
   // time here / there, eight heads of 256: four tokens of one sequence over 500, 4000, 8000
   // keys 6.4 / 14.1, 13.4 / 17.0, 20.7 / 19.9 us; of four over 2000 14.5 / 18.9, of eight
   // over 500 9.6 / 21.8; 40 tokens over 500, 2000 8.6 / 16.9, 18.2 / 18.3; 100 over 50, 500
   // 8.4 / 16.0, 16.8 / 18.5; 16 tokens of 16 heads of 512 on one KV head over 500, 2000 10.0
   // / 18.9, 18.8 / 20.3. Where the lengths differ the longest counts here: four tokens of
   // four sequences over 100 .. 4000 keys 24.0 / 19.1.
-  if (most * D > 640 * 256 * int64_t(cluster)) return cudaSuccess;
+  if (most_keys(a, table_end, 1) * D <= 640 * 256 * int64_t(size)) *cluster = size;
+  return cudaSuccess;
+}
+
+template <int D>
+cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cudaStream_t stream, bool *taken,
+                    int give_up_at) {
+  int cluster = 0;
+  const cudaError_t st = few_cluster<D>(a, device, table_end, &cluster);
+  if (st != cudaSuccess || cluster == 0) return st;
   *taken = true;
+  const int box = box_tokens(a.cfg.page_size, kFewUnit);
+  const int tiles = int(few_tiles(a));  // (no more than clusters that run at once)
   CUtensorMap map_k = {}, map_v = {}, map_k_rows = {}, map_v_rows = {};
   if (box > 0 &&
       (!make_cache_map(&map_k, a.cache_k, a.cfg, box) || !make_cache_map(&map_v, a.cache_v, a.cfg, box) ||
@@ -643,15 +656,23 @@ cudaError_t try_few(const ChunkAttentionArgs &a, int device, int table_end, cuda
          !make_rows_map(&map_v_rows, a.v_rows, a.runs.rows, a.cfg.num_heads, D))))) {
     return cudaErrorInvalidValue;
   }
-  const FewLaunch launch(cluster, a.cfg.num_heads, a.runs.run_count * tiles, kSmem, stream);
+  const FewLaunch launch(cluster, a.cfg.num_heads, a.runs.run_count * tiles, int(sizeof(FewShared<D>)), stream);
   const FewDivs div = {FastDiv::by(uint32_t(a.cfg.page_size)), FastDiv::by(uint32_t(a.cfg.max_pages_per_seq)),
-                       FastDiv::by(uint32_t(group)), FastDiv::by(uint32_t(cluster)),
+                       FastDiv::by(uint32_t(a.q_heads / a.cfg.num_heads)), FastDiv::by(uint32_t(cluster)),
                        FastDiv::by(uint32_t(tiles))};
-  return cudaLaunchKernelEx(&launch.config, kernel, a, map_k, map_v, map_k_rows, map_v_rows,
+  return cudaLaunchKernelEx(&launch.config, chunk_attention_few_kernel<D>, a, map_k, map_v, map_k_rows, map_v_rows,
                             table_end, box, div, give_up_at);
 }
 
 }  // namespace
+
+bool chunk_attention_few_takes(const ChunkAttentionArgs &a, int device, int table_end) {
+  if (a.q_heads / a.cfg.num_heads > kFewRows) return false;
+  int cluster = 0;
+  const cudaError_t st = a.cfg.head_dim == 256 ? few_cluster<256>(a, device, table_end, &cluster)
+                                               : few_cluster<512>(a, device, table_end, &cluster);
+  return st == cudaSuccess && cluster > 0;
+}
 
 cudaError_t chunk_attention_few_bf16(const ChunkAttentionArgs &a, int device, int table_end,
                                      cudaStream_t stream, bool *taken, int give_up_at) {

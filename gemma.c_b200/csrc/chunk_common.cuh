@@ -2,6 +2,8 @@
 // the write and the attention share.
 #pragma once
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.cuh"
 
@@ -87,6 +89,15 @@ inline bool valid_chunk_runs(const ChunkRuns &r) {
   return r.seq_batch != nullptr && r.first_position != nullptr && r.row_count != nullptr &&
          r.row_start != nullptr && r.run_count >= 0 && r.run_count <= B200KV_MAX_RUNS &&
          r.max_row_count > 0 && r.rows >= 0;
+}
+
+// The most keys that the rows of `tokens` consecutive tokens of a run can see, whatever
+// the lengths: the table's positions and the run's own rows, or the window's and the
+// first tokens'. table_end: first position past a linear cache's table.
+inline int64_t most_keys(const ChunkAttentionArgs &a, int table_end, int64_t tokens) {
+  const int64_t own = a.k_rows != nullptr ? std::min(a.runs.max_row_count, a.runs.rows) : 0;
+  const int64_t all = table_end + own;
+  return a.window > 0 ? std::min(all, int64_t(a.window) + tokens - 1 + a.sinks) : all;
 }
 
 inline bool valid_cache_config(const Gemma4KvCacheConfig &c, int layer) {

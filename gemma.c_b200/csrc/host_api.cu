@@ -1342,6 +1342,10 @@ int b200kv_chunk_attention_bf16(const B200KvChunkArgs *s, b200kv_stream stream) 
   return b200kv::chunk_attention_bf16(chunk_attention_args(s), static_cast<cudaStream_t>(stream));
 }
 
+int32_t b200kv_chunk_attention_launches(const B200KvChunkArgs *s) {
+  return s == nullptr ? 0 : b200kv::chunk_attention_launches(chunk_attention_args(s));
+}
+
 int b200kv_chunk_attention_give_up_selftest(const B200KvChunkArgs *s, int32_t tile, b200kv_stream stream) {
   if (s == nullptr) return cudaErrorInvalidValue;
   return b200kv::chunk_attention_give_up_selftest(chunk_attention_args(s), tile,

@@ -336,6 +336,8 @@ cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &args, cudaStream_t st
 // key tile of every CTA whose wait counts as run out (-1: none).
 cudaError_t chunk_attention_few_bf16(const ChunkAttentionArgs &args, int device, int table_end,
                                      cudaStream_t stream, bool *taken, int give_up_at = -1);
+bool chunk_attention_few_takes(const ChunkAttentionArgs &args, int device, int table_end);
+int chunk_attention_launches(const ChunkAttentionArgs &args);
 cudaError_t chunk_attention_give_up_selftest(const ChunkAttentionArgs &args, int32_t tile,
                                              cudaStream_t stream);
 size_t chunk_workspace_bytes(int q_heads, int kv_heads, int head_dim, int run_count,

@@ -675,8 +675,9 @@ int b200kv_chunk_append_bf16(const B200KvChunkArgs *args, b200kv_stream stream);
  * 512, any number G of query heads per KV head up to 64. With P = run_count *
  * ceil(min(max_row_count, rows) / floor(128 / G)) query tiles: P <= 2^24 and
  * P * kv_heads * (head_dim / 256) * (keys / 64 + 16) < 2^31, keys being the most
- * that a row can see (the window, or the table's positions) and, with k_rows,
- * max_row_count; larger calls are refused.
+ * that a tile of floor(128 / G) tokens can see: the table's positions and, with
+ * k_rows, min(max_row_count, rows), or with a window window_size + sink_tokens +
+ * floor(128 / G) - 1 if that is less; larger calls are refused.
  * `workspace` holds the partial results of rows whose keys several CTAs share;
  * it need not be cleared and nothing is kept in it between calls; calls that may
  * overlap on the GPU (two streams, two captured graphs) need one each. */
@@ -687,11 +688,15 @@ size_t b200kv_chunk_workspace_bytes(int32_t q_heads, int32_t kv_heads,
                                     int32_t head_dim, int32_t run_count,
                                     int32_t max_row_count, int32_t sm_count);
 
-/* Self-test of the attention's give-up path, for calls of few rows over few keys (which
- * a kernel of their own computes; others are refused): the wait of every CTA for its key
- * tile `tile` (from 0; a tile is 64 keys, of head_dim 512 32) counts as run out although the
- * tile comes. CTAs that have such a tile write B200KV_STATUS_WAIT_TIMEOUT to status[0], which
- * must be given, and the rows they share come out as NaN with a NaN lse; nothing faults. */
+/* Kernels that the attention of these arguments launches on the current device: 1 (a call
+ * of few rows over few keys), 2, or 0 for a call that is refused or has nothing to do. */
+int32_t b200kv_chunk_attention_launches(const B200KvChunkArgs *args);
+
+/* Self-test of the attention's give-up path, for calls that take one launch (see
+ * above; others are refused): the wait of every CTA for its key tile `tile` (from 0; a
+ * tile is 64 keys, of head_dim 512 32) counts as run out although the tile comes. CTAs
+ * that have such a tile write B200KV_STATUS_WAIT_TIMEOUT to status[0], which must be
+ * given, and the rows they share come out as NaN with a NaN lse; nothing faults. */
 int b200kv_chunk_attention_give_up_selftest(const B200KvChunkArgs *args, int32_t tile,
                                             b200kv_stream stream);
 

@@ -8,6 +8,7 @@ import torch
 
 from tests.chunk_cases import check_attention, device_args, make_case
 from tests.gpu_util import need_gpu
+from tests.test_gpu_chunk_attention import CASES as ATTENTION_CASES
 
 pytestmark = [pytest.mark.gpu, need_gpu]
 
@@ -147,3 +148,48 @@ def test_give_up_selftest_refuses(kv):
     assert kv.chunk_attention_give_up_selftest(a, 0, check=False) == 1
     large, _ = device_args(kv, make_case(28, [1, 2], [6000, 5200], heads=1, group=16, dim=512, page=64))
     assert kv.chunk_attention_give_up_selftest(large, 0, check=False) == 1
+
+
+# --------------------------------------------------------------------------------------------- which kernel, and what is refused
+@pytest.mark.parametrize("name", [n for n in ATTENTION_CASES if n.startswith(("few_", "large_"))])
+def test_the_cases_of_each_kernel_reach_it(kv, name):
+    a, _ = device_args(kv, make_case(len(name) * 7 + 1, **ATTENTION_CASES[name]))
+    assert kv.chunk_attention_launches(a) == (1 if name.startswith("few_") else 2)
+
+
+SIZE_RULE = {
+    # a row sees no more than the table has, however wide the window
+    "window_wider_than_the_table": (1, dict(counts=[3], firsts=[500], window=100000)),
+    "window_of_all_positions": (1, dict(counts=[3], firsts=[500], window=MOST, sinks=3)),
+    # the run's own rows are keys too: 1600 of them in 100 tiles for a CTA each
+    "own_rows_behind_a_short_table": (2, dict(counts=[1600], firsts=[10], heads=1, group=1, own_rows=True)),
+    "own_rows_in_a_window": (1, dict(counts=[1600], firsts=[10], heads=1, group=1, own_rows=True, window=64)),
+}
+
+
+@pytest.mark.parametrize("name", list(SIZE_RULE))
+def test_small_calls_go_by_what_a_row_can_see(kv, name):
+    launches, over = SIZE_RULE[name]
+    case = make_case(29, **over)
+    a, t = device_args(kv, case)
+    assert kv.chunk_attention_launches(a) == launches
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_a_window_over_a_table_of_all_positions_is_not_refused(kv, own):
+    """The limit of a call's key tiles goes by the window, as documented, not by the table."""
+    case = make_case(30, [520, 3], [300, 40], page=64, window=100, sinks=3, own_rows=own)
+    slots = 2**31 // 64
+    table = np.full((2, slots), -1, dtype=np.int32)
+    table[:, :case.table.shape[1]] = case.table
+    case.table = table
+    case.cfg = (*case.cfg[:3], slots, *case.cfg[4:])
+    a, t = device_args(kv, case)
+    kv.chunk_attention(a)
+    torch.cuda.synchronize()
+    check_attention(case, t)
+    a.window_size = a.sink_tokens = 0           # without a window it goes by the table
+    assert kv.chunk_attention_launches(a) == 0 and kv.chunk_attention(a, check=False) == 1
