@@ -12,7 +12,8 @@
 // 500 pages of an 8-bit cache in 2 layers (131 MB both ways) 25 us; the first rows of
 // 16 pages in 4 layers 3.2 us of the GPU.
 #include <algorithm>
-#include <vector>
+#include <memory>
+#include <new>
 
 #include "chunk_common.cuh"
 #include "kernels.cuh"
@@ -137,6 +138,13 @@ bool valid_copy_list(const int32_t *src, const int32_t *dst, const int32_t *rows
          (capacity == 0 || (src != nullptr && dst != nullptr && rows != nullptr));
 }
 
+// n times -1; nullptr where there is no memory for it (no exception leaves a C entry).
+std::unique_ptr<int32_t[]> no_pages(int64_t n) {
+  std::unique_ptr<int32_t[]> list(new (std::nothrow) int32_t[size_t(n)]);
+  if (list != nullptr) std::fill_n(list.get(), n, -1);
+  return list;
+}
+
 bool holds(const int32_t *list, int32_t count, int32_t page) {
   return count > 0 && std::find(list, list + count, page) != list + count;
 }
@@ -164,7 +172,8 @@ int32_t b200kv_pages_ensure(int32_t *h_page_table, int32_t *h_ref_count,
   const int32_t kept_rows = first % ps;  // rows of the first page that stay
 
   // what every slot needs, before anything changes
-  std::vector<int32_t> fresh(size_t(hi - lo + 1), -1);
+  const auto fresh = no_pages(int64_t(hi) - lo + 1);
+  if (fresh == nullptr) return -1;
   int32_t cursor = 0, copies = *copy_count;
   for (int32_t slot = lo; slot <= hi; ++slot) {
     const int32_t page = table[slot];
@@ -269,7 +278,8 @@ int32_t b200kv_pages_compact(int32_t *h_page_table, int32_t *h_ref_count,
   int32_t moves = 0;
   for (int32_t p = live; p < config->num_pages; ++p) moves += h_ref_count[p] > 0 ? 1 : 0;
   if (moves > capacity) return -1;
-  std::vector<int32_t> now(size_t(config->num_pages), -1);
+  const auto now = no_pages(config->num_pages);
+  if (now == nullptr) return -1;
   int32_t hole = 0;
   for (int32_t p = live; p < config->num_pages; ++p) {
     if (h_ref_count[p] <= 0) continue;

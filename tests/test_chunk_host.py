@@ -2,6 +2,8 @@
 from __future__ import annotations
 
 import ctypes
+import subprocess
+import sys
 from pathlib import Path
 
 import numpy as np
@@ -227,6 +229,41 @@ def test_compact_needs_an_empty_list_and_room(kv):
     q.fork(0, 1, 6)
     q.ensure(1, 6, 1)
     assert kv.pages_compact(q.table, q.refs, q.cfg, q.copies)[0] == -1          # a copy is still to be made
+
+
+OUT_OF_MEMORY = """
+import importlib.util, resource, sys
+from pathlib import Path
+import numpy as np
+pkg = Path(sys.argv[1])
+spec = importlib.util.spec_from_file_location("gemma_c_b200", pkg / "__init__.py", submodule_search_locations=[str(pkg)])
+kv = sys.modules["gemma_c_b200"] = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(kv)
+kv.load_library()
+n = 1 << 24
+cfg = kv.make_kv_config(1, n, 1, n, 1, 8, 256, 0)
+table, refs, copies = np.full((1, n), -1, dtype=np.int32), np.zeros(n, dtype=np.int32), kv.PageCopies(4)
+if sys.argv[2] == "compact":
+    table[0, 0], refs[n - 1] = n - 1, 1
+state = table.copy(), refs.copy()
+size = int(Path("/proc/self/statm").read_text().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (size + (16 << 20), resource.RLIM_INFINITY))
+if sys.argv[2] == "compact":
+    code = kv.pages_compact(table, refs, cfg, copies)[0]
+else:
+    code = kv.pages_ensure(table, refs, cfg, 0, 0, n, copies)
+resource.setrlimit(resource.RLIMIT_AS, (resource.RLIM_INFINITY, resource.RLIM_INFINITY))
+assert code == -1 and copies.count == 0
+assert np.array_equal(state[0], table) and np.array_equal(state[1], refs)
+"""
+
+
+@pytest.mark.parametrize("call", ["ensure", "compact"])
+def test_a_call_without_memory_fails_and_changes_nothing(kv, call):
+    """In a process of its own whose address space has no room for the call's 64 MB: -1, not an exception that ends it."""
+    done = subprocess.run([sys.executable, "-c", OUT_OF_MEMORY, str(Path(kv.__file__).parent), call], capture_output=True,
+                          text=True, timeout=120)
+    assert done.returncode == 0, done.stderr[-500:]
 
 
 # --------------------------------------------------------------------------------------------- sources
