@@ -249,12 +249,18 @@ int32_t b200kv_pages_release(int32_t *h_page_table, int32_t *h_ref_count,
   }
   int32_t *table = h_page_table + int64_t(batch) * config->max_pages_per_seq + first_slot;
   for (int32_t s = 0; s < slot_count; ++s) {
-    if (table[s] >= 0 && (table[s] >= config->num_pages || h_ref_count[table[s]] <= 0)) return -1;
+    if (table[s] < 0) continue;
+    // (a page may be named by several of the slots: its count has to last for all)
+    if (table[s] < config->num_pages && h_ref_count[table[s]] > 0) {
+      --h_ref_count[table[s]];
+      continue;
+    }
+    while (--s >= 0) {
+      if (table[s] >= 0) ++h_ref_count[table[s]];
+    }
+    return -1;
   }
-  for (int32_t s = 0; s < slot_count; ++s) {
-    if (table[s] >= 0) --h_ref_count[table[s]];
-    table[s] = -1;
-  }
+  std::fill_n(table, slot_count, -1);
   return 0;
 }
 

@@ -184,6 +184,21 @@ def test_nothing_changes_when_there_is_no_room(kv):
     assert kv.pages_fork(p.table, p.refs, ringed, 0, 2, 1) == -1
 
 
+def test_release_of_a_page_named_twice(kv):
+    """A sequence may map one page in two slots; where the counts say less than the slots, nothing changes."""
+    p = Pool(kv)
+    p.ensure(0, 0, 12)
+    p.table[0, 3], p.refs[1] = 1, 2
+    assert p.release(0, 0, 4) == 0 and p.consistent() and p.refs.max() == 0
+    p.ensure(0, 0, 12)
+    p.table[0, 3] = 1
+    state = p.table.copy(), p.refs.copy()
+    assert p.release(0, 0, 4) == -1
+    assert np.array_equal(state[0], p.table) and np.array_equal(state[1], p.refs)
+    p.table[0, 2] = 12                                # not a page of the pool
+    assert p.release(0, 0, 3) == -1 and np.array_equal(state[1], p.refs)
+
+
 def test_release_of_the_middle_for_sinks(kv):
     p = Pool(kv)
     p.ensure(0, 0, 24)
