@@ -99,7 +99,8 @@ cudaError_t copy_pages(void *cache_k, void *cache_v, float *scale_k, float *scal
   p.row_bytes = int64_t(c.num_heads) * c.head_dim * element_bytes;
   p.page_bytes = p.row_bytes * c.page_size;
   const int64_t pieces = div_up(p.page_bytes, int64_t(kPieceBytes));
-  if (p.row_bytes % 16 != 0 || pieces > 65535 ||
+  // (16 bytes at a time: an 8-bit row may be an odd number of eights, but eight rows are not)
+  if (int64_t(c.num_heads) * c.head_dim % 8 != 0 || pieces > 65535 ||
       ((reinterpret_cast<uintptr_t>(cache_k) | reinterpret_cast<uintptr_t>(cache_v)) & 15u) != 0) {
     return cudaErrorInvalidValue;
   }

@@ -759,7 +759,8 @@ int32_t b200kv_pages_compact(int32_t *h_page_table, int32_t *h_ref_count,
  * pair's source or destination. Caches are 16-byte aligned, a row (num_heads x
  * head_dim) is a multiple of 8 elements. The fp8 form takes the 8-bit cache of
  * b200kv_decode_append_fp8 with its scales: rows are copied in its blocks of
- * eight (a row count is rounded up), the page's scales with them
+ * eight (a row count is rounded up), the page's scales with them: rows behind them
+ * in the destination keep their codes, which then stand for other values
  * (page_size % 8 == 0; a row count of 0 copies nothing). */
 int b200kv_copy_pages_bf16(b200kv_bf16 *d_cache_k, b200kv_bf16 *d_cache_v,
                            Gemma4KvCacheConfig config, const int32_t *d_src_page,

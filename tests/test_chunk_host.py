@@ -104,6 +104,13 @@ def test_copy_pages_fp8_needs_scales_and_blocks_of_eight(kv):
     assert kv.copy_pages(4096, 4096, cfg, None, None, None, 0, stream=0) == 0
 
 
+def test_copy_pages_refuses_rows_that_are_no_multiple_of_eight_elements(kv):
+    for heads, dim in ((1, 4), (3, 4), (1, 12)):
+        cfg = kv.make_kv_config(2, 40, 16, 10, 4, heads, dim, 0)
+        assert kv.copy_pages_fp8(4096, 4096, 4096, 4096, cfg, 4096, 4096, None, 3, stream=0, check=False) == 1
+        assert kv.copy_pages(4096, 4096, cfg, 4096, 4096, None, 3, stream=0, check=False) == 1
+
+
 # --------------------------------------------------------------------------------------------- page bookkeeping
 class Pool:
     def __init__(self, kv, pages=12, slots=6, batch=3, ps=4, capacity=8):

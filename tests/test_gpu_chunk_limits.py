@@ -193,3 +193,28 @@ def test_a_window_over_a_table_of_all_positions_is_not_refused(kv, own):
     check_attention(case, t)
     a.window_size = a.sink_tokens = 0           # without a window it goes by the table
     assert kv.chunk_attention_launches(a) == 0 and kv.chunk_attention(a, check=False) == 1
+
+
+# --------------------------------------------------------------------------------------------- page copies
+@pytest.mark.parametrize("partial", [False, True])
+@pytest.mark.parametrize("pages,ps,heads,dim,count", [(30, 8, 1, 8, 11), (30, 16, 3, 8, 11), (40, 24, 5, 72, 13)])
+def test_copies_of_8_bit_rows_of_an_odd_number_of_eights(kv, pages, ps, heads, dim, count, partial):
+    """A row is a multiple of 8 elements, of an 8-bit cache as little as 8 bytes."""
+    from tests.test_gpu_chunk_append import copy_case
+
+    cfg, caches, scales = copy_case(kv, 2, pages, ps, heads, dim, True, 4)
+    rng = np.random.default_rng(5)
+    pick = rng.permutation(pages).astype(np.int32)
+    src, dst = pick[:count].copy(), pick[count:2 * count].copy()
+    rows = rng.integers(0, ps + 3, count).astype(np.int32) if partial else None
+    want, want_scales = [c.clone() for c in caches], [s.clone() for s in scales]
+    for i in range(count):
+        n = ps if rows is None else -(-min(int(rows[i]), ps) // 8) * 8
+        for c, s in zip(want, want_scales):
+            c[:, dst[i], :n] = c[:, src[i], :n]
+            if n:
+                s[:, dst[i]] = s[:, src[i]]
+    up = lambda x: None if x is None else torch.from_numpy(x).cuda()  # noqa: E731
+    kv.copy_pages_fp8(*caches, *scales, cfg, up(src), up(dst), up(rows), count)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(caches + scales, want + want_scales))
