@@ -188,6 +188,12 @@ __device__ __forceinline__ bool few_wait(uint32_t bar, uint32_t parity) {
   }
   return true;
 }
+// Gives the copies of tiles j .. end - 1 time to land (out of line: calls never come here).
+__device__ __noinline__ void few_drain(uint32_t bar_full, int j, int end) {
+  for (; j < end; ++j) {
+    mbar_wait_bounded(bar_full + 8u * uint32_t(j % kFewStages), uint32_t(j / kFewStages) & 1u, 1ll << 26);
+  }
+}
 
 // grid (CTAs of a cluster, KV heads, query tiles of the runs). give_up_at: the wait for
 // this key tile counts as run out (-1 but in the self-test).
@@ -440,9 +446,7 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
       // A tile did not come: its copies and those of the next one, asked for above, get the
       // time to land before the CTA gives its shared memory back. A NaN in the sums makes
       // the rows and their log-sum-exp NaN, whichever CTA joins them.
-      for (int i = j; i < min(j + 2, tiles); ++i) {
-        mbar_wait_bounded(bar_full + 8u * uint32_t(i % kFewStages), uint32_t(i / kFewStages) & 1u, 1ll << 26);
-      }
+      few_drain(bar_full, j, min(j + 2, tiles));
       set_status(a.status, B200KV_STATUS_WAIT_TIMEOUT);
       l = __int_as_float(0x7fffffff);
       break;
