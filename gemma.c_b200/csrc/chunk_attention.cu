@@ -47,7 +47,11 @@
 //
 // Keys that no row of the tile sees (before the window, behind the last row, pages
 // that are not mapped) may hold anything: their scores are replaced, and their V
-// rows cleared in shared memory before P V (0 * NaN).
+// rows cleared in shared memory before P V (0 * NaN). A NaN or an infinity in V that some
+// rows of the tile see and others do not is left to the results: a row that is not finite,
+// although its scores are, is computed again from the keys that it sees (chunk_exact.cuh),
+// by the combine. The look at what is written costs 0 to 1 % (ragged runs over rings 98.4 ->
+// 99.2 us, 1024 tokens behind 4096 86.5 -> 87.5).
 //
 // Every wait is bounded; one that runs out writes B200KV_STATUS_WAIT_TIMEOUT and
 // makes the CTA fall through to its exit, which frees the tensor memory.
@@ -78,6 +82,7 @@
 #include <algorithm>
 
 #include "chunk_common.cuh"
+#include "chunk_exact.cuh"
 #include "chunk_maps.cuh"
 #include "kernels.cuh"
 #include "umma_common.cuh"
@@ -118,6 +123,7 @@ constexpr uint32_t kWaitPolls = 1u << 20;     // tens of milliseconds at least; 
 // 115.9 us; least share 2, 4, 8 for four tokens over a ring of 1024: 15.9, 16.1, 20.1.
 constexpr int kItemCost = 8;
 constexpr int kMinShare = 4;
+constexpr int kNotFinite = 4;  // in a meta word's w
 
 template <int kHeadDim_>
 struct ChunkTraits {
@@ -301,8 +307,10 @@ struct SmallState {
   float row_sum[2][kRows];
   int scan[kThreads / 32];
   Walk start;
+  int4 meta;                  // of this CTA, for the combine
   uint32_t tmem_base;
   int abort;
+  int not_finite;             // a row that this CTA has written is not
 };
 
 template <class T>
@@ -460,6 +468,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     mbar_init(bar_drained, 1);
     for (int i = 0; i < kSegments; ++i) mbar_init(bar_seg_full + 8u * i, 1);
     small.abort = 0;
+    small.not_finite = 0;
     mbar_fence_init();
   }
   if (warp == 0) {
@@ -874,7 +883,7 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
     }
     if (ok) tell_segment(0);
     failed = !ok;
-    if (!is_v && lane == 0) p.meta[blockIdx.x] = meta;
+    if (!is_v && lane == 0) small.meta = meta;
     if (!ok || *abort_flag != 0) {
       // nobody may be waiting for the last loads any more: see them land before the
       // CTA gives its shared memory back. The slots before the cursor were filled in
@@ -1277,6 +1286,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
       static_assert(T::kPShared || T::kQHiBytes >= kSoftmaxWarps * 4096, "place for the rows");
       uint8_t *stage = smem_raw + (T::kPShared ? T::kPAt : 0) + (4 * group + quarter) * 4096;
       const int valid = now_rows.rows - 32 * quarter;  // rows of the warp
+      const __nv_bfloat162 none = __floats2bfloat162_rn(0.0f, 0.0f);
+      __nv_bfloat162 odd = none;  // 0 times what is written: NaN if any of it is not finite
 #pragma unroll 1
       for (int h = 0; h < steps; ++h) {
         const int column = 128 * group + step_columns * h;
@@ -1300,6 +1311,11 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
                                   bf16_pair(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
                                   bf16_pair(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
                                   bf16_pair(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+                const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  odd = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&words[j]), none, odd);
+                }
               }
             } else {
               float o[16];
@@ -1341,6 +1357,8 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_o_free);
       }
+      // (a NaN of the sum comes of the scores: the row's own)
+      if (writes && l_row == l_row && pair_not_finite(*reinterpret_cast<const uint32_t *>(&odd))) small.not_finite = 1;
       if (writes && group == 0) {
         if (!whole) {
           piece[p.rows_cap * kPartDims + row] = ref;
@@ -1361,10 +1379,49 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
   }
   tc_fence_before();
   __syncthreads();
+  if (tid == 0) {
+    int4 meta = small.meta;
+    if (small.not_finite != 0) meta.w |= kNotFinite;
+    p.meta[blockIdx.x] = meta;
+  }
   if (warp == 0) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(kTmemColumns)
                  : "memory");
+  }
+}
+
+// Rows that one CTA has written whole, where some are not finite. The combine's blocks of the
+// CTAs that say so look through all rows between them, but for those of items that are
+// joined (their joins look by themselves).
+template <int D>
+__device__ __noinline__ void combine_not_finite(const ChunkParams &p, const ChunkAttentionArgs &a) {
+  const int lane = int(threadIdx.x) & 31;
+  const int parts = D / kPartDims;
+  int ctas = 0, before = 0;  // CTAs that say so, those before this one
+  for (int c = 0; c < int(gridDim.x); c += 32) {
+    const bool says = c + lane < int(gridDim.x) && (p.meta[c + lane].w & kNotFinite) != 0;
+    ctas += __popc(__ballot_sync(0xffffffffu, says));
+    before += __popc(__ballot_sync(0xffffffffu, says && c + lane < int(blockIdx.x)));
+  }
+  const int block_warps = int(blockDim.x) / 32;
+  const int64_t warps = int64_t(ctas) * gridDim.y * block_warps;
+  const int64_t rows = int64_t(a.runs.rows) * a.q_heads * parts;
+  for (int64_t i = (int64_t(before) * gridDim.y + blockIdx.y) * block_warps + threadIdx.x / 32; i < rows; i += warps) {
+    const int part = int(i % parts);
+    const int q_head = int(i / parts % a.q_heads);
+    const int64_t row = i / parts / a.q_heads;
+    const int dims = part * kPartDims + lane * 8;
+    const uint4 v = *reinterpret_cast<const uint4 *>(a.out + (row * a.q_heads + q_head) * D + dims);
+    if (!__any_sync(0xffffffffu, pack_not_finite(v))) continue;
+    bool joined = false;
+    for (int c = lane; c < int(gridDim.x); c += 32) {
+      const int4 meta = p.meta[c];
+      joined |= meta.x == part * p.cfg.num_heads + q_head / p.group && row >= meta.y &&
+                (row - meta.y) * p.group < meta.z;
+    }
+    if (__any_sync(0xffffffffu, joined)) continue;
+    chunk_exact_row<D>(a, p.table_end, row, q_head, dims, true);
   }
 }
 
@@ -1377,7 +1434,9 @@ __global__ __launch_bounds__(kThreads, 1) void chunk_attention_kernel(
 // Bound by the latency of its few dependent loads: the pieces' rows are asked for four
 // at a time, together with what weighs them.
 constexpr int kCombineWarps = 4;
-__global__ __launch_bounds__(kCombineWarps * 32) void chunk_combine_kernel(ChunkParams p, int head_dim) {
+template <int D>
+__global__ __launch_bounds__(kCombineWarps * 32, 8) void chunk_combine_kernel(
+    const __grid_constant__ ChunkParams p, const __grid_constant__ ChunkAttentionArgs a) {
   pdl_wait_for_predecessor();
   const int lane = int(threadIdx.x) & 31;
   const int row = int(blockIdx.y) * kCombineWarps + (int(threadIdx.x) >> 5);
@@ -1385,10 +1444,11 @@ __global__ __launch_bounds__(kCombineWarps * 32) void chunk_combine_kernel(Chunk
   const int cta = int(blockIdx.x);
   const int4 meta = p.meta[cta];
   int state = cta + 1 + lane < ctas ? p.meta[cta + 1 + lane].w : 1;
+  if ((meta.w & kNotFinite) != 0) combine_not_finite<D>(p, a);
   if (meta.x < 0 || row >= meta.z) return;
   int pieces = 1;  // the first and those behind it
   for (int base = cta + 1;;) {
-    const uint32_t end = __ballot_sync(0xffffffffu, state != 2);
+    const uint32_t end = __ballot_sync(0xffffffffu, (state & ~kNotFinite) != 2);
     if (end != 0) {
       pieces += __ffs(int(end));
       break;
@@ -1445,11 +1505,15 @@ __global__ __launch_bounds__(kCombineWarps * 32) void chunk_combine_kernel(Chunk
   const int token = p.group_div.quotient(row);
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   const int64_t at = (int64_t(meta.y) + token) * p.q_heads + head * p.group + (row - token * p.group);
-  reinterpret_cast<uint4 *>(p.out + at * head_dim + part * kPartDims)[lane] =
-      make_uint4(bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv),
-                 bf16_pair(acc[4] * inv, acc[5] * inv), bf16_pair(acc[6] * inv, acc[7] * inv));
+  const uint4 packed = make_uint4(bf16_pair(acc[0] * inv, acc[1] * inv), bf16_pair(acc[2] * inv, acc[3] * inv),
+                                  bf16_pair(acc[4] * inv, acc[5] * inv), bf16_pair(acc[6] * inv, acc[7] * inv));
+  reinterpret_cast<uint4 *>(p.out + at * D + part * kPartDims)[lane] = packed;
   if (p.lse != nullptr && part == 0 && lane == 0) {
     p.lse[at] = l != 0.0f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  }
+  if (l == l && __any_sync(0xffffffffu, pack_not_finite(packed))) {
+    chunk_exact_row<D>(a, p.table_end, int64_t(meta.y) + token, head * p.group + (row - token * p.group),
+                       part * kPartDims + lane * 8, true);
   }
 }
 
@@ -1538,8 +1602,8 @@ cudaError_t launch_chunk(const ChunkAttentionArgs &a, int ctas, cudaStream_t str
                   map_q);
   if (st != cudaSuccess) return st;
   const unsigned row_blocks = unsigned(div_up(p.rows_cap, kCombineWarps));
-  return launch_pdl(chunk_combine_kernel, dim3(unsigned(ctas), row_blocks), dim3(kCombineWarps * 32), 0,
-                    stream, p, int(c.head_dim));
+  return launch_pdl(chunk_combine_kernel<T::kHeadDim>, dim3(unsigned(ctas), row_blocks), dim3(kCombineWarps * 32), 0,
+                    stream, p, a);
 }
 
 }  // namespace

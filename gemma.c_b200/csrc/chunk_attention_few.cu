@@ -30,6 +30,7 @@
 #include <atomic>
 
 #include "chunk_common.cuh"
+#include "chunk_exact.cuh"
 #include "chunk_maps.cuh"
 #include "kernels.cuh"
 
@@ -192,6 +193,18 @@ __device__ __forceinline__ bool few_wait(uint32_t bar, uint32_t parity) {
 __device__ __noinline__ void few_drain(uint32_t bar_full, int j, int end) {
   for (; j < end; ++j) {
     mbar_wait_bounded(bar_full + 8u * uint32_t(j % kFewStages), uint32_t(j / kFewStages) & 1u, 1ll << 26);
+  }
+}
+// This warp's two rows where the lanes of `odd` have a value that is not finite, in the dims
+// that the CTA joins (out of line, too). row0: packed row of the tile's first token.
+template <int D>
+__device__ __noinline__ void few_not_finite(const ChunkAttentionArgs &a, int table_end, int64_t row0, uint32_t odd) {
+  const int group = a.q_heads / a.cfg.num_heads, lane = int(threadIdx.x) & 31;
+  for (int i = 0; i < 2 * (D / 256); ++i) {  // 256 dims at a time
+    if (((odd >> (16 * (i & 1))) & 0xffffu) == 0) continue;
+    const int r = int(threadIdx.x) / 32 * 2 + (i & 1), dims = i / 2 * 256 + lane * 8;
+    chunk_exact_row<D>(a, table_end, row0 + r / group, int(blockIdx.y) * group + r % group, dims,
+                       dims / 16 % int(gridDim.x) == int(blockIdx.x));
   }
 }
 
@@ -539,6 +552,7 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
   for (uint32_t left = 32 * kFewPolls; ok && !try_wait_for_peers(bar_joined); --left) ok = left > 0;
   ok = __all_sync(0xffffffffu, ok);
   // ---- joined: out = sum 2^(m_k - M) O_k / sum 2^(m_k - M) l_k
+  bool odd = false;  // a value is not finite, and not because the scores are not
   if (row < rows) {
     float2 ml = make_float2(-INFINITY, 0.0f);  // of CTA `place`
     if (place < ctas) ml = s.row[place][row];
@@ -564,11 +578,15 @@ __global__ __launch_bounds__(kFewWarps * 32, 1) void chunk_attention_few_kernel(
         acc = fmaf(s.factor[row][k], s.sent[((k * slots + slot) * kFewRows + row) * 16 + place], acc);
       }
       a.out[out * D + (slot * ctas + rank) * 16 + place] = __float2bfloat16_rn(acc);
+      odd |= !(fabsf(acc) < INFINITY);
     }
+    odd = odd && sum == sum;
     if (a.lse != nullptr && rank == 0 && place == 0) {
       a.lse[out] = sum != 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
     }
   }
+  const uint32_t odd_lanes = __ballot_sync(0xffffffffu, odd);
+  if (odd_lanes != 0) few_not_finite<D>(a, table_end, row0, odd_lanes);
   if (!ok) set_status(a.status, B200KV_STATUS_WAIT_TIMEOUT);
 }
 

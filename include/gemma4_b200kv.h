@@ -669,10 +669,10 @@ int b200kv_chunk_append_bf16(const B200KvChunkArgs *args, b200kv_stream stream);
  * sink_tokens (0: none; needs a window) choose it; pages between the sinks and
  * the first row's window may be given back (-1 in the page table). A row that
  * sees no key gets zeros and an lse of -inf. Keys past a linear cache's table do
- * not exist. Values at positions that no row of the call sees are not used,
- * whatever they hold; a NaN or an infinity in V at a position that a later row of
- * the same run sees may reach earlier rows of it too (as 0 * NaN). head_dim 256 or
- * 512, any number G of query heads per KV head up to 64. With P = run_count *
+ * not exist. A NaN or an infinity in K or V is in the results of the rows that see
+ * its position and of no others; rows that share a tile with one in V which they do
+ * not see are computed once more, key by key (slow, in proportion to the keys they
+ * see: a millisecond or so for thousands). head_dim 256 or 512, any number G of query heads per KV head up to 64. With P = run_count *
  * ceil(min(max_row_count, rows) / floor(128 / G)) query tiles: P <= 2^24 and
  * P * kv_heads * (head_dim / 256) * (keys / 64 + 16) < 2^31, keys being the most
  * that a tile of floor(128 / G) tokens can see: the table's positions and, with
