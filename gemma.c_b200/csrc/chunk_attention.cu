@@ -1654,13 +1654,17 @@ cudaError_t validate_chunk_attention(const ChunkAttentionArgs &a) {
   return (align & 15u) == 0 ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// A window of all the positions hides nothing; cut to those, the distance of its start
+// from a key tile behind the row (t - window + 1 - base) fits 32 bits in both kernels.
+static ChunkAttentionArgs with_window_cut(ChunkAttentionArgs a) {
+  a.window = std::min(a.window, kMaxPosition);
+  return a;
+}
+
 cudaError_t chunk_attention_bf16(const ChunkAttentionArgs &given, cudaStream_t stream) {
   const cudaError_t valid = validate_chunk_attention(given);
   if (valid != cudaSuccess) return valid;
-  // A window of all the positions hides nothing; cut to those, the distance of its start
-  // from a key tile behind the row (t - window + 1 - base) fits 32 bits in both kernels.
-  ChunkAttentionArgs a = given;
-  a.window = std::min(a.window, kMaxPosition);
+  const ChunkAttentionArgs a = with_window_cut(given);
   if (a.runs.run_count == 0 || a.runs.rows == 0) return cudaSuccess;
   int device = 0, sms = 0;
   cudaError_t st = cudaGetDevice(&device);
@@ -1696,7 +1700,7 @@ cudaError_t chunk_attention_give_up_selftest(const ChunkAttentionArgs &a, int32_
   cudaError_t st = cudaGetDevice(&device);
   if (st != cudaSuccess) return st;
   bool taken = false;
-  st = chunk_attention_few_bf16(a, device, table_end(a.cfg), stream, &taken, tile);
+  st = chunk_attention_few_bf16(with_window_cut(a), device, table_end(a.cfg), stream, &taken, tile);
   return st != cudaSuccess || taken ? st : cudaErrorInvalidValue;
 }
 

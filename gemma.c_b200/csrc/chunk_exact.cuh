@@ -176,7 +176,7 @@ __device__ __noinline__ void chunk_exact_row(const ChunkAttentionArgs &a, int ta
         acc[i + 1] = fmaf(add, __uint_as_float(words[i / 2] & 0xffff0000u), acc[i + 1] * old);
       }
     }
-    return true;
+    return l == l;  // (a NaN of the scores: so is the row)
   });
 #pragma unroll
   for (int i = 0; i < 8; ++i) {

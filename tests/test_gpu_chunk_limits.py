@@ -133,8 +133,9 @@ def test_rows_of_a_call_that_gives_up_are_nan(kv, name):
     check_attention(case, t)
 
 
-def test_give_up_selftest_of_a_tile_that_no_cta_has(kv):
-    case = make_case(27, [4], [500])
+@pytest.mark.parametrize("window", [0, MOST])
+def test_give_up_selftest_of_a_tile_that_no_cta_has(kv, window):
+    case = make_case(27, [4], [500], window=window)
     a, t = device_args(kv, case)
     kv.chunk_attention_give_up_selftest(a, 1000)
     torch.cuda.synchronize()
