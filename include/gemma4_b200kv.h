@@ -607,8 +607,10 @@ int b200kv_decode_step_plan(const B200KvLayerStepArgs *layers, int32_t layer_cou
  * >= every row_count[i] (it sizes grids and workspace), rows is the number of
  * rows of those tensors. A run whose sequence, position, count or rows are out
  * of range (positions end below 2^31 - 1024), or with no rows, is skipped; rows
- * that no run names are left as they were. The runs of one call must name distinct rows and distinct
- * sequences' positions. run_count <= B200KV_MAX_RUNS.
+ * that no run names are left as they were. The runs of one call must name distinct
+ * rows and distinct positions; two of one sequence only over a linear cache without
+ * k_rows (the later one's attention reads the earlier one's rows from the cache).
+ * No output overlaps an input. run_count <= B200KV_MAX_RUNS.
  *
  * k_rows / v_rows ([rows, kv_heads, head_dim], both or neither):
  *   NULL   the runs' K and V rows live in the cache: the append stores them

@@ -302,3 +302,32 @@ def test_fork_append_attend_release_compact(kv):
     make_copies()
     step([1, 2], [140, 95], [3, 40])
     step([0], [0], [20])
+
+
+@pytest.mark.parametrize("counts", [[4, 3], [70, 200]])
+def test_two_runs_of_one_sequence_in_a_layer_step(kv, counts):
+    """Over a linear cache, without rows beside it: the later run sees the earlier one's rows."""
+    case = make_case(7, [sum(counts)], [90])
+    b, tb = device_args(kv, case)
+    raw = raw_inputs(kv, case, 256, 5)
+    fill(b, raw)
+    b.rotary_dim = 256
+    kv.chunk_layer_step(b)
+    a, t = device_args(kv, case)
+    fill(a, raw)
+    a.rotary_dim = 256
+    runs = {"seq_batch": [0, 0], "first_position": [90, 90 + counts[0]], "row_count": counts, "row_start": [0, counts[0]]}
+    for name, x in runs.items():
+        t[name] = torch.tensor(x, dtype=torch.int32, device="cuda")
+        setattr(a, name, t[name].data_ptr())
+    a.run_count, a.max_row_count = 2, max(counts)
+    size = kv.chunk_workspace_bytes(16, 8, 256, 2, max(counts))
+    t["workspace"] = torch.empty(size, dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = t["workspace"].data_ptr(), size
+    kv.chunk_layer_step(a)
+    torch.cuda.synchronize()
+    bits = lambda x: x.view(torch.int16).reshape(-1)  # noqa: E731
+    for name in ("q", "cache_k", "cache_v"):
+        assert torch.equal(bits(t[name]), bits(tb[name]))
+    case.q, case.cache_k, case.cache_v = t["q"].cpu(), t["cache_k"].cpu(), t["cache_v"].cpu()
+    check_attention(case, t)
