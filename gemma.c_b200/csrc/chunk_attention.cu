@@ -50,8 +50,8 @@
 // rows cleared in shared memory before P V (0 * NaN). A NaN or an infinity in V that some
 // rows of the tile see and others do not is left to the results: a row that is not finite,
 // although its scores are, is computed again from the keys that it sees (chunk_exact.cuh),
-// by the combine. The look at what is written costs 0 to 1 % (ragged runs over rings 98.4 ->
-// 99.2 us, 1024 tokens behind 4096 86.5 -> 87.5).
+// by the combine. The look at what is written costs about 1 % (in a row of calls the ragged
+// runs below 139.8 -> 141.6 us, head_dim 512 295 -> 298).
 //
 // Every wait is bounded; one that runs out writes B200KV_STATUS_WAIT_TIMEOUT and
 // makes the CTA fall through to its exit, which frees the tensor memory.
@@ -63,13 +63,14 @@
 // step) and 2500. An item's start and end cost some 10k clocks in which the tensor pipe
 // has little to do: draining P V (1.1k), reading O back and writing it (4k; 7k the first
 // time, when the code has to be fetched), the first tile's softmax, the masked tiles. Few
-// rows: HBM. Measured (16 + 8 heads of 256 unless said): 4096 tokens behind 12288 0.82 to
-// 0.99 ms by the GPU's power (1160 TFLOP/s at best); 32 runs of 1 .. 8 tokens over 512 ..
-// 12000 keys 261 us, 6.5 TB/s; runs of 239 .. 1211 tokens over rings of 1024 116 us; 64
-// tokens with a window of 2048 and 4 sinks 171 us, 6.3 TB/s; three runs of 406 .. 695
-// tokens of 16 heads of 512 on one KV head 250 us, 760 TFLOP/s. Pages of five tokens (a
-// copy of 16 bytes per lane by one warp, a tile of 64 keys some 5000 clocks): 453, 204,
-// 212 (725 .. 896 tokens, window 2048), 530.
+// rows: HBM. Measured (16 + 8 heads of 256 unless said), in the first fraction of a second
+// and in a row of calls under the power cap: 4096 tokens behind 12288 0.82 and 1.00 ms (1160
+// and 960 TFLOP/s); 32 runs of 1 .. 8 tokens over 512 .. 12000 keys 262 and 283 us (6.5 TB/s
+// at best); runs of 239 .. 1211 tokens over rings of 1024 116 and 141 us; 64 tokens with a
+// window of 2048 and 4 sinks 171 and 188 us; three runs of 406 .. 695 tokens of 16 heads of
+// 512 on one KV head 250 and 298 us. Pages of five tokens (a copy of 16 bytes per lane by
+// one warp, a tile of 64 keys some 5000 clocks), at best: 453, 204, 212 (725 .. 896 tokens,
+// window 2048), 530.
 //
 // The roles share one instruction cache and much of what was tried is about that: waits
 // out of line and rolled MMA and epilogue loops (6000 to 4500 instructions) made the tile

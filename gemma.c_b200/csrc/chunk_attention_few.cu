@@ -19,8 +19,8 @@
 // those have come, and waits for nobody to end. One launch, no partial results in memory.
 //
 // Latency bounds it. Measured, four tokens of 16 + 8 heads of 256 over a ring of 1024
-// (8.4 MB of K and V, 1.3 us of HBM): 7.5 us of the GPU in a row of calls, 15.2 by the
-// other kernel and its join; one token over 100 keys 6.0; over pages of five 7.9 instead
+// (8.4 MB of K and V, 1.3 us of HBM): 7.6 us of the GPU in a row of calls, 15.2 by the
+// other kernel and its join; one token over 100 keys 6.0; over pages of five 8.0 instead
 // of 21.7. Of the way (80 CTAs, 2 tiles each) in clocks: the runs 800, what follows from
 // them 1100, page and first tile 1800, a tile 1500 (of which the first is fetching code),
 // sending and joining 2000. Earlier forms: 64 CTAs with tiles of 32 keys 10.1 us, a bulk
