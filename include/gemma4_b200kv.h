@@ -680,6 +680,7 @@ int b200kv_chunk_append_bf16(const B200KvChunkArgs *args, b200kv_stream stream);
  * that a tile of floor(128 / G) tokens can see: the table's positions and, with
  * k_rows, min(max_row_count, rows), or with a window window_size + sink_tokens +
  * floor(128 / G) - 1 if that is less; larger calls are refused.
+ * `status` tells of a wait that ran out; the call's rows are then not to be used.
  * `workspace` holds the partial results of rows whose keys several CTAs share;
  * it need not be cleared and nothing is kept in it between calls; calls that may
  * overlap on the GPU (two streams, two captured graphs) need one each. */
