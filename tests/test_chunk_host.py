@@ -75,6 +75,17 @@ def test_empty_calls_and_null_blocks(kv):
         assert fn(None, None) == 1
 
 
+def test_give_up_selftest_and_launches_refuse(kv):
+    lib = kv.load_library()
+    assert lib.b200kv_chunk_attention_launches(None) == 0
+    assert lib.b200kv_chunk_attention_give_up_selftest(None, 0, None) == 1
+    for over in (dict(), dict(status=4096, run_count=0), dict(status=4096, out=None)):       # no status; nothing to do; no output
+        assert lib.b200kv_chunk_attention_give_up_selftest(ctypes.byref(args(kv, **over)), 0, None) == 1
+    assert lib.b200kv_chunk_attention_give_up_selftest(ctypes.byref(args(kv, status=4096)), -1, None) == 1
+    for over in (dict(run_count=0), dict(rows=0), dict(out=None)):
+        assert lib.b200kv_chunk_attention_launches(ctypes.byref(args(kv, **over))) == 0
+
+
 def test_workspace_bytes(kv):
     w = lambda *a: kv.chunk_workspace_bytes(*a)  # noqa: E731
     small, large = w(16, 8, 256, 1, 1, 148), w(16, 8, 256, 32, 4096, 148)
